@@ -147,6 +147,36 @@ int nitro_kvpool_data(const nitro_kvpool* pool, float** k_pool, float** v_pool);
 int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* num_layers,
                        int32_t* kv_dim);
 
+/* A pool that holds K and V in 8 bits (no counterpart in the reference; its weights
+ * are held so, src/model_q8.cpp:28-32).  Entry points below take it in place of an
+ * fp32 pool wherever they take rows or attention of it, with n_kv_heads and head_dim
+ * those it was created with; activations stay fp32.  A row x of one K/V head is held
+ * as int8 codes and an fp32 scale of its own: with a = max |x|, scale = a / 127 and
+ * code = rint(x * inv), inv = 127 / a (both quotients fp32, the product exact, ties
+ * to even); the value is code * scale.  Rows with a < 2^-100 are held as zeros.  A
+ * head's row of K or V with an infinity or a NaN in it is held as NaN, K and V both:
+ * every output that attends the token is NaN, no other one is.  Attention works on
+ * the values held, the step's own rows among them.
+ *   Storage: num_pages * num_layers * n_kv_heads records [page][layer][kv_head] of
+ * nitro_kvpool_q8_record_bytes(head_dim) = 32 * hdp + 128 bytes, hdp = head_dim
+ * rounded up to 16: K codes [4][hdp/16][4][16] (token 4a + r, dimension 16c + i at
+ * [a][c][r][i]), V codes [hdp][16] (dimension, token), K scales [16], V scales [16].
+ * create_q8 owns zero-filled memory, wrap_q8 borrows a caller's (16-byte aligned).
+ *   A pool is used on the device that was current when it was made: calls with
+ * another one current are refused.  nitro_kvpool_data and nitro_kvpool_wrap's
+ * buffers do not exist for it (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape reports
+ * kv_dim = n_kv_heads * head_dim. */
+int nitro_kvpool_create_q8(int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
+                           nitro_kvpool** out);
+int nitro_kvpool_wrap_q8(void* cache, int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
+                         nitro_kvpool** out);
+int nitro_kvpool_q8_record_bytes(int32_t head_dim, int32_t* bytes);
+int nitro_kvpool_q8_data(const nitro_kvpool* pool, void** cache);
+/* k, v (device [rows][kv_dim]) = the values an 8-bit pool holds for the rows that
+ * nitro_kv_append / nitro_kv_append_prefill of the uploaded batch write. */
+int nitro_kv_read(nitro_kvpool* pool, int32_t layer, float* k, float* v, void* stream);
+int nitro_kv_read_prefill(nitro_kvpool* pool, int32_t layer, float* k, float* v, void* stream);
+
 /* ----------------------------- decode ------------------------------------
  * The decode batch of forward_decode_batch (src/model_q8.cpp:571-662):
  * host tables[batch][max_pages] and positions[batch] (pos_b = the sequence's

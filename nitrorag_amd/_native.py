@@ -78,6 +78,12 @@ SIGNATURES = {
     "nitro_kvpool_create": [_i32, _i32, _i32, ctypes.POINTER(_vp)],
     "nitro_kvpool_wrap": [_fp, _fp, _i32, _i32, _i32, ctypes.POINTER(_vp)],
     "nitro_kvpool_wrap_contiguous": [_fp, _fp, _i32, _i32, _i32, ctypes.POINTER(_vp)],
+    "nitro_kvpool_create_q8": [_i32, _i32, _i32, _i32, ctypes.POINTER(_vp)],
+    "nitro_kvpool_wrap_q8": [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(_vp)],
+    "nitro_kvpool_q8_record_bytes": [_i32, _i32p],
+    "nitro_kvpool_q8_data": [_vp, ctypes.POINTER(_vp)],
+    "nitro_kv_read": [_vp, _i32, _fp, _fp, _vp],
+    "nitro_kv_read_prefill": [_vp, _i32, _fp, _fp, _vp],
     "nitro_kvpool_destroy": [_vp],
     "nitro_kvpool_data": [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
     "nitro_kvpool_shape": [_vp, _i32p, _i32p, _i32p],

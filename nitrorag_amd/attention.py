@@ -55,8 +55,19 @@ def _host_i32(a) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(a, dtype=np.int64).astype(np.int32))
 
 
+def kv_record_bytes(head_dim: int) -> int:
+    """Bytes that an 8-bit pool holds per page, layer and K/V head."""
+    out = ctypes.c_int32()
+    N.call("nitro_kvpool_q8_record_bytes", head_dim, ctypes.byref(out))
+    return out.value
+
+
 class KVPool:
-    """Device K/V pools with the reference layout, plus the uploaded batches."""
+    """Device K/V pools with the reference layout, plus the uploaded batches.
+
+    KVPool.create_q8 / KVPool.wrap_q8 make a pool that holds K and V as int8
+    codes with an fp32 scale per token and head, a quarter of the bytes (3% of
+    them scales at head size 128); its methods are called as an fp32 pool's."""
 
     def __init__(self, num_pages: int, num_layers: int, kv_dim: int, k=None, v=None,
                  contiguous: bool = False):
@@ -75,6 +86,9 @@ class KVPool:
                 N.call("nitro_kvpool_wrap", _dev(k, "k"), _dev(v, "v"), num_pages, num_layers,
                        kv_dim, ctypes.byref(h))
             self._keep = (k, v)
+        self._set(h, num_pages, num_layers, kv_dim)
+
+    def _set(self, h, num_pages: int, num_layers: int, kv_dim: int):
         self._h = h
         self.num_pages, self.num_layers, self.kv_dim = num_pages, num_layers, kv_dim
         self.decode_batch = 0      # sequences in the uploaded decode batch
@@ -104,6 +118,33 @@ class KVPool:
             raise ValueError("seq_len must be a multiple of 16")
         return cls(seq_len // 16, layers, kv_dim, key_cache, value_cache, contiguous=True)
 
+    @classmethod
+    def create_q8(cls, num_pages: int, num_layers: int, n_kv_heads: int, head_dim: int):
+        """A pool that holds K and V in 8 bits, zero-filled."""
+        self, h = cls.__new__(cls), ctypes.c_void_p()
+        N.call("nitro_kvpool_create_q8", num_pages, num_layers, n_kv_heads, head_dim, ctypes.byref(h))
+        self._keep = None
+        self._set(h, num_pages, num_layers, n_kv_heads * head_dim)
+        return self
+
+    @classmethod
+    def wrap_q8(cls, cache, head_dim: int):
+        """Borrow a uint8 tensor [pages][layers][kv_heads][kv_record_bytes(head_dim)]
+        as a pool that holds K and V in 8 bits."""
+        torch = _torch or _torch_module()
+        if not isinstance(cache, torch.Tensor) or not cache.is_cuda:
+            raise TypeError("cache must be a GPU tensor")
+        if cache.dtype is not torch.uint8 or not cache.is_contiguous():
+            raise TypeError("cache must be contiguous uint8")
+        if cache.dim() != 4 or cache.shape[3] != kv_record_bytes(head_dim):
+            raise ValueError(f"cache must be [pages][layers][kv_heads][{kv_record_bytes(head_dim)}]")
+        self, h = cls.__new__(cls), ctypes.c_void_p()
+        pages, layers, heads, _ = cache.shape
+        N.call("nitro_kvpool_wrap_q8", cache.data_ptr(), pages, layers, heads, head_dim, ctypes.byref(h))
+        self._keep = cache
+        self._set(h, pages, layers, heads * head_dim)
+        return self
+
     @property
     def handle(self):
         return self._h
@@ -119,6 +160,12 @@ class KVPool:
             self.close()
         except Exception:
             pass
+
+    def q8_data_ptr(self) -> int:
+        """Address of an 8-bit pool's records."""
+        p = ctypes.c_void_p()
+        N.call("nitro_kvpool_q8_data", self._h, ctypes.byref(p))
+        return p.value
 
     def data_ptrs(self) -> tuple[int, int]:
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
@@ -139,6 +186,12 @@ class KVPool:
         self._need(k, self.decode_batch * self.kv_dim, "k")
         self._need(v, self.decode_batch * self.kv_dim, "v")
         N.call("nitro_kv_append", self._h, layer, _dev(k, "k"), _dev(v, "v"), _stream_ptr(stream))
+
+    def kv_read(self, layer: int, k, v, stream=None) -> None:
+        """k, v = the values an 8-bit pool holds for the decode batch's new rows."""
+        self._need(k, self.decode_batch * self.kv_dim, "k")
+        self._need(v, self.decode_batch * self.kv_dim, "v")
+        N.call("nitro_kv_read", self._h, layer, _dev(k, "k"), _dev(v, "v"), _stream_ptr(stream))
 
     def decode(self, layer: int, q, out, n_heads: int, n_kv_heads: int, head_dim: int,
                stream=None) -> None:
@@ -176,6 +229,12 @@ class KVPool:
         self._need(v, self.prefill_rows * self.kv_dim, "v")
         N.call("nitro_kv_append_prefill", self._h, layer, _dev(k, "k"), _dev(v, "v"),
                _stream_ptr(stream))
+
+    def kv_read_prefill(self, layer: int, k, v, stream=None) -> None:
+        """k, v = the values an 8-bit pool holds for the prefill batch's rows."""
+        self._need(k, self.prefill_rows * self.kv_dim, "k")
+        self._need(v, self.prefill_rows * self.kv_dim, "v")
+        N.call("nitro_kv_read_prefill", self._h, layer, _dev(k, "k"), _dev(v, "v"), _stream_ptr(stream))
 
     def prefill(self, layer: int, q, out, n_heads: int, n_kv_heads: int, head_dim: int,
                 stream=None) -> None:

@@ -153,6 +153,8 @@ void check_shape(const nitro_kvpool* pool, int layer, int n_heads, int n_kv_head
     require(attention_head_dim(head_dim), ERR_UNSUPPORTED, "head_dim must be a multiple of 4 from 4 to 256");
     require(n_kv_heads * head_dim == pool->kv_dim, ERR_INVALID_ARGUMENT,
             "n_kv_heads * head_dim must equal the pool's kv_dim");
+    require(!pool->q8 || (n_kv_heads == pool->q8_kv_heads && head_dim == pool->q8_head_dim), ERR_INVALID_ARGUMENT,
+            "n_kv_heads and head_dim must be those of the 8-bit pool");
 }
 
 int env_int(const char* name, int fallback) {
@@ -542,9 +544,106 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
     pool->last_stream = s;
 }
 
+// Launch shape of a decode over an 8-bit pool: tiles per split.  One wave takes a
+// tile at a time, a workgroup's waves a split's tiles in turn.
+struct Q8DecodeShape {
+    int waves, tps, groups, cols;
+};
+template <class Ctx>
+Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_heads, int n_kv_heads, int head_dim) {
+    Q8DecodeShape sh;
+    // (four waves' parts of 16 heads of 256 dimensions are more than 64 KB of LDS)
+    sh.waves = kv_q8_padded(head_dim) > 192 ? 2 : 4;
+    const int kv_mul = n_heads / n_kv_heads;
+    sh.cols = std::min(kv_mul, KV_Q8_COLUMNS);
+    sh.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
+    long long tiles = 0;
+    int longest = 1;
+    for (int b = 0; b < B; b++) {
+        const int n = (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE;
+        tiles += n;
+        longest = std::max(longest, n);
+    }
+    const long long resident = 8LL / sh.waves * std::max(pool->num_cus, 1);  // 8 waves per CU
+    const long long each = (tiles * n_kv_heads * sh.groups + resident - 1) / resident;
+    sh.tps = (int)std::min<long long>(longest, (each + sh.waves - 1) / sh.waves * sh.waves);
+    sh.tps = std::max(sh.tps, sh.waves);
+    return sh;
+}
+
+KvQ8Decode q8_decode_args(const nitro_kvpool* pool, int layer, const float* q, float* out, int n_heads,
+                          const Q8DecodeShape& sh) {
+    KvQ8Decode a{};
+    a.c = kv_q8_layer(pool, layer);
+    a.q = q;
+    a.out = out;
+    a.n_heads = n_heads;
+    a.tiles_per_split = sh.tps;
+    a.waves = sh.waves;
+    a.pstride = (a.c.head_dim + 2 + 3) / 4 * 4;
+    a.qscale = (float)(1.4426950408889634 / std::sqrt((double)a.c.head_dim));
+    return a;
+}
+
+// One decode launch over an 8-bit pool's uploaded batch.
+void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out, int n_heads, int n_kv_heads,
+                      int head_dim, hipStream_t s) {
+    DecodeBatch& d = pool->decode;
+    auto ctx = [&](int b) { return d.positions[b] + 1; };
+    const Q8DecodeShape sh = plan_q8_decode(pool, d.batch, ctx, n_heads, n_kv_heads, head_dim);
+    KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh);
+    int longest = 1;
+    for (int b = 0; b < d.batch; b++) longest = std::max(longest, (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE);
+    a.num_splits = (longest + sh.tps - 1) / sh.tps;
+    if (a.num_splits > 1) {
+        pool->partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
+        if (pool->counters.reserve((size_t)d.batch * n_kv_heads * sh.groups))
+            hip_check(hipMemset(pool->counters.ptr, 0, pool->counters.count * sizeof(int32_t)), "hipMemset");
+    }
+    a.tables = d.tables.ptr;
+    a.positions = d.pos.ptr;
+    a.partials = pool->partials.ptr;
+    a.counters = pool->counters.ptr;
+    a.batch = d.batch;
+    a.max_pages = d.max_pages;
+    a.ctx_limit = d.max_pages * BLOCK_SIZE;
+    d.launches++;
+    hip_check(launch_kv_q8_decode(a, s), "kv_q8_decode launch");
+    pool->last_stream = s;
+}
+
+// The rows of the uploaded decode or prefill batch.
+KvQ8Rows q8_decode_rows(const DecodeBatch& d) { return {d.slots.ptr, d.pos.ptr, d.batch}; }
+KvQ8Rows q8_prefill_rows(const PrefillBatch& p) { return {p.slots.ptr, p.row_pos.ptr, p.total_rows}; }
+
+void append_q8(nitro_kvpool* pool, int layer, const KvQ8Rows& rows, float* q, float* k, const float* v,
+               const float* fr, const float* fi, int n_heads, hipStream_t s) {
+    hip_check(launch_kv_q8_append(kv_q8_layer(pool, layer), rows, q, k, v, fr, fi, n_heads, s), "kv_q8_append launch");
+    pool->last_stream = s;
+}
+
 }  // namespace
 
 namespace nitro {
+
+KvQ8 kv_q8_layer(const nitro_kvpool* pool, int layer) {
+    require(pool->q8 != nullptr, ERR_UNSUPPORTED, "the pool does not hold K and V in 8 bits");
+    require(layer >= 0 && layer < pool->num_layers, ERR_INVALID_ARGUMENT, "layer out of range");
+    int device = -1;
+    hip_check(hipGetDevice(&device), "hipGetDevice");
+    require(device == pool->device, ERR_INVALID_ARGUMENT, "the current device is not the pool's");
+    KvQ8 c;
+    c.cache = pool->q8;
+    c.kv_heads = pool->q8_kv_heads;
+    c.head_dim = pool->q8_head_dim;
+    c.hdp = kv_q8_padded(c.head_dim);
+    c.record = kv_q8_record_bytes(c.head_dim);
+    c.layer_off = (int64_t)layer * c.kv_heads * c.record;
+    c.page_stride = (int64_t)pool->num_layers * c.kv_heads * c.record;
+    c.num_pages = pool->num_pages;
+    c.bad_pages = pool->bad_pages.ptr;
+    return c;
+}
 
 void set_device_decode_batch(nitro_kvpool* pool, int batch, int max_pages, const int32_t* positions,
                              bool shared_pages, int32_t** tables, int32_t** device_positions,
@@ -651,6 +750,96 @@ int nitro_kvpool_wrap_contiguous(float* key_cache, float* value_cache, int32_t s
                      seq_len);
 }
 
+static int make_pool_q8(void* cache, bool owned, int32_t num_pages, int32_t num_layers, int32_t n_kv_heads,
+                        int32_t head_dim, nitro_kvpool** out) {
+    return guarded([&] {
+        require(out != nullptr, ERR_INVALID_ARGUMENT, "null output pointer");
+        *out = nullptr;
+        require(num_pages > 0 && num_layers > 0 && n_kv_heads > 0, ERR_INVALID_ARGUMENT,
+                "pool dimensions must be positive");
+        require(attention_head_dim(head_dim), ERR_UNSUPPORTED, "head_dim must be a multiple of 4 from 4 to 256");
+        require((long long)n_kv_heads * head_dim <= INT32_MAX && num_pages <= INT32_MAX / BLOCK_SIZE, ERR_UNSUPPORTED,
+                "a row or the slots do not fit 32 bits");
+        require(owned || (cache != nullptr && (uintptr_t)cache % 16 == 0), ERR_INVALID_ARGUMENT,
+                "the cache must be a 16-byte aligned buffer");
+        nitro_kvpool* pool = new nitro_kvpool();
+        try {
+            hip_check(hipGetDevice(&pool->device), "hipGetDevice");
+            hip_check(hipDeviceGetAttribute(&pool->num_cus, hipDeviceAttributeMultiprocessorCount, pool->device),
+                      "hipDeviceGetAttribute");
+            pool->num_pages = num_pages;
+            pool->num_layers = num_layers;
+            pool->kv_dim = n_kv_heads * head_dim;
+            pool->q8_kv_heads = n_kv_heads;
+            pool->q8_head_dim = head_dim;
+            pool->owned = owned;
+            pool->q8 = static_cast<uint8_t*>(cache);
+            if (owned) {
+                const size_t bytes = (size_t)num_pages * num_layers * n_kv_heads * kv_q8_record_bytes(head_dim);
+                hip_check(hipMalloc((void**)&pool->q8, bytes), "hipMalloc(8-bit K/V pool)");
+                hip_check(hipMemset(pool->q8, 0, bytes), "hipMemset");
+            }
+            pool->bad_pages.reserve(1);
+            hip_check(hipMemset(pool->bad_pages.ptr, 0, sizeof(int32_t)), "hipMemset");
+            hip_check(hipDeviceSynchronize(), "hipDeviceSynchronize");
+        } catch (...) {
+            if (owned && pool->q8) (void)hipFree(pool->q8);
+            delete pool;
+            throw;
+        }
+        *out = pool;
+    });
+}
+
+int nitro_kvpool_create_q8(int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
+                           nitro_kvpool** out) {
+    return make_pool_q8(nullptr, true, num_pages, num_layers, n_kv_heads, head_dim, out);
+}
+
+int nitro_kvpool_wrap_q8(void* cache, int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
+                         nitro_kvpool** out) {
+    return make_pool_q8(cache, false, num_pages, num_layers, n_kv_heads, head_dim, out);
+}
+
+int nitro_kvpool_q8_record_bytes(int32_t head_dim, int32_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, ERR_INVALID_ARGUMENT, "null output pointer");
+        require(attention_head_dim(head_dim), ERR_UNSUPPORTED, "head_dim must be a multiple of 4 from 4 to 256");
+        *bytes = kv_q8_record_bytes(head_dim);
+    });
+}
+
+int nitro_kvpool_q8_data(const nitro_kvpool* pool, void** cache) {
+    return guarded([&] {
+        require_pool(pool);
+        require(cache != nullptr, ERR_INVALID_ARGUMENT, "null output pointer");
+        require(pool->q8 != nullptr, ERR_UNSUPPORTED, "the pool does not hold K and V in 8 bits");
+        *cache = pool->q8;
+    });
+}
+
+static int kv_read(nitro_kvpool* pool, int32_t layer, float* k, float* v, bool prefill, void* stream) {
+    return guarded([&] {
+        require_pool(pool);
+        require(k != nullptr && v != nullptr, ERR_INVALID_ARGUMENT, "null k/v");
+        require((prefill ? pool->prefill.batch : pool->decode.batch) > 0, ERR_NO_BATCH,
+                prefill ? "no prefill batch uploaded" : "no decode batch uploaded");
+        hipStream_t s = as_stream(stream);
+        hip_check(launch_kv_q8_read(kv_q8_layer(pool, layer),
+                                    prefill ? q8_prefill_rows(pool->prefill) : q8_decode_rows(pool->decode), k, v, s),
+                  "kv_q8_read launch");
+        pool->last_stream = s;
+    });
+}
+
+int nitro_kv_read(nitro_kvpool* pool, int32_t layer, float* k, float* v, void* stream) {
+    return kv_read(pool, layer, k, v, false, stream);
+}
+
+int nitro_kv_read_prefill(nitro_kvpool* pool, int32_t layer, float* k, float* v, void* stream) {
+    return kv_read(pool, layer, k, v, true, stream);
+}
+
 int nitro_kvpool_destroy(nitro_kvpool* pool) {
     if (!pool) return NITRO_OK;
     return guarded([&] {
@@ -658,6 +847,7 @@ int nitro_kvpool_destroy(nitro_kvpool* pool) {
         if (pool->owned) {
             (void)hipFree(pool->k);
             (void)hipFree(pool->v);
+            (void)hipFree(pool->q8);
         }
         delete pool;
     });
@@ -666,6 +856,7 @@ int nitro_kvpool_destroy(nitro_kvpool* pool) {
 int nitro_kvpool_data(const nitro_kvpool* pool, float** k_pool, float** v_pool) {
     return guarded([&] {
         require_pool(pool);
+        require(pool->q8 == nullptr, ERR_UNSUPPORTED, "an 8-bit pool has no fp32 buffers");
         if (k_pool) *k_pool = pool->k;
         if (v_pool) *v_pool = pool->v;
     });
@@ -719,6 +910,10 @@ int nitro_kv_append(nitro_kvpool* pool, int32_t layer, const float* k, const flo
         const DecodeBatch& d = pool->decode;
         require(d.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
+        if (pool->q8) {
+            append_q8(pool, layer, q8_decode_rows(d), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            return;
+        }
         hip_check(launch_kv_append_decode(pool->k, pool->v, k, v, d.tables.ptr, d.pos.ptr, d.batch,
                                           d.max_pages, pool->kv_dim, pool->page_stride(),
                                           pool->layer_offset(layer), pool->num_pages,
@@ -735,7 +930,10 @@ int nitro_paged_attn_decode(nitro_kvpool* pool, int32_t layer, const float* q, f
         require(q != nullptr && out != nullptr, ERR_INVALID_ARGUMENT, "null q/out");
         check_shape(pool, layer, n_heads, n_kv_heads, head_dim);
         require(pool->decode.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
-        launch_decode(pool, layer, q, out, nullptr, nullptr, n_heads, n_kv_heads, head_dim, as_stream(stream));
+        if (pool->q8)
+            launch_q8_decode(pool, layer, q, out, n_heads, n_kv_heads, head_dim, as_stream(stream));
+        else
+            launch_decode(pool, layer, q, out, nullptr, nullptr, n_heads, n_kv_heads, head_dim, as_stream(stream));
     });
 }
 
@@ -755,16 +953,7 @@ int nitro_paged_attn_decode_static(nitro_kvpool* pool, int32_t layer, const floa
         // Every sequence is planned at max_context, so the splits are uniform
         // and implied by the block id: no work list, nothing to upload.
         auto ctx = [&](int) { return (int)max_context; };
-        const DecodeShape sh = plan_decode_shape(pool, batch, ctx, n_heads, n_kv_heads, head_dim);
-        const int tile = decode_tile_rows(head_dim);
-        const int splits = ((max_context + tile - 1) / tile + sh.tps - 1) / sh.tps;
-        // page sharing is the caller's to say: plain (cacheable) K/V loads
-        // unless no page is read twice
-        DecodeLaunch a = decode_launch_base(pool, layer, q, out, n_heads, n_kv_heads, head_dim, sh, !pages_private);
-        float* ws = nullptr;
-        if (splits > 1) {
-            const size_t counters = (size_t)batch * (n_heads / sh.qh);
-            const size_t partial_floats = (size_t)batch * splits * n_heads * a.pstride;
+        auto static_scratch = [&](size_t counters, size_t partial_floats) {
             const size_t room = DECODE_STATIC_SCRATCH_BYTES / sizeof(float) - DECODE_STATIC_COUNTERS;
             if (counters > DECODE_STATIC_COUNTERS || partial_floats > room)
                 throw Error(ERR_INVALID_ARGUMENT,
@@ -773,7 +962,38 @@ int nitro_paged_attn_decode_static(nitro_kvpool* pool, int32_t layer, const floa
                                 " bytes of split-K partials; the static workspace holds " +
                                 std::to_string(DECODE_STATIC_COUNTERS) + " and " +
                                 std::to_string(room * sizeof(float)) + " (use nitro_paged_attn_decode)");
+            float* ws = nullptr;
             hip_check(decode_static_scratch(&ws), "hipGetSymbolAddress(scratch)");
+            return ws;
+        };
+        if (pool->q8) {
+            const Q8DecodeShape sh = plan_q8_decode(pool, batch, ctx, n_heads, n_kv_heads, head_dim);
+            KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh);
+            a.num_splits = ((max_context + KV_Q8_TILE - 1) / KV_Q8_TILE + sh.tps - 1) / sh.tps;
+            if (a.num_splits > 1) {
+                float* ws = static_scratch((size_t)batch * n_kv_heads * sh.groups,
+                                           (size_t)batch * a.num_splits * n_heads * a.pstride);
+                a.counters = reinterpret_cast<int32_t*>(ws);
+                a.partials = ws + DECODE_STATIC_COUNTERS;
+            }
+            a.tables = tables;
+            a.positions = positions;
+            a.batch = batch;
+            a.max_pages = max_pages;
+            a.ctx_limit = max_context;
+            hip_check(launch_kv_q8_decode(a, as_stream(stream)), "kv_q8_decode launch");
+            pool->last_stream = as_stream(stream);
+            return;
+        }
+        const DecodeShape sh = plan_decode_shape(pool, batch, ctx, n_heads, n_kv_heads, head_dim);
+        const int tile = decode_tile_rows(head_dim);
+        const int splits = ((max_context + tile - 1) / tile + sh.tps - 1) / sh.tps;
+        // page sharing is the caller's to say: plain (cacheable) K/V loads
+        // unless no page is read twice
+        DecodeLaunch a = decode_launch_base(pool, layer, q, out, n_heads, n_kv_heads, head_dim, sh, !pages_private);
+        float* ws = nullptr;
+        if (splits > 1) {
+            ws = static_scratch((size_t)batch * (n_heads / sh.qh), (size_t)batch * splits * n_heads * a.pstride);
         }
         a.tables = tables;
         a.positions = positions;
@@ -800,6 +1020,11 @@ int nitro_paged_attn_decode_append(nitro_kvpool* pool, int32_t layer, const floa
         const DecodeBatch& d = pool->decode;
         require(d.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
+        if (pool->q8) {
+            append_q8(pool, layer, q8_decode_rows(d), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            launch_q8_decode(pool, layer, q, out, n_heads, n_kv_heads, head_dim, s);
+            return;
+        }
         if (d.new_rows_private || !d.shared_pages) {
             launch_decode(pool, layer, q, out, k, v, n_heads, n_kv_heads, head_dim, s);
         } else {  // another row reads a page being appended to: append first
@@ -948,6 +1173,10 @@ int nitro_kv_append_prefill(nitro_kvpool* pool, int32_t layer, const float* k, c
         const PrefillBatch& p = pool->prefill;
         require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
         hipStream_t s = as_stream(stream);
+        if (pool->q8) {
+            append_q8(pool, layer, q8_prefill_rows(p), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            return;
+        }
         hip_check(launch_kv_scatter_rows(pool->k, pool->v, k, v, p.slots.ptr, p.total_rows,
                                          pool->kv_dim, pool->page_stride(), pool->layer_offset(layer),
                                          pool->num_pages, pool->bad_pages.ptr, s),
@@ -999,9 +1228,37 @@ static PrefillLaunch prefill_args(nitro_kvpool* pool, int32_t layer, const float
     return a;
 }
 
+// One prefill launch over an 8-bit pool's uploaded batch (checked as prefill_args does).
+static void launch_q8_prefill(nitro_kvpool* pool, int32_t layer, const float* q, float* out, int32_t n_heads,
+                              int32_t n_kv_heads, int32_t head_dim, hipStream_t s) {
+    require(q != nullptr && out != nullptr, ERR_INVALID_ARGUMENT, "null q/out");
+    check_shape(pool, layer, n_heads, n_kv_heads, head_dim);
+    const PrefillBatch& p = pool->prefill;
+    require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
+    KvQ8Prefill a{};
+    a.c = kv_q8_layer(pool, layer);
+    a.q = q;
+    a.out = out;
+    a.tables = p.tables.ptr;
+    a.seqs = p.seqs.ptr;
+    a.work = p.work.ptr;
+    a.work_items = p.work_items;
+    a.item_rows = p.work_block_m;
+    a.n_heads = n_heads;
+    a.max_pages = p.max_pages;
+    a.qscale = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+    hip_check(launch_kv_q8_prefill(a, s), "kv_q8_prefill launch");
+    pool->last_stream = s;
+}
+
 int nitro_paged_attn_prefill(nitro_kvpool* pool, int32_t layer, const float* q, float* out,
                              int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, void* stream) {
     return guarded([&] {
+        require_pool(pool);
+        if (pool->q8) {
+            launch_q8_prefill(pool, layer, q, out, n_heads, n_kv_heads, head_dim, as_stream(stream));
+            return;
+        }
         const PrefillLaunch a = prefill_args(pool, layer, q, out, n_heads, n_kv_heads, head_dim);
         hipStream_t s = as_stream(stream);
         hip_check(launch_paged_attn_prefill(a, s), "paged_attn_prefill launch");
@@ -1013,6 +1270,19 @@ int nitro_paged_attn_prefill_append(nitro_kvpool* pool, int32_t layer, const flo
                                     const float* v, float* out, int32_t n_heads, int32_t n_kv_heads,
                                     int32_t head_dim, void* stream) {
     return guarded([&] {
+        require_pool(pool);
+        if (pool->q8) {
+            require(k != nullptr && v != nullptr && q != nullptr && out != nullptr, ERR_INVALID_ARGUMENT,
+                    "null q/k/v/out");
+            check_shape(pool, layer, n_heads, n_kv_heads, head_dim);
+            PrefillBatch& p = pool->prefill;
+            require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
+            p.append_launches++;
+            append_q8(pool, layer, q8_prefill_rows(p), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0,
+                      as_stream(stream));
+            launch_q8_prefill(pool, layer, q, out, n_heads, n_kv_heads, head_dim, as_stream(stream));
+            return;
+        }
         PrefillLaunch a = prefill_args(pool, layer, q, out, n_heads, n_kv_heads, head_dim);
         require(k != nullptr && v != nullptr, ERR_INVALID_ARGUMENT, "null k/v");
         PrefillBatch& p = pool->prefill;
@@ -1066,6 +1336,10 @@ int nitro_rope_kv_append(nitro_kvpool* pool, int32_t layer, float* q, float* k, 
         check_rope(pool, layer, n_heads, n_kv_heads, head_dim, seq_len, max_pos, q, k, v,
                    freq_real, freq_imag);
         hipStream_t s = as_stream(stream);
+        if (pool->q8) {
+            append_q8(pool, layer, q8_decode_rows(d), q, k, v, freq_real, freq_imag, n_heads, s);
+            return;
+        }
         hip_check(launch_rope_kv_append(pool->k, pool->v, q, k, v, freq_real, freq_imag,
                                         d.tables.ptr, d.pos.ptr, nullptr, nullptr, d.batch,
                                         d.max_pages, n_heads * head_dim, pool->kv_dim, head_dim,
@@ -1087,6 +1361,10 @@ int nitro_rope_kv_append_prefill(nitro_kvpool* pool, int32_t layer, float* q, fl
         check_rope(pool, layer, n_heads, n_kv_heads, head_dim, seq_len, p.max_pos, q, k, v,
                    freq_real, freq_imag);
         hipStream_t s = as_stream(stream);
+        if (pool->q8) {
+            append_q8(pool, layer, q8_prefill_rows(p), q, k, v, freq_real, freq_imag, n_heads, s);
+            return;
+        }
         hip_check(launch_rope_kv_append(pool->k, pool->v, q, k, v, freq_real, freq_imag, nullptr,
                                         nullptr, p.slots.ptr, p.row_pos.ptr, p.total_rows,
                                         p.max_pages, n_heads * head_dim, pool->kv_dim, head_dim,

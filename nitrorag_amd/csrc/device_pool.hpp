@@ -9,6 +9,7 @@
 #include <string>
 #include <vector>
 
+#include "kv_q8.hpp"
 #include "paged_memory.hpp"
 
 namespace nitro {
@@ -248,6 +249,10 @@ struct nitro_kvpool {
     int64_t page_elems = 0, layer_elems = 0;
     int64_t page_stride() const { return page_elems; }
     int64_t layer_offset(int layer) const { return (int64_t)layer * layer_elems; }
+
+    // An 8-bit pool (kv_q8.hpp) has its records here and no k / v.
+    uint8_t* q8 = nullptr;
+    int32_t q8_kv_heads = 0, q8_head_dim = 0;
 };
 
 namespace nitro {
@@ -483,6 +488,10 @@ hipError_t launch_paged_attn_prefill(const PrefillLaunch& a, hipStream_t stream)
 }  // namespace nitro
 
 namespace nitro {
+
+// What a launch over a layer of an 8-bit pool is given (throws for another pool,
+// a layer outside it, or a device that is not the pool's).
+KvQ8 kv_q8_layer(const nitro_kvpool* pool, int layer);
 
 // Makes pool->decode a batch whose tables [batch][max_pages] and positions
 // the caller writes on the device (stream-ordered before the next launch);

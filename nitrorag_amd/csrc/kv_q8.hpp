@@ -1,0 +1,81 @@
+// The 8-bit K/V cache: its record and what its kernels are launched with.
+//
+// One record per (page, layer, K/V head), hdp = the head size rounded up to 16:
+//   K codes   int8 [4][hdp/16][4][16]: token 4a + r, dimension 16c + i at
+//             ((a * hdp/16 + c) * 4 + r) * 16 + i
+//   V codes   int8 [hdp][16]: dimension d, token t at d * 16 + t
+//   K scales, V scales   fp32 [16] each, one per token
+// Both orders are those of the integer matrix instructions' operands: a lane's
+// 16 bytes are 16 dimensions of one K row, or the page's 16 tokens of one V
+// column, so attention loads operands straight from the cache.  A scale covers
+// one token of one head: pages fill a token at a time (and a batch may write
+// several tokens of a page at once), and a scale over more tokens would have to
+// be raised, and older codes rounded again, as they arrive.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace nitro {
+
+inline constexpr int kv_q8_padded(int head_dim) { return (head_dim + 15) / 16 * 16; }
+inline constexpr int kv_q8_record_bytes(int head_dim) { return 32 * kv_q8_padded(head_dim) + 128; }
+
+// A layer of an 8-bit cache.
+struct KvQ8 {
+    uint8_t* cache;
+    int64_t page_stride, layer_off;  // bytes
+    int32_t kv_heads, head_dim, hdp, record, num_pages;
+    int32_t* bad_pages;
+};
+
+// New rows of a step: row r lies at position pos[r] in slot slots[r] (page * 16
+// + position % 16).
+struct KvQ8Rows {
+    const int32_t* slots;
+    const int32_t* pos;
+    int32_t rows;
+};
+
+// Appends k, v [rows][kv_heads * head_dim].  With freq_real, q [rows][n_heads *
+// head_dim] and k are first rotated in place.
+hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v,
+                               const float* freq_real, const float* freq_imag, int n_heads, hipStream_t stream);
+// k, v = the values that those slots hold.
+hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v, hipStream_t stream);
+
+// Keys that a wave takes at a time: four pages.
+constexpr int KV_Q8_TILE = 64;
+// Query heads of one K/V head that a decode workgroup serves at most (the
+// columns of its matrix instructions).
+constexpr int KV_Q8_COLUMNS = 16;
+
+struct KvQ8Decode {
+    KvQ8 c;
+    const float* q;
+    float* out;
+    const int32_t* tables;
+    const int32_t* positions;
+    float* partials;    // per (b, split, head): acc[head_dim], m, l; pstride floats
+    int32_t* counters;  // per (b, K/V head, group of its query heads), zero between launches
+    int32_t batch, n_heads, max_pages, ctx_limit;
+    int32_t tiles_per_split, num_splits, waves, pstride;
+    float qscale;  // log2(e) / sqrt(head_dim)
+};
+hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream);
+
+struct PrefillSeq;
+struct KvQ8Prefill {
+    KvQ8 c;
+    const float* q;
+    float* out;
+    const int32_t* tables;
+    const PrefillSeq* seqs;
+    const int32_t* work;  // pairs (seq, first query row of the chunk)
+    int32_t work_items, item_rows, n_heads, max_pages;
+    float qscale;
+};
+hipError_t launch_kv_q8_prefill(const KvQ8Prefill& a, hipStream_t stream);
+
+}  // namespace nitro

@@ -111,6 +111,7 @@ void check_model_pool(const nitro_model* m, const nitro_kvpool* pool) {
     require(pool != nullptr, ERR_INVALID_ARGUMENT, "null pool");
     require(pool->num_layers == m->n_layers && pool->kv_dim == m->kv_dim, ERR_INVALID_ARGUMENT,
             "pool layers / kv_dim do not match the model");
+    require(pool->q8 == nullptr, ERR_UNSUPPORTED, "a model steps over an fp32 pool");
 }
 
 void upload_tokens(nitro_model* m, const int32_t* tokens, int rows, hipStream_t s) {

@@ -1,0 +1,115 @@
+"""Plain 64-bit restatement of the 8-bit K/V cache: its records, the rows put into
+them, and attention over the values they hold (numpy; test infrastructure only).
+The reference has no 8-bit K/V cache: this follows the definition in
+include/nitro_paged_attn.h."""
+from __future__ import annotations
+
+import numpy as np
+
+PAGE = 16
+LEAST = 2.0 ** -100
+
+
+def padded(head_dim: int) -> int:
+    return (head_dim + 15) // 16 * 16
+
+
+def record_bytes(head_dim: int) -> int:
+    return 32 * padded(head_dim) + 8 * PAGE
+
+
+def rotate(x, cos, sin):
+    """x [rows][heads][head_dim], cos / sin [rows][head_dim/2] fp32 -> fp32."""
+    a, b = x[..., 0::2].astype(np.float64), x[..., 1::2].astype(np.float64)
+    c, s = cos[:, None].astype(np.float64), sin[:, None].astype(np.float64)
+    out = np.empty(x.shape, np.float32)
+    out[..., 0::2] = (a * c - b * s).astype(np.float32)
+    out[..., 1::2] = (a * s + b * c).astype(np.float32)
+    return out
+
+
+def quantise(k, v):
+    """(k codes, k scales, v codes, v scales) of fp32 rows [...][head_dim]."""
+    with np.errstate(all="ignore"):
+        finite = np.isfinite(k).all(-1) & np.isfinite(v).all(-1)
+        got = []
+        for x in (k, v):
+            top = np.where(finite, np.abs(x).max(-1), 0).astype(np.float32)
+            live = top >= np.float32(LEAST)
+            safe = np.where(live, top, np.float32(1))
+            inverse = np.where(live, np.float32(127) / safe, np.float32(0)).astype(np.float32)
+            scale = np.where(live, safe / np.float32(127), np.float32(0)).astype(np.float32)
+            exact = np.where(finite[..., None], x, 0).astype(np.float64) * inverse[..., None].astype(np.float64)
+            got += [np.rint(exact).astype(np.int8), np.where(finite, scale, np.float32("nan")).astype(np.float32)]
+        return tuple(got)
+
+
+class Cache:
+    """Records [pages][layers][kv_heads][record_bytes] as one uint8 array."""
+
+    def __init__(self, data, head_dim):
+        self.data, self.hd, self.hdp = data, head_dim, padded(head_dim)
+
+    def _places(self, token):
+        """Byte offsets of a token's K codes and V codes for each padded dimension."""
+        d = np.arange(self.hdp)
+        return ((token // 4 * (self.hdp // 16) + d // 16) * 4 + token % 4) * 16 + d % 16, 16 * self.hdp + d * PAGE + token
+
+    def put(self, layer, slots, k, v):
+        """Rows k, v [rows][kv_heads][head_dim] into slots (page * 16 + token)."""
+        kc, ks, vc, vs = quantise(k, v)
+        pad = ((0, 0), (0, self.hdp - self.hd))
+        for r, slot in enumerate(slots):
+            page, t = divmod(int(slot), PAGE)
+            at_k, at_v = self._places(t)
+            rec = self.data[page, layer]
+            rec[:, at_k] = np.pad(kc[r], pad).view(np.uint8)
+            rec[:, at_v] = np.pad(vc[r], pad).view(np.uint8)
+            for base, s in ((0, ks[r]), (64, vs[r])):
+                at = 32 * self.hdp + base + 4 * t
+                rec[:, at:at + 4] = s[:, None].view(np.uint8)
+
+    def values(self, layer, table, tokens):
+        """K and V of a sequence's first `tokens` tokens, float64 [tokens][kv_heads][head_dim]."""
+        k = np.empty((tokens, self.data.shape[2], self.hd))
+        v = np.empty_like(k)
+        with np.errstate(invalid="ignore"):
+            for t in range(PAGE):
+                which = np.arange(t, tokens, PAGE)
+                if not which.size:
+                    continue
+                rec = self.data[np.asarray(table)[which // PAGE], layer]  # [n][kv_heads][record]
+                at_k, at_v = self._places(t)
+                s = np.ascontiguousarray(rec[:, :, 32 * self.hdp:]).view(np.float32).astype(np.float64)
+                k[which] = rec[:, :, at_k[:self.hd]].view(np.int8) * s[:, :, t, None]
+                v[which] = rec[:, :, at_v[:self.hd]].view(np.int8) * s[:, :, 16 + t, None]
+        return k, v
+
+
+def attention(q, positions, k, v):
+    """q [rows][heads][hd] at `positions` over keys 0..position; with a bound on what
+    fp32 arithmetic with 24-bit fixed point may be off, elementwise [rows][heads][1].
+
+    The bound: an entry of q is off by at most 6e-8 of its row's largest (half a unit
+    of 1/8355000), so a score is off by that times the key's 1-norm; fp32 rounds it
+    about six times (conversions, the two factors, the sum of the digits, the
+    difference from the maximum).  A weight is then off by that, relative, and 2^-22
+    (exp2, its sum).  As numerator and denominator: twice.  The weights' own
+    fixed point: at most 64 half units per tile of the tile's largest, whose sum over
+    tiles is at most the denominator.  Joining the tiles: two roundings each."""
+    rows, heads, hd = q.shape
+    out, bound = np.empty((rows, heads, hd)), np.empty((rows, heads, 1))
+    per = heads // k.shape[1]
+    for r in range(rows):
+        n = int(positions[r]) + 1
+        for h in range(heads):
+            kh, vh = k[:n, h // per], v[:n, h // per]
+            x = q[r, h].astype(np.float64)
+            s = kh @ x / np.sqrt(hd)
+            p = np.exp(s - s.max())
+            out[r, h] = p @ vh / p.sum()
+            off = np.abs(x).max() * 6e-8 * np.abs(kh).sum(-1).max() / np.sqrt(hd) + 6 * 2.0 ** -24 * np.abs(s).max()
+            weight = off + 2.0 ** -22
+            tiles = (n + 63) // 64
+            bound[r, h] = np.abs(vh).max() * (2 * weight + 64 * 6e-8 + (2 * tiles + 20) * 2.0 ** -24) + 1e-30
+    return out, bound
