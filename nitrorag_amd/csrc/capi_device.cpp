@@ -613,13 +613,26 @@ void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out,
 }
 
 // The rows of the uploaded decode or prefill batch.
-KvQ8Rows q8_decode_rows(const DecodeBatch& d) { return {d.slots.ptr, d.pos.ptr, d.batch}; }
-KvQ8Rows q8_prefill_rows(const PrefillBatch& p) { return {p.slots.ptr, p.row_pos.ptr, p.total_rows}; }
+KvQ8Rows q8_rows(const nitro_kvpool* pool, bool prefill) {
+    const DecodeBatch& d = pool->decode;
+    const PrefillBatch& p = pool->prefill;
+    return prefill ? KvQ8Rows{p.slots.ptr, p.row_pos.ptr, p.total_rows} : KvQ8Rows{d.slots.ptr, d.pos.ptr, d.batch};
+}
+KvQ8Chunks q8_chunks(const nitro_kvpool* pool, bool prefill) {
+    const PrefillBatch& p = pool->prefill;
+    return prefill ? KvQ8Chunks{p.seqs.ptr, p.work.ptr, p.work_items, p.work_block_m} : KvQ8Chunks{};
+}
 
-void append_q8(nitro_kvpool* pool, int layer, const KvQ8Rows& rows, float* q, float* k, const float* v,
-               const float* fr, const float* fi, int n_heads, hipStream_t s) {
-    hip_check(launch_kv_q8_append(kv_q8_layer(pool, layer), rows, q, k, v, fr, fi, n_heads, s), "kv_q8_append launch");
+// Appends the batch's rows (fr, fi: after rotating q and k).
+void append_q8(nitro_kvpool* pool, int layer, bool prefill, float* q, float* k, const float* v, const float* fr,
+               const float* fi, int n_heads, hipStream_t s) {
+    hip_check(launch_kv_q8_append(kv_q8_layer(pool, layer), q8_rows(pool, prefill), q8_chunks(pool, prefill), q, k, v, fr,
+                                  fi, n_heads, s),
+              "kv_q8_append launch");
     pool->last_stream = s;
+}
+void append_q8(nitro_kvpool* pool, int layer, bool prefill, const float* k, const float* v, hipStream_t s) {
+    append_q8(pool, layer, prefill, nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);  // k is only read
 }
 
 }  // namespace
@@ -825,8 +838,7 @@ static int kv_read(nitro_kvpool* pool, int32_t layer, float* k, float* v, bool p
         require((prefill ? pool->prefill.batch : pool->decode.batch) > 0, ERR_NO_BATCH,
                 prefill ? "no prefill batch uploaded" : "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
-        hip_check(launch_kv_q8_read(kv_q8_layer(pool, layer),
-                                    prefill ? q8_prefill_rows(pool->prefill) : q8_decode_rows(pool->decode), k, v, s),
+        hip_check(launch_kv_q8_read(kv_q8_layer(pool, layer), q8_rows(pool, prefill), q8_chunks(pool, prefill), k, v, s),
                   "kv_q8_read launch");
         pool->last_stream = s;
     });
@@ -911,7 +923,7 @@ int nitro_kv_append(nitro_kvpool* pool, int32_t layer, const float* k, const flo
         require(d.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
         if (pool->q8) {
-            append_q8(pool, layer, q8_decode_rows(d), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            append_q8(pool, layer, false, k, v, s);
             return;
         }
         hip_check(launch_kv_append_decode(pool->k, pool->v, k, v, d.tables.ptr, d.pos.ptr, d.batch,
@@ -1021,7 +1033,7 @@ int nitro_paged_attn_decode_append(nitro_kvpool* pool, int32_t layer, const floa
         require(d.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
         if (pool->q8) {
-            append_q8(pool, layer, q8_decode_rows(d), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            append_q8(pool, layer, false, k, v, s);
             launch_q8_decode(pool, layer, q, out, n_heads, n_kv_heads, head_dim, s);
             return;
         }
@@ -1174,7 +1186,7 @@ int nitro_kv_append_prefill(nitro_kvpool* pool, int32_t layer, const float* k, c
         require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
         hipStream_t s = as_stream(stream);
         if (pool->q8) {
-            append_q8(pool, layer, q8_prefill_rows(p), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0, s);
+            append_q8(pool, layer, true, k, v, s);
             return;
         }
         hip_check(launch_kv_scatter_rows(pool->k, pool->v, k, v, p.slots.ptr, p.total_rows,
@@ -1278,8 +1290,7 @@ int nitro_paged_attn_prefill_append(nitro_kvpool* pool, int32_t layer, const flo
             PrefillBatch& p = pool->prefill;
             require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
             p.append_launches++;
-            append_q8(pool, layer, q8_prefill_rows(p), nullptr, const_cast<float*>(k), v, nullptr, nullptr, 0,
-                      as_stream(stream));
+            append_q8(pool, layer, true, k, v, as_stream(stream));
             launch_q8_prefill(pool, layer, q, out, n_heads, n_kv_heads, head_dim, as_stream(stream));
             return;
         }
@@ -1337,7 +1348,7 @@ int nitro_rope_kv_append(nitro_kvpool* pool, int32_t layer, float* q, float* k, 
                    freq_real, freq_imag);
         hipStream_t s = as_stream(stream);
         if (pool->q8) {
-            append_q8(pool, layer, q8_decode_rows(d), q, k, v, freq_real, freq_imag, n_heads, s);
+            append_q8(pool, layer, false, q, k, v, freq_real, freq_imag, n_heads, s);
             return;
         }
         hip_check(launch_rope_kv_append(pool->k, pool->v, q, k, v, freq_real, freq_imag,
@@ -1362,7 +1373,7 @@ int nitro_rope_kv_append_prefill(nitro_kvpool* pool, int32_t layer, float* q, fl
                    freq_real, freq_imag);
         hipStream_t s = as_stream(stream);
         if (pool->q8) {
-            append_q8(pool, layer, q8_prefill_rows(p), q, k, v, freq_real, freq_imag, n_heads, s);
+            append_q8(pool, layer, true, q, k, v, freq_real, freq_imag, n_heads, s);
             return;
         }
         hip_check(launch_rope_kv_append(pool->k, pool->v, q, k, v, freq_real, freq_imag, nullptr,

@@ -38,12 +38,22 @@ struct KvQ8Rows {
     int32_t rows;
 };
 
+struct PrefillSeq;
+// The same rows as chunks of sequences, in items of item_rows consecutive rows.
+struct KvQ8Chunks {
+    const PrefillSeq* seqs = nullptr;
+    const int32_t* work = nullptr;  // pairs (seq, first row of the item in its chunk)
+    int32_t work_items = 0, item_rows = 0;
+};
+
 // Appends k, v [rows][kv_heads * head_dim].  With freq_real, q [rows][n_heads *
-// head_dim] and k are first rotated in place.
-hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v,
-                               const float* freq_real, const float* freq_imag, int n_heads, hipStream_t stream);
+// head_dim] and k are first rotated in place.  chunks: the rows are also these.
+hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& chunks, float* q, float* k,
+                               const float* v, const float* freq_real, const float* freq_imag, int n_heads,
+                               hipStream_t stream);
 // k, v = the values that those slots hold.
-hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v, hipStream_t stream);
+hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& chunks, float* k, float* v,
+                             hipStream_t stream);
 
 // Keys that a wave takes at a time: four pages.
 constexpr int KV_Q8_TILE = 64;
@@ -65,7 +75,6 @@ struct KvQ8Decode {
 };
 hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream);
 
-struct PrefillSeq;
 struct KvQ8Prefill {
     KvQ8 c;
     const float* q;

@@ -27,11 +27,42 @@ namespace {
 constexpr int THREADS = 256;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
+constexpr float LEAST = 0x1p-100f;
+
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(dpp<CTRL>(__float_as_int(x)));
+}
+// A lane's partner l ^ M within 16 lanes.
+template <int M>
+__device__ __forceinline__ int from_xor(int x) {
+    if constexpr (M == 1) return dpp<0xB1>(x);                // quad_perm [1,0,3,2]
+    if constexpr (M == 2) return dpp<0x4E>(x);                // quad_perm [2,3,0,1]
+    if constexpr (M == 4) return dpp<0x1B>(dpp<0x141>(x));    // row_half_mirror (l ^ 7), then quad_perm [3,2,1,0]
+    return dpp<0x128>(x);                                     // row_ror:8
+}
+__device__ __forceinline__ float max_across_16(float x) {  // l, l ^ 16
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_across_32(float x) {  // l, l ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Maximum of x over the LPH (16, 32, 64) lanes that hold a head's row.
 template <int LPH>
 __device__ __forceinline__ float head_max(float x) {
-#pragma unroll
-    for (int d = 1; d < LPH; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));  // row_half_mirror: the other four of eight
+    x = fmaxf(x, dpp<0x140>(x));  // row_mirror: the other eight of sixteen
+    if constexpr (LPH >= 32) x = max_across_16(x);
+    if constexpr (LPH >= 64) x = max_across_32(x);
     return x;
 }
 
@@ -60,8 +91,15 @@ __device__ __forceinline__ float abs_max(f4 x) {
 // 0, or NaN where x holds an infinity or a NaN (which a maximum would drop).
 __device__ __forceinline__ float poison(f4 x) { return (x.x * 0.0f + x.y * 0.0f) + (x.z * 0.0f + x.w * 0.0f); }
 
-// A unit is one head of one row: query heads first (rotation only), then K/V
-// heads.  LPH lanes hold a unit, four dimensions each.
+// What a page's or row's scale and inverse are, from the largest magnitude; a row
+// that is not good is held as NaN.
+__device__ __forceinline__ float inverse_of(float top, bool good) { return good && top >= LEAST ? 127.0f / top : 0.0f; }
+__device__ __forceinline__ float scale_of(float top, bool good) {
+    return !good ? __uint_as_float(0x7fc00000u) : top >= LEAST ? top / 127.0f : 0.0f;
+}
+
+// Rows anywhere (a decode batch).  A unit is one head of one row: query heads first
+// (rotation only), then K/V heads.  LPH lanes hold a unit, four dimensions each.
 template <int LPH, bool ROPE>
 __global__ __launch_bounds__(THREADS) void kv_q8_append_kernel(KvQ8 c, KvQ8Rows rows, float* __restrict__ q,
                                                                float* __restrict__ k, const float* __restrict__ v,
@@ -70,62 +108,50 @@ __global__ __launch_bounds__(THREADS) void kv_q8_append_kernel(KvQ8 c, KvQ8Rows 
     const int units = (ROPE ? n_heads : 0) + c.kv_heads;
     const int64_t total = (int64_t)rows.rows * units;
     const int lane = threadIdx.x % LPH, dim = lane * 4;
+    const bool in = dim < c.head_dim;
     for (int64_t u = (int64_t)blockIdx.x * (THREADS / LPH) + threadIdx.x / LPH; u < total;
          u += (int64_t)gridDim.x * (THREADS / LPH)) {
         const int row = (int)(u / units);
         int h = (int)(u - (int64_t)row * units);
-        const bool in = dim < c.head_dim;
-        const float *fr = nullptr, *fi = nullptr;
-        if (ROPE && in) {
-            const int64_t at = (int64_t)rows.pos[row] * (c.head_dim / 2) + dim / 2;
-            fr = freq_real + at;
-            fi = freq_imag + at;
-        }
-        if (ROPE && h < n_heads) {
-            if (in) {
-                f4* at = reinterpret_cast<f4*>(q + ((int64_t)row * n_heads + h) * c.head_dim + dim);
-                *at = rotated(*at, fr, fi);
-            }
-            continue;
-        }
-        if (ROPE) h -= n_heads;
-        f4 kx = {0.f, 0.f, 0.f, 0.f}, vx = kx;
+        const bool query = ROPE && h < n_heads;
+        if (ROPE && !query) h -= n_heads;
+        // every load that waits for nothing, then the angles, which wait for the position
+        const int pos = ROPE ? rows.pos[row] : 0, slot = rows.slots[row];
+        float* const x_at = query ? q + ((int64_t)row * n_heads + h) * c.head_dim + dim
+                                  : k + ((int64_t)row * c.kv_heads + h) * c.head_dim + dim;
+        f4 x = {0.f, 0.f, 0.f, 0.f}, vx = x;
         if (in) {
-            const int64_t at = ((int64_t)row * c.kv_heads + h) * c.head_dim + dim;
-            kx = *reinterpret_cast<const f4*>(k + at);
-            vx = *reinterpret_cast<const f4*>(v + at);
+            x = *reinterpret_cast<const f4*>(x_at);
+            if (!query) vx = *reinterpret_cast<const f4*>(v + ((int64_t)row * c.kv_heads + h) * c.head_dim + dim);
             if (ROPE) {
-                kx = rotated(kx, fr, fi);
-                *reinterpret_cast<f4*>(k + at) = kx;
+                const int64_t at = (int64_t)pos * (c.head_dim / 2) + dim / 2;
+                x = rotated(x, freq_real + at, freq_imag + at);
+                *reinterpret_cast<f4*>(x_at) = x;
             }
         }
-        const float ka = head_max<LPH>(abs_max(kx)), va = head_max<LPH>(abs_max(vx));
-        const bool good = head_max<LPH>(poison(kx) + poison(vx) == 0.0f ? 0.0f : 1.0f) == 0.0f;
-        const int slot = rows.slots[row];
+        if (query) continue;  // (all the lanes of a unit)
+        const float ka = head_max<LPH>(abs_max(x)), va = head_max<LPH>(abs_max(vx));
+        const bool good = head_max<LPH>(poison(x) + poison(vx) == 0.0f ? 0.0f : 1.0f) == 0.0f;
         const int page = slot >> 4, t = slot & 15;
         if (slot < 0 || page >= c.num_pages) {
             if (lane == 0 && h == 0) atomicAdd(c.bad_pages, 1);
             continue;
         }
-        constexpr float LEAST = 0x1p-100f;
-        const float nan = __uint_as_float(0x7fc00000u);
-        const uint32_t kc = codes_of(kx, good && ka >= LEAST ? 127.0f / ka : 0.0f);
-        const uint32_t vc = codes_of(vx, good && va >= LEAST ? 127.0f / va : 0.0f);
+        const uint32_t kc = good ? codes_of(x, inverse_of(ka, good)) : 0, vc = good ? codes_of(vx, inverse_of(va, good)) : 0;
         uint8_t* rec = c.cache + (int64_t)page * c.page_stride + c.layer_off + (int64_t)h * c.record;
         if (dim < c.hdp) {
             const int at = (((t >> 2) * (c.hdp >> 4) + (dim >> 4)) * 4 + (t & 3)) * 16 + (dim & 15);
-            *reinterpret_cast<uint32_t*>(rec + at) = good ? kc : 0;
+            *reinterpret_cast<uint32_t*>(rec + at) = kc;
             uint8_t* vb = rec + 16 * c.hdp + dim * 16 + t;
-            const uint32_t w = good ? vc : 0;
-            vb[0] = (uint8_t)w;
-            vb[16] = (uint8_t)(w >> 8);
-            vb[32] = (uint8_t)(w >> 16);
-            vb[48] = (uint8_t)(w >> 24);
+            vb[0] = (uint8_t)vc;
+            vb[16] = (uint8_t)(vc >> 8);
+            vb[32] = (uint8_t)(vc >> 16);
+            vb[48] = (uint8_t)(vc >> 24);
         }
         if (lane == 0) {
             float* s = reinterpret_cast<float*>(rec + 32 * c.hdp);
-            s[t] = !good ? nan : ka >= LEAST ? ka / 127.0f : 0.0f;
-            s[16 + t] = !good ? nan : va >= LEAST ? va / 127.0f : 0.0f;
+            s[t] = scale_of(ka, good);
+            s[16 + t] = scale_of(va, good);
         }
     }
 }
@@ -159,14 +185,259 @@ __global__ __launch_bounds__(THREADS) void kv_q8_read_kernel(KvQ8 c, KvQ8Rows ro
     }
 }
 
+// -------------------------------------------------------------- whole pages
+//
+// Rows of chunks lie together, up to 16 of one sequence to a page.  A wave takes
+// one K/V head of one page: lane (tq = lane % 4, dg = lane / 4) holds four tokens
+// (4 tq ..) of dimensions 64 j + 4 dg ..+ 4.  That makes both operand orders whole
+// 16-byte runs after a 4 x 4 exchange: K among the lanes dg % 4 (16 dimensions of
+// one token each), V among tq (the 16 tokens of one dimension each, after the
+// bytes of a lane's own 4 x 4 are turned).  A byte of V at a time, as the kernel
+// above writes it, took 815 us for 16384 rows of 32 heads of 128.
+
+__device__ __forceinline__ int pick(bool c, int a, int b) { return c ? a : b; }
+
+// x[j] of lane i of four = x[i] of lane j; the four differ in bits A and 2A (A = 1
+// or 4) of the lane.
+template <int A>
+__device__ __forceinline__ void exchange(int (&x)[4], int lane) {
+    const bool lo = lane & A, hi = lane & (2 * A);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const int got = from_xor<A>(pick(lo, x[i], x[i + 1]));
+        x[i] = pick(lo, got, x[i]);
+        x[i + 1] = pick(lo, x[i + 1], got);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int got = from_xor<2 * A>(pick(hi, x[i], x[i + 2]));
+        x[i] = pick(hi, got, x[i]);
+        x[i + 2] = pick(hi, x[i + 2], got);
+    }
+}
+// Byte r of x[i] <-> byte i of x[r].
+__device__ __forceinline__ void turn_bytes(int (&x)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+    x[0] = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
+    x[1] = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+    x[2] = (int)__builtin_amdgcn_perm(d, c, 0x05040100u);
+    x[3] = (int)__builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+__device__ __forceinline__ float page_max(float x) {  // over dg
+    x = fmaxf(x, dpp<0x124>(x));                      // row_ror:4
+    x = fmaxf(x, dpp<0x128>(x));                      // row_ror:8
+    return max_across_32(max_across_16(x));
+}
+
+// Where a wave's page lies: its rows are first .. first + count - 1 of the packed
+// ones, tokens t0 .. t0 + count - 1 of the page.
+struct PageRows {
+    int first, count, t0, page;
+};
+// Page `which` (0 .. item_rows / 16) of an item: the pages whose first row of the
+// chunk is one of the item's rows.  count = 0: the item has no such page.
+__device__ __forceinline__ PageRows page_rows(const KvQ8Rows& rows, const KvQ8Chunks& ch, int item, int which) {
+    const PrefillSeq seq = ch.seqs[ch.work[2 * item]];
+    const int q0 = ch.work[2 * item + 1];
+    const int page = (q0 == 0 ? seq.start_pos : seq.start_pos + q0 + 15) / 16 + which;
+    const int from = max(page * 16 - seq.start_pos, 0);  // in the chunk
+    PageRows p{0, 0, 0, 0};
+    if (from >= min(seq.num_tokens, q0 + ch.item_rows)) return p;
+    p.first = seq.row_off + from;
+    const int slot = rows.slots[p.first];
+    p.t0 = slot & 15;
+    p.page = slot >> 4;
+    p.count = min(16 - p.t0, seq.num_tokens - from);
+    return p;
+}
+
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+// J = hdp / 64, rounded up.  Workgroups past page_blocks rotate q.
+template <int J, bool ROPE>
+__global__ __launch_bounds__(THREADS) void kv_q8_append_pages_kernel(KvQ8 c, KvQ8Rows rows, KvQ8Chunks ch,
+                                                                     float* __restrict__ q, float* __restrict__ k,
+                                                                     const float* __restrict__ v,
+                                                                     const float* __restrict__ freq_real,
+                                                                     const float* __restrict__ freq_imag, int n_heads,
+                                                                     unsigned page_blocks) {
+    if (ROPE && blockIdx.x >= page_blocks) {
+        const int per_row = n_heads * c.head_dim / 4;  // float4
+        const int64_t total = (int64_t)rows.rows * per_row;
+        for (int64_t i = (int64_t)(blockIdx.x - page_blocks) * THREADS + threadIdx.x; i < total;
+             i += (int64_t)(gridDim.x - page_blocks) * THREADS) {
+            const int row = (int)(i / per_row), dim = (int)(i - (int64_t)row * per_row) * 4 % c.head_dim;
+            const int64_t at = (int64_t)rows.pos[row] * (c.head_dim / 2) + dim / 2;
+            f4* x = reinterpret_cast<f4*>(q + 4 * i);
+            *x = rotated(*x, freq_real + at, freq_imag + at);
+        }
+        return;
+    }
+    const int pages = ch.item_rows / 16 + 1;
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
+    const int h = (int)(unit % c.kv_heads);
+    const int64_t rest = unit / c.kv_heads;
+    if (rest >= (int64_t)ch.work_items * pages) return;
+    const PageRows p = page_rows(rows, ch, (int)(rest / pages), (int)(rest % pages));
+    if (p.count == 0) return;
+    const int lane = threadIdx.x & 63, tq = lane & 3, dg = lane >> 2;
+
+    f4 kx[J][4], vx[J][4];
+    float ka[4] = {0.f, 0.f, 0.f, 0.f}, va[4] = {0.f, 0.f, 0.f, 0.f}, bad[4] = {0.f, 0.f, 0.f, 0.f};
+    bool here[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        here[r] = (unsigned)(4 * tq + r - p.t0) < (unsigned)p.count;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int dim = 64 * j + 4 * dg;
+            kx[j][r] = vx[j][r] = f4{0.f, 0.f, 0.f, 0.f};
+            if (here[r] && dim < c.head_dim) {
+                const int64_t at = ((int64_t)(p.first + 4 * tq + r - p.t0) * c.kv_heads + h) * c.head_dim + dim;
+                kx[j][r] = *reinterpret_cast<const f4*>(k + at);
+                vx[j][r] = *reinterpret_cast<const f4*>(v + at);
+            }
+        }
+    }
+    if (ROPE) {
+        const int64_t pos = rows.pos[p.first] - p.t0;  // of token 0
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int dim = 64 * j + 4 * dg;
+                if (here[r] && dim < c.head_dim) {
+                    const int64_t f = (pos + 4 * tq + r) * (c.head_dim / 2) + dim / 2;
+                    kx[j][r] = rotated(kx[j][r], freq_real + f, freq_imag + f);
+                    const int64_t at = ((int64_t)(p.first + 4 * tq + r - p.t0) * c.kv_heads + h) * c.head_dim + dim;
+                    *reinterpret_cast<f4*>(k + at) = kx[j][r];
+                }
+            }
+    }
+    float ks[4], vs[4], ki[4], vi[4];
+    bool good[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            ka[r] = fmaxf(ka[r], abs_max(kx[j][r]));
+            va[r] = fmaxf(va[r], abs_max(vx[j][r]));
+            bad[r] += poison(kx[j][r]) + poison(vx[j][r]);
+        }
+        ka[r] = page_max(ka[r]);
+        va[r] = page_max(va[r]);
+        good[r] = page_max(bad[r] == 0.0f ? 0.0f : 1.0f) == 0.0f;
+        ks[r] = scale_of(ka[r], good[r]), ki[r] = inverse_of(ka[r], good[r]);
+        vs[r] = scale_of(va[r], good[r]), vi[r] = inverse_of(va[r], good[r]);
+    }
+    if (p.page < 0 || p.page >= c.num_pages) {
+        if (lane == 0 && h == 0) atomicAdd(c.bad_pages, p.count);
+        return;
+    }
+    uint8_t* rec = c.cache + (int64_t)p.page * c.page_stride + c.layer_off + (int64_t)h * c.record;
+    const int chunks = c.hdp >> 4, mine = 4 * tq + (dg & 3);  // the token this lane has of K after the exchange
+    const bool whole = p.count == 16;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        int kc[4], vc[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            kc[r] = good[r] ? (int)codes_of(kx[j][r], ki[r]) : 0;
+            vc[r] = good[r] ? (int)codes_of(vx[j][r], vi[r]) : 0;
+        }
+        exchange<4>(kc, lane);
+        turn_bytes(vc);
+        exchange<1>(vc, lane);
+        const int chunk = 4 * j + (dg >> 2);
+        if (chunk >= chunks) continue;
+        if (whole || (unsigned)(mine - p.t0) < (unsigned)p.count)
+            *reinterpret_cast<i4*>(rec + ((tq * chunks + chunk) * 4 + (dg & 3)) * 16) = i4{kc[0], kc[1], kc[2], kc[3]};
+        uint8_t* vb = rec + 16 * c.hdp + (64 * j + 4 * dg + tq) * 16;
+        if (whole) {
+            *reinterpret_cast<i4*>(vb) = i4{vc[0], vc[1], vc[2], vc[3]};
+        } else {  // the page's other tokens stay as they are
+#pragma unroll
+            for (int t = 0; t < 16; t++)
+                if ((unsigned)(t - p.t0) < (unsigned)p.count) vb[t] = (uint8_t)(vc[t >> 2] >> (8 * (t & 3)));
+        }
+    }
+    if (dg == 0) {
+        float* s = reinterpret_cast<float*>(rec + 32 * c.hdp) + 4 * tq;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (here[r]) s[r] = ks[r], s[16 + r] = vs[r];
+    }
+}
+
+template <int J>
+__global__ __launch_bounds__(THREADS) void kv_q8_read_pages_kernel(KvQ8 c, KvQ8Rows rows, KvQ8Chunks ch,
+                                                                   float* __restrict__ k, float* __restrict__ v) {
+    const int pages = ch.item_rows / 16 + 1;
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
+    const int h = (int)(unit % c.kv_heads);
+    const int64_t rest = unit / c.kv_heads;
+    if (rest >= (int64_t)ch.work_items * pages) return;
+    const PageRows p = page_rows(rows, ch, (int)(rest / pages), (int)(rest % pages));
+    if (p.count == 0) return;
+    const int lane = threadIdx.x & 63, tq = lane & 3, dg = lane >> 2;
+    if (p.page < 0 || p.page >= c.num_pages) {
+        if (lane == 0 && h == 0) atomicAdd(c.bad_pages, p.count);
+        return;
+    }
+    const uint8_t* rec = c.cache + (int64_t)p.page * c.page_stride + c.layer_off + (int64_t)h * c.record;
+    const int chunks = c.hdp >> 4;
+    const f4 ks = *reinterpret_cast<const f4*>(rec + 32 * c.hdp + 16 * tq);
+    const f4 vs = *reinterpret_cast<const f4*>(rec + 32 * c.hdp + 64 + 16 * tq);
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int chunk = 4 * j + (dg >> 2), dim = 64 * j + 4 * dg;
+        i4 kl = {0, 0, 0, 0}, vl = kl;
+        if (chunk < chunks) {
+            kl = *reinterpret_cast<const i4*>(rec + ((tq * chunks + chunk) * 4 + (dg & 3)) * 16);
+            vl = *reinterpret_cast<const i4*>(rec + 16 * c.hdp + (dim + tq) * 16);
+        }
+        int kc[4] = {kl[0], kl[1], kl[2], kl[3]}, vc[4] = {vl[0], vl[1], vl[2], vl[3]};
+        exchange<4>(kc, lane);
+        exchange<1>(vc, lane);
+        turn_bytes(vc);
+        if (dim >= c.head_dim) continue;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if ((unsigned)(4 * tq + r - p.t0) >= (unsigned)p.count) continue;
+            const int64_t at = ((int64_t)(p.first + 4 * tq + r - p.t0) * c.kv_heads + h) * c.head_dim + dim;
+            *reinterpret_cast<f4*>(k + at) = f4{(float)(int8_t)kc[r] * ks[r], (float)(int8_t)(kc[r] >> 8) * ks[r],
+                                                (float)(int8_t)(kc[r] >> 16) * ks[r], (float)(kc[r] >> 24) * ks[r]};
+            *reinterpret_cast<f4*>(v + at) = f4{(float)(int8_t)vc[r] * vs[r], (float)(int8_t)(vc[r] >> 8) * vs[r],
+                                                (float)(int8_t)(vc[r] >> 16) * vs[r], (float)(vc[r] >> 24) * vs[r]};
+        }
+    }
+}
+
 unsigned groups(int64_t units, int lph) {
     const int64_t per = THREADS / lph, g = (units + per - 1) / per;
     return (unsigned)(g < 1 ? 1 : g > 65536 ? 65536 : g);
 }
+// Workgroups that take the pages of a batch's chunks.
+int64_t page_groups(const KvQ8& c, const KvQ8Chunks& ch) {
+    return ((int64_t)ch.work_items * (ch.item_rows / 16 + 1) * c.kv_heads + THREADS / 64 - 1) / (THREADS / 64);
+}
 
-template <int LPH>
-void append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v, const float* fr, const float* fi,
-            int n_heads, hipStream_t s) {
+template <int J>
+void append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* q, float* k, const float* v, const float* fr,
+            const float* fi, int n_heads, hipStream_t s) {
+    constexpr int LPH = J == 1 ? 16 : J == 2 ? 32 : 64;
+    if (ch.work_items) {
+        const unsigned pages = (unsigned)page_groups(c, ch);
+        const unsigned turn = fr ? groups((int64_t)r.rows * n_heads * c.head_dim / 4, 1) : 0;
+        if (fr)
+            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, true>), dim3(pages + turn), dim3(THREADS), 0, s, c, r, ch, q,
+                               k, v, fr, fi, n_heads, pages);
+        else
+            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, false>), dim3(pages), dim3(THREADS), 0, s, c, r, ch, q, k, v,
+                               fr, fi, n_heads, pages);
+        return;
+    }
     const int64_t units = (int64_t)r.rows * ((fr ? n_heads : 0) + c.kv_heads);
     if (fr)
         hipLaunchKernelGGL((kv_q8_append_kernel<LPH, true>), dim3(groups(units, LPH)), dim3(THREADS), 0, s, c, r, q, k,
@@ -176,25 +447,39 @@ void append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v
                            v, fr, fi, n_heads);
 }
 
-template <int LPH>
-void read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v, hipStream_t s) {
-    hipLaunchKernelGGL((kv_q8_read_kernel<LPH>), dim3(groups((int64_t)r.rows * c.kv_heads, LPH)), dim3(THREADS), 0, s, c,
-                       r, k, v);
+template <int J>
+void read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* k, float* v, hipStream_t s) {
+    constexpr int LPH = J == 1 ? 16 : J == 2 ? 32 : 64;
+    if (ch.work_items)
+        hipLaunchKernelGGL((kv_q8_read_pages_kernel<J>), dim3((unsigned)page_groups(c, ch)), dim3(THREADS), 0, s, c, r, ch,
+                           k, v);
+    else
+        hipLaunchKernelGGL((kv_q8_read_kernel<LPH>), dim3(groups((int64_t)r.rows * c.kv_heads, LPH)), dim3(THREADS), 0, s,
+                           c, r, k, v);
+}
+
+// The pages' workgroups have a grid index each.
+bool fits(const KvQ8& c, const KvQ8Chunks& ch) {
+    return c.head_dim >= 4 && c.head_dim <= 256 && c.head_dim % 4 == 0 && ch.item_rows % 16 == 0 &&
+           page_groups(c, ch) <= INT32_MAX - 65536;
 }
 
 }  // namespace
 
-hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v,
-                               const float* freq_real, const float* freq_imag, int n_heads, hipStream_t stream) {
-    if (c.head_dim > 256 || c.head_dim % 4) return hipErrorInvalidValue;
-    (c.hdp <= 64 ? append<16> : c.hdp <= 128 ? append<32> : append<64>)(c, r, q, k, v, freq_real, freq_imag, n_heads,
-                                                                       stream);
+hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* q, float* k,
+                               const float* v, const float* freq_real, const float* freq_imag, int n_heads,
+                               hipStream_t stream) {
+    if (!fits(c, ch)) return hipErrorInvalidValue;
+    auto* const f = c.hdp <= 64 ? append<1> : c.hdp <= 128 ? append<2> : c.hdp <= 192 ? append<3> : append<4>;
+    f(c, r, ch, q, k, v, freq_real, freq_imag, n_heads, stream);
     return hipGetLastError();
 }
 
-hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v, hipStream_t stream) {
-    if (c.head_dim > 256 || c.head_dim % 4) return hipErrorInvalidValue;
-    (c.hdp <= 64 ? read<16> : c.hdp <= 128 ? read<32> : read<64>)(c, r, k, v, stream);
+hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* k, float* v,
+                             hipStream_t stream) {
+    if (!fits(c, ch)) return hipErrorInvalidValue;
+    auto* const f = c.hdp <= 64 ? read<1> : c.hdp <= 128 ? read<2> : c.hdp <= 192 ? read<3> : read<4>;
+    f(c, r, ch, k, v, stream);
     return hipGetLastError();
 }
 
