@@ -544,35 +544,57 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
     pool->last_stream = s;
 }
 
-// Launch shape of a decode over an 8-bit pool: tiles per split.  One wave takes a
-// tile at a time, a workgroup's waves a split's tiles in turn.
+// Launch shape of a decode over an 8-bit pool: four waves to a workgroup (two where
+// four waves' parts of all columns do not fit LDS), and the tiles per split that an
+// estimate of the launch's time finds best.  Its constants, in us: a tile takes a
+// wave t_alone where the memory is not what it waits for (measured 1.8 at head size
+// 64, 3.2 at 128: loads' latency and the products), t_busy where every resident wave
+// streams at 6.7 TB/s; a workgroup begins in 2.5, and a split that has to be joined
+// costs 5 more.  Where a launch has more workgroups than are resident, they follow
+// one another as they finish; the last ones run alone.
 struct Q8DecodeShape {
-    int waves, tps, groups, cols;
+    int waves, tps, groups, splits;
 };
 template <class Ctx>
 Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_heads, int n_kv_heads, int head_dim) {
-    Q8DecodeShape sh;
-    // (four waves' parts of 16 heads of 256 dimensions are more than 64 KB of LDS)
-    sh.waves = kv_q8_padded(head_dim) > 192 ? 2 : 4;
-    const int kv_mul = n_heads / n_kv_heads;
-    sh.cols = std::min(kv_mul, KV_Q8_COLUMNS);
-    sh.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
+    Q8DecodeShape best{};
+    const int kv_mul = n_heads / n_kv_heads, hdp = kv_q8_padded(head_dim);
+    best.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
+    best.waves = kv_q8_decode_lds(n_heads, n_kv_heads, kv_q8_partial_floats(head_dim), 4, 1) <= KV_Q8_LDS ? 4 : 2;
+    const double W = best.waves, columns = (double)n_kv_heads * best.groups;
     long long tiles = 0;
     int longest = 1;
+    auto tiles_of = [&](int b) { return (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE; };
     for (int b = 0; b < B; b++) {
-        const int n = (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE;
-        tiles += n;
-        longest = std::max(longest, n);
+        tiles += tiles_of(b);
+        longest = std::max(longest, tiles_of(b));
     }
-    const long long resident = 8LL / sh.waves * std::max(pool->num_cus, 1);  // 8 waves per CU
-    const long long each = (tiles * n_kv_heads * sh.groups + resident - 1) / resident;
-    sh.tps = (int)std::min<long long>(longest, (each + sh.waves - 1) / sh.waves * sh.waves);
-    sh.tps = std::max(sh.tps, sh.waves);
-    return sh;
+    const double waves = 4.0 * kv_q8_decode_occupancy(hdp) * std::max(pool->num_cus, 1), resident = waves / W;
+    const double t_alone = hdp <= 64 ? 1.8 : hdp <= 128 ? 3.2 : 5.0;
+    const double t_busy = waves * KV_Q8_TILE * (2 * hdp + 8) / 6.7e6;
+    double least = 1e30;
+    for (int rounds = (longest + 256 * best.waves - 1) / (256 * best.waves);; rounds += 1 + rounds / 8) {
+        const int tps = rounds * best.waves;
+        long long items = 0;
+        for (int b = 0; b < B; b++) items += (tiles_of(b) + tps - 1) / tps;
+        const double load = (double)items * columns / resident;  // workgroups per place
+        const double begin = 2.5 + (tps < longest ? 5.0 : 0.0);
+        const double deep = std::min<double>(rounds, (longest + W - 1) / W);
+        const double cost = load <= 1 ? deep * std::max(t_alone, t_busy * load) + begin
+                                      : load * ((double)tiles / items / W * t_busy + begin) +
+                                            0.5 * (deep * t_alone + begin);
+        if (cost < least) {
+            least = cost;
+            best.tps = tps;
+        }
+        if (tps >= longest) break;
+    }
+    best.splits = (longest + best.tps - 1) / best.tps;
+    return best;
 }
 
 KvQ8Decode q8_decode_args(const nitro_kvpool* pool, int layer, const float* q, float* out, int n_heads,
-                          const Q8DecodeShape& sh) {
+                          const Q8DecodeShape& sh, bool shared_pages) {
     KvQ8Decode a{};
     a.c = kv_q8_layer(pool, layer);
     a.q = q;
@@ -580,7 +602,9 @@ KvQ8Decode q8_decode_args(const nitro_kvpool* pool, int layer, const float* q, f
     a.n_heads = n_heads;
     a.tiles_per_split = sh.tps;
     a.waves = sh.waves;
-    a.pstride = (a.c.head_dim + 2 + 3) / 4 * 4;
+    a.num_splits = sh.splits;
+    a.pstride = kv_q8_partial_floats(a.c.head_dim);
+    a.stream_kv = sh.groups == 1 && !shared_pages;
     a.qscale = (float)(1.4426950408889634 / std::sqrt((double)a.c.head_dim));
     return a;
 }
@@ -591,10 +615,7 @@ void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out,
     DecodeBatch& d = pool->decode;
     auto ctx = [&](int b) { return d.positions[b] + 1; };
     const Q8DecodeShape sh = plan_q8_decode(pool, d.batch, ctx, n_heads, n_kv_heads, head_dim);
-    KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh);
-    int longest = 1;
-    for (int b = 0; b < d.batch; b++) longest = std::max(longest, (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE);
-    a.num_splits = (longest + sh.tps - 1) / sh.tps;
+    KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh, d.shared_pages);
     if (a.num_splits > 1) {
         pool->partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
         if (pool->counters.reserve((size_t)d.batch * n_kv_heads * sh.groups))
@@ -980,8 +1001,7 @@ int nitro_paged_attn_decode_static(nitro_kvpool* pool, int32_t layer, const floa
         };
         if (pool->q8) {
             const Q8DecodeShape sh = plan_q8_decode(pool, batch, ctx, n_heads, n_kv_heads, head_dim);
-            KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh);
-            a.num_splits = ((max_context + KV_Q8_TILE - 1) / KV_Q8_TILE + sh.tps - 1) / sh.tps;
+            KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh, !pages_private);
             if (a.num_splits > 1) {
                 float* ws = static_scratch((size_t)batch * n_kv_heads * sh.groups,
                                            (size_t)batch * a.num_splits * n_heads * a.pstride);

@@ -19,8 +19,8 @@
 
 namespace nitro {
 
-inline constexpr int kv_q8_padded(int head_dim) { return (head_dim + 15) / 16 * 16; }
-inline constexpr int kv_q8_record_bytes(int head_dim) { return 32 * kv_q8_padded(head_dim) + 128; }
+constexpr int kv_q8_padded(int head_dim) { return (head_dim + 15) / 16 * 16; }
+constexpr int kv_q8_record_bytes(int head_dim) { return 32 * kv_q8_padded(head_dim) + 128; }
 
 // A layer of an 8-bit cache.
 struct KvQ8 {
@@ -71,8 +71,20 @@ struct KvQ8Decode {
     int32_t* counters;  // per (b, K/V head, group of its query heads), zero between launches
     int32_t batch, n_heads, max_pages, ctx_limit;
     int32_t tiles_per_split, num_splits, waves, pstride;
+    int32_t stream_kv;  // no record is read twice: loads that stay out of the caches
     float qscale;  // log2(e) / sqrt(head_dim)
 };
+// Waves per SIMD of the decode kernel.
+constexpr int kv_q8_decode_occupancy(int hdp) { return hdp <= 64 ? 4 : hdp <= 128 ? 2 : 1; }
+// Floats of a partial: acc[head_dim], m, l, on 16 bytes.
+inline int kv_q8_partial_floats(int head_dim) { return (head_dim + 2 + 3) / 4 * 4; }
+constexpr size_t KV_Q8_LDS = 65536 - 64;  // of a decode workgroup at most
+// Bytes of LDS of a decode workgroup: its waves' parts, later a join's factors.
+inline size_t kv_q8_decode_lds(int n_heads, int kv_heads, int pstride, int waves, int num_splits) {
+    const int kv_mul = n_heads / kv_heads, cols = kv_mul < KV_Q8_COLUMNS ? kv_mul : KV_Q8_COLUMNS;
+    const size_t parts = (size_t)waves * cols * pstride, join = (size_t)cols * (num_splits + 1);
+    return sizeof(float) * (parts > join ? parts : join);
+}
 hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream);
 
 struct KvQ8Prefill {

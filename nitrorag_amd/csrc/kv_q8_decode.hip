@@ -1,0 +1,206 @@
+// Decode over an 8-bit paged cache on gfx950: one token per sequence, long contexts
+// split over workgroups (the pass over the keys: kv_q8_attn.hpp).
+#include <hip/hip_runtime.h>
+
+#include "device_pool.hpp"
+#include "kv_q8.hpp"
+#include "kv_q8_attn.hpp"
+
+namespace nitro {
+namespace {
+
+// Device-coherent accesses of the partials and counters: relaxed atomics at agent
+// scope, written through to and read from where the XCDs' caches agree.  Two floats
+// at a time (8-byte aligned).
+__device__ __forceinline__ void store_coherent(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_coherent(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(p)), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+// out = A / L; 0 where no key was seen.
+__device__ __forceinline__ float divided(float A, float L) { return L == 0.0f ? 0.0f : A / L; }
+
+constexpr int JOIN = 16;  // partials whose loads go out together
+
+// A workgroup takes one split of one sequence's keys for up to 16 query heads of a
+// K/V head; its waves take the split's tiles in turn.  Waves per SIMD are what the
+// registers allow without spills (at head size 128, 183 of them: three waves with 13
+// spilled took 404 us where two take 337).
+template <int CH, bool STREAM>
+__global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_decode_kernel(KvQ8Decode a) {
+    extern __shared__ float s_part[];  // [waves][cols][pstride], then of a join [cols][parts] factors and [cols] sums
+    __shared__ int s_last;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv_mul = a.n_heads / a.c.kv_heads;
+    const int groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
+    int w = blockIdx.x;
+    const int hg = w % groups;
+    w /= groups;
+    const int kv_h = w % a.c.kv_heads;
+    w /= a.c.kv_heads;
+    // Workgroups go round the CUs in order of their index, and the splits that a
+    // short sequence lacks end at once: an odd number of places per sequence keeps
+    // those from falling on the same CUs (24 sequences of 512 to 8192 tokens at 32/8
+    // heads of 128 in splits of 2048: 61 us with four places, 47 with five).
+    const int places = a.num_splits | 1;
+    const int split = w % places, b = w / places;
+    const int h0 = kv_h * kv_mul + hg * KV_Q8_COLUMNS;  // first query head
+    const int cols = min(KV_Q8_COLUMNS, kv_mul - hg * KV_Q8_COLUMNS);
+    const int hd = a.c.head_dim;
+    const int col = lane & 15, g = lane >> 4;
+
+    // Table entries past the sequence's own may be read (their ids are checked,
+    // their keys hidden): the first tile's loads wait for its entries alone.
+    const int32_t* trow = a.tables + (int64_t)b * a.max_pages;
+    auto page = [&](int i) { return trow[min(i, a.max_pages - 1)]; };
+    const int t0 = split * a.tiles_per_split;
+    const int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
+    const int ctx = max(0, min(a.positions[b] + 1, a.ctx_limit));
+    const int tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
+    const int parts = max(1, (tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+    if (split >= parts) return;
+    if (ctx == 0 && hg == 0 && kv_h == 0 && threadIdx.x == 0) atomicAdd(a.c.bad_pages, 1);  // a position below 0
+    const int t1 = min(tiles, t0 + a.tiles_per_split);
+
+    State<CH> st;
+#pragma unroll
+    for (int t = 0; t < CH; t++) st.o[t] = f4{0.f, 0.f, 0.f, 0.f};
+    if (t0 + wave < t1) {
+        const auto q =
+            load_query<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, a.qscale, g);
+        attend<CH, STREAM>(st, q, a.c, a.c.cache + a.c.layer_off + (int64_t)kv_h * a.c.record, t0 + wave, t1, a.waves,
+                           lane, kp, vp, page, [&](int t) { return ctx - t * KV_Q8_TILE - 16 * g; });
+    }
+
+    // The waves' parts meet in LDS.
+    st.l = column_sum(st.l);
+    if (col < cols) {
+        float* part = s_part + (wave * cols + col) * a.pstride;
+#pragma unroll
+        for (int t = 0; t < CH; t++) {
+            const int dim = 16 * t + 4 * g;
+            if (dim < hd) *reinterpret_cast<f4*>(part + dim) = st.o[t];
+        }
+        if (g == 0) {
+            part[hd] = st.m;
+            part[hd + 1] = st.l;
+        }
+    }
+    __syncthreads();
+    const int pairs = cols * hd / 2;
+    for (int o = threadIdx.x; o < pairs; o += blockDim.x) {
+        const int c = 2 * o / hd, d = 2 * o - c * hd;
+        float M = -INFINITY, L = 0.0f, A0 = 0.0f, A1 = 0.0f;
+        for (int wv = 0; wv < a.waves; wv++) M = fmaxf(M, s_part[(wv * cols + c) * a.pstride + hd]);
+        for (int wv = 0; wv < a.waves; wv++) {
+            const float* part = s_part + (wv * cols + c) * a.pstride;
+            const float m = part[hd], f = scale_of(m, M);
+            L += m == -INFINITY ? part[hd + 1] : part[hd + 1] * f;  // no finite maximum: 0 or NaN
+            A0 = fmaf(part[d], f, A0);
+            A1 = fmaf(part[d + 1], f, A1);
+        }
+        if (parts == 1) {
+            float* out = a.out + ((int64_t)b * a.n_heads + h0 + c) * hd + d;
+            out[0] = divided(A0, L);
+            out[1] = divided(A1, L);
+        } else {
+            float* part = a.partials + (((int64_t)b * a.num_splits + split) * a.n_heads + h0 + c) * a.pstride;
+            store_coherent(part + d, A0, A1);
+            if (d == 0) store_coherent(part + hd, M, L);
+        }
+    }
+    if (parts == 1) return;
+
+    // The last workgroup of these heads to arrive joins the splits, in their order.
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's stores have arrived
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* counter = a.counters + ((int64_t)b * a.c.kv_heads + kv_h) * groups + hg;
+        const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before == parts - 1;
+        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    const int64_t stride = (int64_t)a.n_heads * a.pstride;  // from split to split
+    const float* parts0 = a.partials + ((int64_t)b * a.num_splits * a.n_heads + h0) * a.pstride;
+    // a wave per head: the splits' factors 2^(m - M) and the sum (lane i holds splits i, i + 64, ..)
+    for (int c = wave; c < cols; c += a.waves) {
+        float M = -INFINITY, L = 0.0f;
+        for (int sp = lane; sp < parts; sp += 64) M = fmaxf(M, load_coherent(parts0 + sp * stride + c * a.pstride + hd).x);
+        M = wave_max(M);
+        for (int sp = lane; sp < parts; sp += 64) {
+            const float2 ml = load_coherent(parts0 + sp * stride + c * a.pstride + hd);
+            const float f = scale_of(ml.x, M);
+            s_part[c * parts + sp] = f;
+            L += ml.x == -INFINITY ? ml.y : ml.y * f;
+        }
+        L = wave_sum(L);
+        if (lane == 0) s_part[cols * parts + c] = L;
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < pairs; o += blockDim.x) {
+        const int c = 2 * o / hd, d = 2 * o - c * hd;
+        const float* from = parts0 + c * a.pstride + d;
+        const float* f = s_part + c * parts;
+        float A0 = 0.0f, A1 = 0.0f;
+        int sp = 0;
+        for (; sp + JOIN <= parts; sp += JOIN) {
+            float2 x[JOIN];
+#pragma unroll
+            for (int i = 0; i < JOIN; i++) x[i] = load_coherent(from + (sp + i) * stride);
+#pragma unroll
+            for (int i = 0; i < JOIN; i++) A0 = fmaf(x[i].x, f[sp + i], A0), A1 = fmaf(x[i].y, f[sp + i], A1);
+        }
+        for (; sp < parts; sp++) {
+            const float2 x = load_coherent(from + sp * stride);
+            A0 = fmaf(x.x, f[sp], A0), A1 = fmaf(x.y, f[sp], A1);
+        }
+        float* out = a.out + ((int64_t)b * a.n_heads + h0 + c) * hd + d;
+        const float L = s_part[cols * parts + c];
+        out[0] = divided(A0, L);
+        out[1] = divided(A1, L);
+    }
+}
+
+// launch(kernel) with the kernel built for `chunks` runs of 16 dimensions.
+template <int CH, class F>
+void pick(int chunks, bool stream, F launch) {
+    if (chunks == CH)
+        stream ? launch(kv_q8_decode_kernel<CH, true>) : launch(kv_q8_decode_kernel<CH, false>);
+    else if constexpr (CH < 16)
+        pick<CH + 1>(chunks, stream, launch);
+}
+
+}  // namespace
+
+hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream) {
+    const int kv_mul = a.n_heads / a.c.kv_heads;
+    const int groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
+    const int64_t blocks = (int64_t)a.batch * (a.num_splits | 1) * a.c.kv_heads * groups;
+    const int chunks = a.c.hdp / 16;
+    const size_t lds = kv_q8_decode_lds(a.n_heads, a.c.kv_heads, a.pstride, a.waves, a.num_splits);
+    if (a.waves < 1 || a.waves > 4 || a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
+        blocks > INT32_MAX || lds > KV_Q8_LDS)
+        return hipErrorInvalidValue;
+    const dim3 grid((unsigned)blocks), block(64 * a.waves);
+    pick<1>(chunks, a.stream_kv, [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, a); });
+    return hipGetLastError();
+}
+
+}  // namespace nitro
