@@ -514,6 +514,8 @@ void set_device_decode_groups(nitro_kvpool* pool, const int32_t* tables, int max
 void forward_mixed(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, int prefill_rows,
                    int decode_rows, bool prefill_as_decode, bool prefill_logits, float* logits,
                    int32_t* next, int semantics, hipStream_t stream);
+// Throws unless the pool is one the model steps over.
+void require_model_pool(const nitro_model* m, const nitro_kvpool* pool);
 // Dimensions the scheduler needs: {dim, vocab, seq_len, n_layers, kv_dim}.
 void model_dims(const nitro_model* m, int32_t* dims);
 

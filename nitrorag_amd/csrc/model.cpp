@@ -37,6 +37,9 @@ struct nitro_model {
     int max_rows = 0;                      // of any forward
     float* hb_floats() const { return hb.ptr ? hb.ptr : reinterpret_cast<float*>(hsplit.ptr); }
     DeviceBuffer<int32_t> tokens;
+    DeviceBuffer<float> kv_rows;   // over an 8-bit pool: a layer's new K rows, then its V rows, on their way there
+    DeviceBuffer<int32_t> kv_at;   // 0, 1, 2, ..: where the products put row r of them
+    int kv_at_rows = 0;            // (filled so far)
     Staging staging;
 
     const float* f32(size_t off) const { return reinterpret_cast<const float*>(weights + off); }
@@ -88,9 +91,20 @@ void ensure_tiled(nitro_model* m, hipStream_t s) {
 // rows as any forward had, and that memory serves SwiGLU's output as floats too
 // unless those have a buffer already.  Only a forward of more rows than any before
 // moves a buffer that exists (a captured forward holds their addresses).
-void reserve_rows(nitro_model* m, int rows, bool last_block) {
+void reserve_rows(nitro_model* m, const nitro_kvpool* pool, int rows, bool last_block) {
     m->max_rows = std::max(m->max_rows, rows);
     const size_t r = (size_t)m->max_rows;
+    if (pool->q8) {
+        m->kv_rows.reserve(2 * r * m->kv_dim);
+        if (m->kv_at.reserve(r)) m->kv_at_rows = 0;
+        if (m->kv_at_rows < rows) {  // all of it, before any stream reads it
+            std::vector<int32_t> at(m->kv_at.count);
+            for (size_t i = 0; i < at.size(); i++) at[i] = (int32_t)i;
+            hip_check(hipMemcpy(m->kv_at.ptr, at.data(), at.size() * sizeof(int32_t), hipMemcpyHostToDevice),
+                      "hipMemcpy(row numbers)");
+            m->kv_at_rows = (int)at.size();
+        }
+    }
     m->x.reserve(r * m->dim);
     m->attn.reserve(r * m->dim);
     m->ss.reserve(r * (size_t)((m->dim + 15) / 16));
@@ -111,7 +125,11 @@ void check_model_pool(const nitro_model* m, const nitro_kvpool* pool) {
     require(pool != nullptr, ERR_INVALID_ARGUMENT, "null pool");
     require(pool->num_layers == m->n_layers && pool->kv_dim == m->kv_dim, ERR_INVALID_ARGUMENT,
             "pool layers / kv_dim do not match the model");
-    require(pool->q8 == nullptr, ERR_UNSUPPORTED, "a model steps over an fp32 pool");
+    if (pool->q8) {
+        require(pool->q8_kv_heads == m->n_kv_heads && pool->q8_head_dim == m->head_size, ERR_INVALID_ARGUMENT,
+                "the 8-bit pool's heads do not match the model");
+        (void)kv_q8_layer(pool, 0);  // the current device is the pool's
+    }
 }
 
 void upload_tokens(nitro_model* m, const int32_t* tokens, int rows, hipStream_t s) {
@@ -221,7 +239,29 @@ Q8Rope rope_args(const nitro_model* m, nitro_kvpool* pool, const int32_t* pos_a,
     r.pos[1] = pos_b;
     r.slot[1] = slot_b;
     r.split = split;
+    if (pool->q8) {
+        // The launch puts K and V into a buffer of rows as if it were a pool, row r in
+        // slot r; append_held then quantises them into the cache.
+        r.k_pool = m->kv_rows.ptr;
+        r.v_pool = m->kv_rows.ptr + (size_t)m->max_rows * m->kv_dim;
+        r.page_stride = (int64_t)BLOCK_SIZE * m->kv_dim;
+        r.num_pages = (m->max_rows + BLOCK_SIZE - 1) / BLOCK_SIZE;
+        r.slot[0] = m->kv_at.ptr;
+        r.slot[1] = m->kv_at.ptr + split;
+    }
     return r;
+}
+
+// Over an 8-bit pool: layer l's rows, `prefill` of the prefill batch's and then
+// `decode` of the decode batch's, into the cache.
+void append_held(const nitro_model* m, nitro_kvpool* pool, int l, int prefill, int decode, void* stream) {
+    if (!pool->q8) return;
+    const float* k = m->kv_rows.ptr;
+    const float* v = k + (size_t)m->max_rows * m->kv_dim;
+    const size_t after = (size_t)prefill * m->kv_dim;
+    require((prefill == 0 || nitro_kv_append_prefill(pool, l, k, v, stream) == NITRO_OK) &&
+                (decode == 0 || nitro_kv_append(pool, l, k + after, v + after, stream) == NITRO_OK),
+            ERR_INVALID_ARGUMENT, nitro_last_error());
 }
 
 void check_positions(const nitro_model* m, int max_pos) {
@@ -247,6 +287,8 @@ void model_dims(const nitro_model* m, int32_t* dims) {
     dims[4] = m->kv_dim;
 }
 
+void require_model_pool(const nitro_model* m, const nitro_kvpool* pool) { check_model_pool(m, pool); }
+
 void forward_mixed(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, int P, int B,
                    bool prefill_as_decode, bool prefill_logits, float* logits, int32_t* next, int semantics,
                    hipStream_t s) {
@@ -268,11 +310,12 @@ void forward_mixed(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, in
     if (!prefill_as_decode && P > 0) check_positions(m, pf.max_pos);
     // every row's RoPE position and K/V slot: the decode batch's, or the
     // prefill batch's for rows [0, P) when those go through the prefill kernel
+    reserve_rows(m, pool, P + B, semantics == NITRO_Q8_LAST_BLOCK);
     const Q8Rope rope = prefill_as_decode || P == 0
                             ? rope_args(m, pool, d.pos.ptr, d.slots.ptr, P + B, nullptr, nullptr)
                             : rope_args(m, pool, pf.row_pos.ptr, pf.slots.ptr, P, d.pos.ptr, d.slots.ptr);
-    reserve_rows(m, P + B, semantics == NITRO_Q8_LAST_BLOCK);
     layers(m, pool, tokens, P + B, semantics, rope, s, [&](int l) {
+        append_held(m, pool, l, prefill_as_decode ? 0 : P, prefill_as_decode ? P + B : B, stream);
         if (prefill_as_decode) {
             // every row attends its own prefix (keys 0..position) in one
             // decode-attention launch; a chunk row at position p sees the same
@@ -409,10 +452,11 @@ int nitro_forward_decode_batch(nitro_model* m, nitro_kvpool* pool, const int32_t
         hipStream_t s = as_stream(stream);
         const DecodeBatch& d = pool->decode;
         check_positions(m, max_of(d.positions));
-        reserve_rows(m, batch, semantics == NITRO_Q8_LAST_BLOCK);
+        reserve_rows(m, pool, batch, semantics == NITRO_Q8_LAST_BLOCK);
         upload_tokens(m, tokens, batch, s);
         const Q8Rope rope = rope_args(m, pool, d.pos.ptr, d.slots.ptr, batch, nullptr, nullptr);
         layers(m, pool, m->tokens.ptr, batch, semantics, rope, s, [&](int l) {
+            append_held(m, pool, l, 0, batch, stream);
             require(nitro_paged_attn_decode(pool, l, m->q.ptr, m->attn.ptr, m->n_heads, m->n_kv_heads,
                                             m->head_size, stream) == NITRO_OK,
                     ERR_INVALID_ARGUMENT, nitro_last_error());
@@ -435,12 +479,13 @@ int nitro_forward_prefill(nitro_model* m, nitro_kvpool* pool, const int32_t* tok
         require(total_rows == p.total_rows, ERR_INVALID_ARGUMENT,
                 "total_rows differs from the uploaded prefill batch");
         hipStream_t s = as_stream(stream);
-        reserve_rows(m, total_rows, semantics == NITRO_Q8_LAST_BLOCK);
+        reserve_rows(m, pool, total_rows, semantics == NITRO_Q8_LAST_BLOCK);
         m->last.reserve((size_t)p.batch * m->dim);
         upload_tokens(m, tokens, total_rows, s);
         check_positions(m, p.max_pos);
         const Q8Rope rope = rope_args(m, pool, p.row_pos.ptr, p.slots.ptr, total_rows, nullptr, nullptr);
         layers(m, pool, m->tokens.ptr, total_rows, semantics, rope, s, [&](int l) {
+            append_held(m, pool, l, total_rows, 0, stream);
             require(nitro_paged_attn_prefill(pool, l, m->q.ptr, m->attn.ptr, m->n_heads, m->n_kv_heads,
                                              m->head_size, stream) == NITRO_OK,
                     ERR_INVALID_ARGUMENT, nitro_last_error());

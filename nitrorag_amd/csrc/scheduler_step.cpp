@@ -139,6 +139,7 @@ int nitro_sched_step(nitro_scheduler* sched, nitro_model* model, nitro_kvpool* p
         const int vocab = dims[1], seq_len = dims[2];
         require(pool->num_layers == dims[3] && pool->kv_dim == dims[4], ERR_INVALID_ARGUMENT,
                 "pool layers / kv_dim do not match the model");
+        require_model_pool(model, pool);
         require(h.block_manager().mem.total_blocks() <= pool->num_pages, ERR_INVALID_ARGUMENT,
                 "the block manager has more pages than the pool");
         hipStream_t s = as_stream(stream);

@@ -86,6 +86,31 @@ class Cache:
         return k, v
 
 
+def held(x, heads):
+    """fp32 rows [rows][heads * head_dim] as the values they are held as."""
+    r = np.ascontiguousarray(x, np.float32).reshape(x.shape[0], heads, -1)
+    codes, scale = quantise(r, r)[:2]
+    return (codes.astype(np.float32) * scale[..., None]).reshape(x.shape)
+
+
+class HeldAttention:
+    """oracle.attn whose appends put the values that 8 bits hold into the fp32 pools."""
+
+    def __init__(self, attn, heads):
+        self._attn, self._heads = attn, heads
+
+    def __getattr__(self, name):
+        return getattr(self._attn, name)
+
+    def kv_append_decode(self, k_pool, v_pool, layer, k, v, tables, positions):
+        return self._attn.kv_append_decode(k_pool, v_pool, layer, held(k, self._heads), held(v, self._heads), tables,
+                                           positions)
+
+    def kv_scatter_prefill(self, k_pool, v_pool, layer, k, v, table, start_pos):
+        return self._attn.kv_scatter_prefill(k_pool, v_pool, layer, held(k, self._heads), held(v, self._heads), table,
+                                             start_pos)
+
+
 def attention(q, positions, k, v):
     """q [rows][heads][hd] at `positions` over keys 0..position; with a bound on what
     fp32 arithmetic with 24-bit fixed point may be off, elementwise [rows][heads][1].
