@@ -794,6 +794,9 @@ static int make_pool_q8(void* cache, bool owned, int32_t num_pages, int32_t num_
         require(attention_head_dim(head_dim), ERR_UNSUPPORTED, "head_dim must be a multiple of 4 from 4 to 256");
         require((long long)n_kv_heads * head_dim <= INT32_MAX && num_pages <= INT32_MAX / BLOCK_SIZE, ERR_UNSUPPORTED,
                 "a row or the slots do not fit 32 bits");
+        // (kernels count pages' places in units of 128 bytes)
+        require((double)num_pages * num_layers * n_kv_heads * kv_q8_record_bytes(head_dim) < 0x1p39, ERR_UNSUPPORTED,
+                "an 8-bit pool holds less than 512 GiB");
         require(owned || (cache != nullptr && (uintptr_t)cache % 16 == 0), ERR_INVALID_ARGUMENT,
                 "the cache must be a 16-byte aligned buffer");
         nitro_kvpool* pool = new nitro_kvpool();

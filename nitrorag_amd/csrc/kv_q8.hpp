@@ -25,7 +25,7 @@ constexpr int kv_q8_record_bytes(int head_dim) { return 32 * kv_q8_padded(head_d
 // A layer of an 8-bit cache.
 struct KvQ8 {
     uint8_t* cache;
-    int64_t page_stride, layer_off;  // bytes
+    int64_t page_stride, layer_off;  // bytes, multiples of 128; pages * page_stride < 2^39
     int32_t kv_heads, head_dim, hdp, record, num_pages;
     int32_t* bad_pages;
 };

@@ -89,30 +89,44 @@ struct Query {
     float scale;
 };
 
-// row: the column's query row, nullptr for a column without one.
+// A lane's part of its column's query row as it lies in memory (zeros where row is
+// nullptr: a column without one).
 template <int NC>
-__device__ __forceinline__ Query<NC> load_query(const float* row, int hd, float qscale, int g) {
+struct QueryRow {
     f4 x[NC][4];
-    float top = 0.0f, bad = 0.0f;
+};
+template <int NC>
+__device__ __forceinline__ QueryRow<NC> load_row(const float* row, int hd, int g) {
+    QueryRow<NC> q;
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int dim = 16 * (4 * j + g) + 4 * i;
-            x[j][i] = f4{0.f, 0.f, 0.f, 0.f};
-            if (row && dim < hd) x[j][i] = *reinterpret_cast<const f4*>(row + dim);
+            q.x[j][i] = f4{0.f, 0.f, 0.f, 0.f};
+            if (row && dim < hd) q.x[j][i] = *reinterpret_cast<const f4*>(row + dim);
+        }
+    return q;
+}
+
+template <int NC>
+__device__ __forceinline__ Query<NC> query_of(const QueryRow<NC>& from, float qscale) {
+    float top = 0.0f, bad = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                top = fmaxf(top, fabsf(x[j][i][e]));
-                bad = fmaf(x[j][i][e], 0.0f, bad);
+                top = fmaxf(top, fabsf(from.x[j][i][e]));
+                bad = fmaf(from.x[j][i][e], 0.0f, bad);
             }
-        }
     top = column_max(top);
     bad = column_sum(bad);  // NaN where the row holds an infinity or a NaN
     const float inv = top >= 0x1p-100f ? FIXED / top : 0.0f;
     Query<NC> q;
     // (never 0: a hidden key's -infinity stays one)
-    q.scale = (top >= 0x1p-100f ? top : 0x1p-100f) * (qscale * (0x1p24f / FIXED)) + bad;
+    q.scale = (top >= 0x1p-100f ? top : 0x1p-100f) * (qscale * (256.0f * 0x1p24f / FIXED)) + bad;
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
@@ -121,7 +135,7 @@ __device__ __forceinline__ Query<NC> load_query(const float* row, int hd, float 
             float v[4];
             int d0, d1, d2;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = __int_as_float((int)rintf(x[j][i][e] * inv) + 0x8080);
+            for (int e = 0; e < 4; e++) v[e] = __int_as_float((int)rintf(from.x[j][i][e] * inv) + 0x8080);
             digits(v[0], v[1], v[2], v[3], d0, d1, d2);
             q.d[j][0][i] = d0, q.d[j][1][i] = d1, q.d[j][2][i] = d2;
         }
@@ -137,20 +151,18 @@ struct State {
 };
 
 // What a wave holds of a tile: the K operands of its four products and the V
-// operands, and the scale of token lane % 16 of page lane / 16 (K's times 2^-24,
-// so that a score before the query's factor is in the range of its key).  STREAM: lines that nothing else
+// operands, and both scales of token lane % 16 of page lane / 16.  STREAM: lines that nothing else
 // reads, kept out of the caches.
 // CH: hdp / 16; a K row is CH runs of 16 dimensions, of which a lane has NC = CH / 4,
 // rounded up (zeros where there are fewer).
 template <int CH>
 struct KTile {
     i4 k[4][(CH + 3) / 4];
-    float s;
+    float ks, vs;
 };
 template <int CH>
 struct VTile {
     i4 v[CH];
-    float s;
 };
 template <bool STREAM, class T>
 __device__ __forceinline__ T load_kv(const uint8_t* p) {
@@ -167,14 +179,14 @@ __device__ __forceinline__ void load_k(KTile<CH>& x, const uint8_t* kr, const ui
 #pragma unroll
         for (int j = 0; j < (CH + 3) / 4; j++)
             if (4 * j + 3 < CH || 4 * j + g < CH) x.k[t][j] = load_kv<STREAM, i4>(at + (t * CH + 4 * j) * 64);
-    x.s = load_kv<STREAM, float>(vr + 512 * CH + (lane & 15) * 4);
+    x.ks = load_kv<STREAM, float>(vr + 512 * CH + (lane & 15) * 4);
+    x.vs = load_kv<STREAM, float>(vr + 512 * CH + 64 + (lane & 15) * 4);
 }
 template <int CH, bool STREAM>
 __device__ __forceinline__ void load_v(VTile<CH>& x, const uint8_t* vr, int lane) {
     const uint8_t* at = vr + 256 * CH + (lane & 15) * 16;
 #pragma unroll
     for (int t = 0; t < CH; t++) x.v[t] = load_kv<STREAM, i4>(at + t * 256);
-    x.s = load_kv<STREAM, float>(vr + 512 * CH + 64 + (lane & 15) * 4);
 }
 
 // Lane n of each 16 lanes' x, in all 16 (row_newbcast).
@@ -189,31 +201,37 @@ __device__ __forceinline__ void each_token(F f) {
     if constexpr (N < 15) each_token<N + 1>(f);
 }
 
+// The sum of products with a number's digits, in units of 256: x2 with the third
+// digit's, x1 with the second's and the first's, this rounded to a whole unit (its
+// sum began at 128 and was shifted down; half a unit is 2^-16 of the number's
+// largest value times one code, beside a sum over 64 codes).
+__device__ __forceinline__ int joined(int x2, int x1) { return (int)(((uint32_t)x2 << 8) + (uint32_t)x1); }
+
 // Scores of a tile before the query's factor, s[t][r] of the lane's column and
 // token 4t + r of page lane / 16; -infinity past the first `keys` of the page's
 // tokens (whatever bits their slots hold).  The column's largest comes back.
 template <int CH>
 __device__ __forceinline__ float scores(f4 (&s)[4], const KTile<CH>& x, const Query<(CH + 3) / 4>& q, int keys) {
     constexpr int NC = (CH + 3) / 4;
-    const float ks = x.s * 0x1p-24f;
-    i4 hi[4], lo[4];
+    const float ks = x.ks * 0x1p-24f;  // (a score before the query's factor is in the range of its key)
+    i4 x2[4], x1[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        hi[t] = lo[t] = i4{0, 0, 0, 0};
+        x2[t] = i4{0, 0, 0, 0}, x1[t] = i4{128, 128, 128, 128};
 #pragma unroll
-        for (int j = 0; j < NC; j++) hi[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][2], hi[t], 0, 0, 0);
+        for (int j = 0; j < NC; j++) x1[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][0], x1[t], 0, 0, 0);
     }
 #pragma unroll
     for (int t = 0; t < 4; t++) {
 #pragma unroll
-        for (int j = 0; j < NC; j++) lo[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][0], lo[t], 0, 0, 0);
-        hi[t] <<= 8;
+        for (int j = 0; j < NC; j++) x2[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][2], x2[t], 0, 0, 0);
+        x1[t] >>= 8;
 #pragma unroll
-        for (int j = 0; j < NC; j++) hi[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][1], hi[t], 0, 0, 0);
+        for (int j = 0; j < NC; j++) x1[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][j], q.d[j][1], x1[t], 0, 0, 0);
     }
     each_token([&](auto n) {
         constexpr int t = n / 4, r = n % 4;
-        s[t][r] = fmaf((float)hi[t][r], 256.0f, (float)lo[t][r]) * of_token<n>(ks);
+        s[t][r] = (float)joined(x2[t][r], x1[t][r]) * of_token<n>(ks);
     });
     // few tiles have hidden keys: a sequence's last, those on a chunk's diagonal
     if (__builtin_amdgcn_ballot_w64(keys < 16))
@@ -224,34 +242,41 @@ __device__ __forceinline__ float scores(f4 (&s)[4], const KTile<CH>& x, const Qu
 }
 
 // The weights' three digits, from the scores and the V scales.  (A NaN scale there
-// is a hidden slot's, or comes with a K scale that makes the sum NaN.)
+// is a hidden slot's, or comes with a K scale that makes the sum NaN.)  H: tiles that
+// share a maximum and a unit, so that their products are added up as integers: what
+// takes an output's integers to fp32 (five operations) is then paid once for them.
+template <int H>
 struct Weights {
-    i4 d[3];
+    i4 d[H][3];
     float unit;  // what the new integers are multiplied by
 };
-template <int CH>
-__device__ __forceinline__ Weights weigh(State<CH>& st, const f4 (&s)[4], float top, float scale, float vs) {
-    const float base = top == -INFINITY ? 0.0f : top * scale;  // no key (or only NaN ones) in the tile
-    vs = fabsf(vs) < INFINITY ? vs : 0.0f;
+template <int CH, int H>
+__device__ __forceinline__ Weights<H> weigh(State<CH>& st, f4 (&s)[H][4], float top, float scale, const float (&scales)[H]) {
+    const float base = top == -INFINITY ? 0.0f : top * scale;  // no key (or only NaN ones) in the tiles
     float sum = 0.0f, big = 0.0f;
-    f4 w[4];
-    each_token([&](auto n) {
-        constexpr int t = n / 4, r = n % 4;
-        const float p = exp2_fast(fmaf(s[t][r], scale, -base));
-        sum += p;
-        w[t][r] = p * of_token<n>(vs);
-        big = fmaxf(big, w[t][r]);
-    });
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+        const float vs = fabsf(scales[h]) < INFINITY ? scales[h] : 0.0f;
+        each_token([&](auto n) {
+            constexpr int t = n / 4, r = n % 4;
+            const float p = exp2_fast(fmaf(s[h][t][r], scale, -base));
+            sum += p;
+            s[h][t][r] = p * of_token<n>(vs);
+            big = fmaxf(big, s[h][t][r]);
+        });
+    }
     big = column_max(big);
     const float inv = big >= LEAST ? FIXED * __builtin_amdgcn_rcpf(big) : 0.0f;
-    Weights x;
+    Weights<H> x;
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-        int d0, d1, d2;
-        digits(fmaf(w[t][0], inv, BIAS), fmaf(w[t][1], inv, BIAS), fmaf(w[t][2], inv, BIAS), fmaf(w[t][3], inv, BIAS), d0,
-               d1, d2);
-        x.d[0][t] = d0, x.d[1][t] = d1, x.d[2][t] = d2;
-    }
+    for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            int d0, d1, d2;
+            digits(fmaf(s[h][t][0], inv, BIAS), fmaf(s[h][t][1], inv, BIAS), fmaf(s[h][t][2], inv, BIAS),
+                   fmaf(s[h][t][3], inv, BIAS), d0, d1, d2);
+            x.d[h][0][t] = d0, x.d[h][1][t] = d1, x.d[h][2][t] = d2;
+        }
     const float m = top == -INFINITY ? top : base, m_new = fmaxf(st.m, m);
     const float f = scale_of(m, m_new), alpha = scale_of(st.m, m_new);
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {  // a column's maximum grew
@@ -261,65 +286,46 @@ __device__ __forceinline__ Weights weigh(State<CH>& st, const f4 (&s)[4], float 
     }
     st.l += m == -INFINITY ? sum : sum * f;  // (a NaN stays)
     st.m = m_new;
-    x.unit = (big >= LEAST ? big : 0.0f) * (1.0f / FIXED) * f;
+    x.unit = (big >= LEAST ? big : 0.0f) * (256.0f / FIXED) * f;
     return x;
 }
 
-template <int CH>
-__device__ __forceinline__ void add_values(State<CH>& st, const VTile<CH>& x, const Weights& w) {
-    const float unit256 = w.unit * 256.0f;
+template <int CH, int H>
+__device__ __forceinline__ void add_values(State<CH>& st, const VTile<CH> (&x)[H], const Weights<H>& w) {
 #pragma unroll
     for (int t = 0; t < CH; t++) {
-        i4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-        hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.v[t], w.d[2], hi, 0, 0, 0);
-        lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.v[t], w.d[0], lo, 0, 0, 0);
-        hi <<= 8;
-        hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.v[t], w.d[1], hi, 0, 0, 0);
+        i4 x2 = {0, 0, 0, 0}, x1 = {128, 128, 128, 128};
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            st.o[t][r] = fmaf((float)hi[r], unit256, fmaf((float)lo[r], w.unit, st.o[t][r]));
+        for (int h = 0; h < H; h++) x1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[h].v[t], w.d[h][0], x1, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < H; h++) x2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[h].v[t], w.d[h][2], x2, 0, 0, 0);
+        x1 >>= 8;
+#pragma unroll
+        for (int h = 0; h < H; h++) x1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[h].v[t], w.d[h][1], x1, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) st.o[t][r] = fmaf((float)joined(x2[r], x1[r]), w.unit, st.o[t][r]);
     }
 }
 
-// A wave's tiles first, first + step, ... below end (end > first) of the keys of one
-// table row: a tile's K loads go out as soon as the previous tile's K is in its
-// products, its V loads likewise, so loads are in flight throughout.  Of tile t the
-// lane's column sees seen(t) tokens of page lane / 16.  kp, vp: the first tile's table entries; page(i): entry i (any i).
-template <int CH, bool STREAM, class Page, class Seen>
-__device__ __forceinline__ void attend(State<CH>& st, const Query<(CH + 3) / 4>& q, const KvQ8& c, const uint8_t* base,
-                                       int first, int end, int step, int lane, int kp, int vp, Page page, Seen seen) {
-    constexpr int NC = (CH + 3) / 4;
-    const int g = lane >> 4, sub = (lane & 15) >> 2;
-    auto good = [&](int id) { return (unsigned)id < (unsigned)c.num_pages; };
-    auto record = [&](int id) { return base + (int64_t)(good(id) ? id : 0) * c.page_stride; };
+template <int CH>
+__device__ __forceinline__ KTile<CH> no_k() {  // (a lane without a last run of its own keeps zeros there)
     KTile<CH> k;
-    VTile<CH> v;
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int j = 0; j < NC; j++) k.k[t][j] = i4{0, 0, 0, 0};
-    load_k<CH, STREAM>(k, record(kp), record(vp), lane);
-    load_v<CH, STREAM>(v, record(vp), lane);
-    int kp_next = page(4 * (first + step) + sub), vp_next = page(4 * (first + step) + g);
-    for (int t = first; t < end; t += step) {
-        const bool more = t + step < end;
-        int keys = seen(t);
-        if (!good(vp)) {  // its keys are left out
-            if (keys > 0 && (lane & 15) == 15) atomicAdd(c.bad_pages, 1);
-            keys = 0;
-        }
-        f4 s[4];
-        const float top = scores<CH>(s, k, q, keys);
-        if (more) load_k<CH, STREAM>(k, record(kp_next), record(vp_next), lane);
-        const Weights w = weigh<CH>(st, s, top, q.scale, v.s);
-        add_values<CH>(st, v, w);
-        vp = vp_next;
-        if (more) {
-            load_v<CH, STREAM>(v, record(vp), lane);
-            kp_next = page(4 * (t + 2 * step) + sub);
-            vp_next = page(4 * (t + 2 * step) + g);
-        }
-    }
+        for (int j = 0; j < (CH + 3) / 4; j++) k.k[t][j] = i4{0, 0, 0, 0};
+    return k;
+}
+// The record of a table entry's page; page 0's of one outside the pool, whose keys
+// seen_on hides (and counts, once for each page and wave).
+__device__ __forceinline__ const uint8_t* record(const KvQ8& c, const uint8_t* base, int id) {
+    // (records are whole multiples of 128 bytes, their places below 2^39)
+    return base + ((uint64_t)(((unsigned)id < (unsigned)c.num_pages ? id : 0) * (uint32_t)(c.page_stride >> 7)) << 7);
+}
+__device__ __forceinline__ int seen_on(const KvQ8& c, int id, int keys, int lane) {
+    if ((unsigned)id < (unsigned)c.num_pages) return keys;
+    if (keys > 0 && (lane & 15) == 15) atomicAdd(c.bad_pages, 1);
+    return 0;
 }
 
 }  // namespace

@@ -9,6 +9,47 @@
 namespace nitro {
 namespace {
 
+// A wave's tiles first, first + step, ... below end (end > first) of the keys of one
+// table row.  A tile's K loads go out as soon as the previous tile's K is in its
+// products and its V loads likewise, so loads are in flight throughout; loads return
+// in order, so table entries are asked for two tiles ahead, where waiting for them is
+// waiting for nothing younger.  Of tile t the lane's column sees seen(t) tokens of
+// page lane / 16.  kp, vp: the first tile's table entries; page(i): entry i (any i).
+template <int CH, bool STREAM, class Page, class Seen>
+__device__ __forceinline__ void attend(State<CH>& st, const QueryRow<(CH + 3) / 4>& row, float qscale, const KvQ8& c,
+                                       const uint8_t* base, int first, int end, int step, int lane, int kp, int vp,
+                                       Page page, Seen seen) {
+    const int g = lane >> 4, sub = (lane & 15) >> 2;
+    KTile<CH> k = no_k<CH>();
+    VTile<CH> v[1];
+    load_k<CH, STREAM>(k, record(c, base, kp), record(c, base, vp), lane);
+    int kp_next = page(4 * (first + step) + sub), vp_next = page(4 * (first + step) + g);
+    load_v<CH, STREAM>(v[0], record(c, base, vp), lane);
+    __builtin_amdgcn_sched_barrier(0);  // the loads are on their way before the query is waited for
+    const auto q = query_of(row, qscale);
+    int t = first;
+    auto tile = [&](auto more) {
+        int kp_then = 0, vp_then = 0;
+        if (more) kp_then = page(4 * (t + 2 * step) + sub), vp_then = page(4 * (t + 2 * step) + g);
+        const int keys = seen_on(c, vp, seen(t), lane);
+        f4 s[1][4];
+        const float top = scores<CH>(s[0], k, q, keys);
+        const float scales[1] = {k.vs};
+        if (more) load_k<CH, STREAM>(k, record(c, base, kp_next), record(c, base, vp_next), lane);
+        const Weights<1> w = weigh<CH, 1>(st, s, top, q.scale, scales);
+        add_values<CH, 1>(st, v, w);
+        if (more) {
+            load_v<CH, STREAM>(v[0], record(c, base, vp_next), lane);
+            vp = vp_next;
+            asm volatile("" : "+v"(kp_then), "+v"(vp_then));  // here by now
+            kp_next = kp_then, vp_next = vp_then;
+        }
+        t += step;
+    };
+    while (t + step < end) tile(std::true_type());
+    tile(std::false_type());  // (on its own: a load that may be missing costs waits for all of them)
+}
+
 // Device-coherent accesses of the partials and counters: relaxed atomics at agent
 // scope, written through to and read from where the XCDs' caches agree.  Two floats
 // at a time (8-byte aligned).
@@ -67,9 +108,12 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     // Table entries past the sequence's own may be read (their ids are checked,
     // their keys hidden): the first tile's loads wait for its entries alone.
     const int32_t* trow = a.tables + (int64_t)b * a.max_pages;
-    auto page = [&](int i) { return trow[min(i, a.max_pages - 1)]; };
+    auto page = [&](int i) {  // (atomic: a load that stays where it is written)
+        return __hip_atomic_load(trow + min(i, a.max_pages - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+    };
     const int t0 = split * a.tiles_per_split;
     const int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
+    const auto row = load_row<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, g);
     const int ctx = max(0, min(a.positions[b] + 1, a.ctx_limit));
     const int tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
     const int parts = max(1, (tiles + a.tiles_per_split - 1) / a.tiles_per_split);
@@ -81,9 +125,7 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
 #pragma unroll
     for (int t = 0; t < CH; t++) st.o[t] = f4{0.f, 0.f, 0.f, 0.f};
     if (t0 + wave < t1) {
-        const auto q =
-            load_query<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, a.qscale, g);
-        attend<CH, STREAM>(st, q, a.c, a.c.cache + a.c.layer_off + (int64_t)kv_h * a.c.record, t0 + wave, t1, a.waves,
+        attend<CH, STREAM>(st, row, a.qscale, a.c, a.c.cache + a.c.layer_off + (int64_t)kv_h * a.c.record, t0 + wave, t1, a.waves,
                            lane, kp, vp, page, [&](int t) { return ctx - t * KV_Q8_TILE - 16 * g; });
     }
 
