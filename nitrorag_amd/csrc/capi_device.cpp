@@ -1281,6 +1281,7 @@ static void launch_q8_prefill(nitro_kvpool* pool, int32_t layer, const float* q,
     a.item_rows = p.work_block_m;
     a.n_heads = n_heads;
     a.max_pages = p.max_pages;
+    a.num_cus = std::max(pool->num_cus, 1);
     a.qscale = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
     hip_check(launch_kv_q8_prefill(a, s), "kv_q8_prefill launch");
     pool->last_stream = s;

@@ -94,7 +94,7 @@ struct KvQ8Prefill {
     const int32_t* tables;
     const PrefillSeq* seqs;
     const int32_t* work;  // pairs (seq, first query row of the chunk)
-    int32_t work_items, item_rows, n_heads, max_pages;
+    int32_t work_items, item_rows, n_heads, max_pages, num_cus;
     float qscale;
 };
 hipError_t launch_kv_q8_prefill(const KvQ8Prefill& a, hipStream_t stream);

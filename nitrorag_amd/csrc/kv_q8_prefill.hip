@@ -12,7 +12,7 @@ namespace {
 // Tiles 0 .. end - 1 (end > 0) of the keys of one table row, two at a time.  K and V
 // come from the caches here (a prompt's rows read them again and again), and what
 // bounds the pass is the vector instructions around the products: V loads go out as
-// the scores are made, the next K's after the V products, so that two waves per SIMD
+// the scores are made, the next K's around the V products, so that two waves per SIMD
 // have the registers they need.  Of tile t the lane's column sees seen(t) tokens of
 // page lane / 16.  page(i): table entry i (any i).
 template <int CH, class Page, class Seen>
@@ -27,7 +27,8 @@ __device__ __forceinline__ void attend_pairs(State<CH>& st, const Query<(CH + 3)
         kp[h] = page(4 * h + sub), vp[h] = page(4 * h + g);
         load_k<CH, false>(k[h], record(c, base, kp[h]), record(c, base, vp[h]), lane);
     }
-    for (int t = 0; t < end; t += 2) {
+    int t = 0;
+    auto pair = [&](auto more) {
         f4 s[2][4];
         float top = -INFINITY, scales[2];
 #pragma unroll
@@ -36,14 +37,16 @@ __device__ __forceinline__ void attend_pairs(State<CH>& st, const Query<(CH + 3)
             const int keys = seen_on(c, vp[h], t + h < end ? seen(t + h) : 0, lane);
             top = fmaxf(top, scores<CH>(s[h], k[h], q, keys));
             scales[h] = k[h].vs;
-            kp[h] = page(4 * (t + 2 + h) + sub), vp[h] = page(4 * (t + 2 + h) + g);
+            if (more) kp[h] = page(4 * (t + 2 + h) + sub), vp[h] = page(4 * (t + 2 + h) + g);
         }
         const Weights<2> w = weigh<CH, 2>(st, s, top, q.scale, scales);
+        if (more) load_k<CH, false>(k[0], record(c, base, kp[0]), record(c, base, vp[0]), lane);
         add_values<CH, 2>(st, v, w);
-        if (t + 2 < end)
-#pragma unroll
-            for (int h = 0; h < 2; h++) load_k<CH, false>(k[h], record(c, base, kp[h]), record(c, base, vp[h]), lane);
-    }
+        if (more) load_k<CH, false>(k[1], record(c, base, kp[1]), record(c, base, vp[1]), lane);
+        t += 2;
+    };
+    while (t + 2 < end) pair(std::true_type());
+    pair(std::false_type());  // (on its own: a load that may be missing costs waits for all of them)
 }
 
 // A wave takes 16 query rows of one head as its columns; the workgroup's waves take
@@ -54,7 +57,13 @@ __device__ __forceinline__ void attend_pairs(State<CH>& st, const Query<(CH + 3)
 template <int CH>
 __global__ __launch_bounds__(256, CH <= 4 ? 3 : CH <= 8 ? 2 : 1) void kv_q8_prefill_kernel(KvQ8Prefill a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.n_heads, item = blockIdx.x / a.n_heads;
+    // The items come longest first.  Workgroups go round the CUs in order of their
+    // index, so every second round goes backwards: the CU that has the longest of one
+    // round has the shortest of the next.
+    const int round = blockIdx.x / a.num_cus, place = blockIdx.x - round * a.num_cus;
+    const int in_round = min(a.num_cus, (int)gridDim.x - round * a.num_cus);
+    const int w = round * a.num_cus + (round % 2 ? in_round - 1 - place : place);
+    const int h = w % a.n_heads, item = w / a.n_heads;
     const int b = a.work[2 * item];
     const PrefillSeq seq = a.seqs[b];
     const int col = lane & 15, g = lane >> 4, hd = a.c.head_dim;
