@@ -552,12 +552,9 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
 // streams at 6.7 TB/s; a workgroup begins in 2.5, and a split that has to be joined
 // costs 5 more.  Where a launch has more workgroups than are resident, they follow
 // one another as they finish; the last ones run alone.
-struct Q8DecodeShape {
-    int waves, tps, groups, splits;
-};
 template <class Ctx>
 Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_heads, int n_kv_heads, int head_dim) {
-    Q8DecodeShape best{};
+    Q8DecodeShape best;
     const int kv_mul = n_heads / n_kv_heads, hdp = kv_q8_padded(head_dim);
     best.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
     best.waves = kv_q8_decode_lds(n_heads, n_kv_heads, kv_q8_partial_floats(head_dim), 4, 1) <= KV_Q8_LDS ? 4 : 2;
@@ -613,18 +610,23 @@ KvQ8Decode q8_decode_args(const nitro_kvpool* pool, int layer, const float* q, f
 void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out, int n_heads, int n_kv_heads,
                       int head_dim, hipStream_t s) {
     DecodeBatch& d = pool->decode;
-    auto ctx = [&](int b) { return d.positions[b] + 1; };
-    const Q8DecodeShape sh = plan_q8_decode(pool, d.batch, ctx, n_heads, n_kv_heads, head_dim);
+    if (pool->q8_shape_generation != d.generation || pool->q8_shape_heads != n_heads) {  // once for a step's layers
+        pool->q8_shape = plan_q8_decode(pool, d.batch, [&](int b) { return d.positions[b] + 1; }, n_heads, n_kv_heads,
+                                        head_dim);
+        pool->q8_shape_generation = d.generation;
+        pool->q8_shape_heads = n_heads;
+    }
+    const Q8DecodeShape& sh = pool->q8_shape;
     KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh, d.shared_pages);
     if (a.num_splits > 1) {
-        pool->partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
-        if (pool->counters.reserve((size_t)d.batch * n_kv_heads * sh.groups))
-            hip_check(hipMemset(pool->counters.ptr, 0, pool->counters.count * sizeof(int32_t)), "hipMemset");
+        pool->q8_partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
+        if (pool->q8_counters.reserve((size_t)d.batch * n_kv_heads * sh.groups))
+            hip_check(hipMemset(pool->q8_counters.now.ptr, 0, pool->q8_counters.now.count * sizeof(int32_t)), "hipMemset");
     }
     a.tables = d.tables.ptr;
     a.positions = d.pos.ptr;
-    a.partials = pool->partials.ptr;
-    a.counters = pool->counters.ptr;
+    a.partials = pool->q8_partials.now.ptr;
+    a.counters = pool->q8_counters.now.ptr;
     a.batch = d.batch;
     a.max_pages = d.max_pages;
     a.ctx_limit = d.max_pages * BLOCK_SIZE;
@@ -913,6 +915,7 @@ int nitro_decode_batch_upload(nitro_kvpool* pool, const int32_t* tables, const i
     return guarded([&] {
         require_pool(pool);
         require(tables != nullptr && positions != nullptr, ERR_INVALID_ARGUMENT, "null array");
+        if (pool->q8) (void)kv_q8_layer(pool, 0);  // the current device is the pool's
         require(batch > 0 && max_pages > 0, ERR_INVALID_ARGUMENT, "batch and max_pages must be positive");
         for (int b = 0; b < batch; b++) check_table_rows(pool, tables, b, max_pages, positions[b]);
         DecodeBatch& d = pool->decode;
@@ -1108,6 +1111,7 @@ int nitro_prefill_batch_upload(nitro_kvpool* pool, const int32_t* tables, const 
         require_pool(pool);
         require(tables != nullptr && start_pos != nullptr && num_tokens != nullptr,
                 ERR_INVALID_ARGUMENT, "null array");
+        if (pool->q8) (void)kv_q8_layer(pool, 0);
         require(batch > 0 && max_pages > 0, ERR_INVALID_ARGUMENT, "batch and max_pages must be positive");
         PrefillBatch& p = pool->prefill;
         p.batch = 0;

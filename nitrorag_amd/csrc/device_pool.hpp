@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <memory>
 #include <string>
 #include <vector>
 
@@ -57,6 +58,23 @@ struct DeviceBuffer {
         reset();
         hip_check(hipMalloc((void**)&ptr, cap * sizeof(T)), "hipMalloc");
         count = cap;
+        return true;
+    }
+};
+
+// A device allocation that grows and keeps what it outgrew until it goes itself: a
+// captured launch may still hold the address.  (It at least doubles each time.)
+template <class T>
+struct KeptBuffer {
+    DeviceBuffer<T> now;
+    std::vector<std::unique_ptr<DeviceBuffer<T>>> outgrown;
+    bool reserve(size_t n) {
+        if (n <= now.count && now.ptr) return false;
+        auto bigger = std::make_unique<DeviceBuffer<T>>();
+        bigger->reserve(n > 2 * now.count ? n : 2 * now.count);
+        std::swap(bigger->ptr, now.ptr);
+        std::swap(bigger->count, now.count);
+        if (bigger->ptr) outgrown.push_back(std::move(bigger));
         return true;
     }
 };
@@ -223,6 +241,13 @@ struct PrefillBatch {
 
 }  // namespace nitro
 
+namespace nitro {
+// Launch shape of a decode over an 8-bit pool.
+struct Q8DecodeShape {
+    int waves = 0, tps = 0, groups = 0, splits = 0;  // waves per workgroup, tiles per split, head groups, splits at most
+};
+}  // namespace nitro
+
 struct nitro_model;
 
 struct nitro_kvpool {
@@ -253,6 +278,11 @@ struct nitro_kvpool {
     // An 8-bit pool (kv_q8.hpp) has its records here and no k / v.
     uint8_t* q8 = nullptr;
     int32_t q8_kv_heads = 0, q8_head_dim = 0;
+    nitro::KeptBuffer<float> q8_partials;    // split decode: acc, m, l per (b, split, head)
+    nitro::KeptBuffer<int32_t> q8_counters;  // arrivals per (b, K/V head, group of heads), zero between launches
+    nitro::Q8DecodeShape q8_shape;           // the decode plan last made ..
+    uint64_t q8_shape_generation = ~0ull;    // .. for this batch
+    int32_t q8_shape_heads = 0;              // .. and this many query heads
 };
 
 namespace nitro {

@@ -350,6 +350,38 @@ def test_captured_steps_replay():
         assert torch.equal(eager, out)
 
 
+def test_captured_decode_outlives_a_larger_launch():
+    """A captured split decode keeps its workspace when a later launch of the pool needs a larger one."""
+    import torch
+
+    heads = (4, 2, 64)
+    c = Case(14, [(1999, 1)], heads, spare=1000)
+    c.fill()
+    c.put()
+    c.cache.copy_(to_gpu(c.ref.data))
+    q = to_gpu(c.q)
+    out = torch.empty_like(q)
+    c.upload(False)
+    c.pool.decode(c.layer, q, out, *heads)
+    torch.cuda.synchronize()
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.pool.decode(c.layer, q, out, *heads)
+    tables = np.concatenate([c.tables[:, :120]] * 8)  # fits the uploaded tables' buffer
+    many = q.repeat(8, 1)
+    got = torch.empty_like(many)
+    c.pool.upload_decode_batch(tables, [1900] * 8)
+    c.pool.decode(c.layer, many, got, *heads)
+    assert torch.equal(got, got[:1].expand_as(got))
+    c.upload(False)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_on_another_stream():
     import torch
 
