@@ -162,10 +162,18 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  * rounded up to 16: K codes [4][hdp/16][4][16] (token 4a + r, dimension 16c + i at
  * [a][c][r][i]), V codes [hdp][16] (dimension, token), K scales [16], V scales [16].
  * create_q8 owns zero-filled memory, wrap_q8 borrows a caller's (16-byte aligned).
- *   A pool is used on the device that was current when it was made: calls with
- * another one current are refused.  nitro_kvpool_data and nitro_kvpool_wrap's
- * buffers do not exist for it (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape reports
- * kv_dim = n_kv_heads * head_dim. */
+ * In records that a caller writes itself, scales are not negative; a token with one that
+ * is not finite counts as NaN.
+ *   Attention takes q and K up to 1e36 in magnitude; parts of its output that come from V
+ * below 2^-96 may be zero.  Two rows of one batch that go to the same slot leave a mixture
+ * of both there, as in an fp32 pool.
+ *   A pool holds less than 512 GiB and is used on the device that was current when it was
+ * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  Its
+ * workspace for splits stays where it is until the pool goes, so a captured
+ * nitro_paged_attn_decode may be replayed after launches that needed more; as for an fp32
+ * pool, launches that overlap on one pool race on it.  nitro_kvpool_data has nothing to
+ * give (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape reports kv_dim = n_kv_heads *
+ * head_dim. */
 int nitro_kvpool_create_q8(int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
                            nitro_kvpool** out);
 int nitro_kvpool_wrap_q8(void* cache, int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
@@ -354,7 +362,7 @@ int nitro_q8_tile_rows(int32_t launch, int32_t batch, int32_t n, int32_t d, int3
  * rms_ffn f32, w1 w2 w3 Q8, rms_final f32, freq_cis_real, freq_cis_imag f32.
  * The weights are copied to the device; the caller may free the blob.  The
  * pool used with a model must have n_layers layers and kv_dim =
- * n_kv_heads * dim / n_heads.  The first forward with more than 4 rows of
+ * n_kv_heads * dim / n_heads (an 8-bit pool: n_kv_heads heads of dim / n_heads).  The first forward with more than 4 rows of
  * full-row products (NITRO_Q8_FULL_ROWS) allocates and builds a tile-layout
  * copy of the Q8 matrices (1.125 bytes per weight) that those products read;
  * a caller capturing such forwards into a graph runs one first.

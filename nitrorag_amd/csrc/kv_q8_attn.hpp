@@ -35,6 +35,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // caller's rows
 
 constexpr float FIXED = 8355000.0f;  // below 127 * 65536 + 127 * 256 + 127, the largest three digits hold
+constexpr float UNIT = 0x1p-20f;  // between a score's two factors
 // Least W that fixed point takes (FIXED / W stays in fp32's range).
 constexpr float LEAST = 0x1p-104f;
 
@@ -126,7 +127,7 @@ __device__ __forceinline__ Query<NC> query_of(const QueryRow<NC>& from, float qs
     const float inv = top >= 0x1p-100f ? FIXED / top : 0.0f;
     Query<NC> q;
     // (never 0: a hidden key's -infinity stays one)
-    q.scale = (top >= 0x1p-100f ? top : 0x1p-100f) * (qscale * (256.0f * 0x1p24f / FIXED)) + bad;
+    q.scale = (top >= 0x1p-100f ? top : 0x1p-100f) * (qscale * (256.0f / UNIT / FIXED)) + bad;
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
@@ -213,7 +214,9 @@ __device__ __forceinline__ int joined(int x2, int x1) { return (int)(((uint32_t)
 template <int CH>
 __device__ __forceinline__ float scores(f4 (&s)[4], const KTile<CH>& x, const Query<(CH + 3) / 4>& q, int keys) {
     constexpr int NC = (CH + 3) / 4;
-    const float ks = x.ks * 0x1p-24f;  // (a score before the query's factor is in the range of its key)
+    // (a score before the query's factor stays in fp32's range; a token with a scale
+    // that is not finite gives NaN by its score)
+    const float ks = fabsf(x.ks) + fabsf(x.vs) < INFINITY ? x.ks * UNIT : __uint_as_float(0x7fc00000u);
     i4 x2[4], x1[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -241,8 +244,8 @@ __device__ __forceinline__ float scores(f4 (&s)[4], const KTile<CH>& x, const Qu
     return column_max(top);
 }
 
-// The weights' three digits, from the scores and the V scales.  (A NaN scale there
-// is a hidden slot's, or comes with a K scale that makes the sum NaN.)  H: tiles that
+// The weights' three digits, from the scores and the V scales.  (A scale there that is
+// not finite is a hidden slot's, or its token's score is NaN.)  H: tiles that
 // share a maximum and a unit, so that their products are added up as integers: what
 // takes an output's integers to fp32 (five operations) is then paid once for them.
 template <int H>

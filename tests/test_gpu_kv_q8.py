@@ -231,6 +231,47 @@ def test_nonfinite_tokens_reach_the_queries_that_see_them():
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_scales_that_are_not_finite(which, value):
+    """Either scale of a visible token (a caller's own records) makes the outputs that see it NaN."""
+    import torch
+
+    heads = (4, 2, 64)
+    c = Case(15, [(0, 90)], heads)
+    c.put()
+    data = c.ref.data.copy()
+    at = 32 * 64 + 64 * which + 4 * (37 % 16)
+    data[c.tables[0, 37 // 16], c.layer, 1, at:at + 4] = np.array([value], np.float32).view(np.uint8)
+    c.cache.copy_(to_gpu(data))
+    c.upload(True)
+    out = torch.full((90, 256), 5.0, device="cuda")
+    c.pool.prefill(c.layer, to_gpu(c.q), out, *heads)
+    want = np.zeros((90, 4), bool)
+    want[37:, 2:] = True
+    np.testing.assert_array_equal(np.isnan(c.heads(out.cpu().numpy())).all(-1), want)
+    c.pool.upload_decode_batch(c.tables, [89])
+    one = torch.full((1, 256), 5.0, device="cuda")
+    c.pool.decode(c.layer, to_gpu(c.q[89:]), one, *heads)
+    np.testing.assert_array_equal(np.isnan(c.heads(one.cpu().numpy())).all(-1), want[89:])
+
+
+@pytest.mark.parametrize("q_scale,k_scale", [(1e29, 1e-29), (1e-29, 1e29), (1e36, 1e-29), (1e-29, 1e36)])
+def test_scores_of_far_apart_magnitudes(q_scale, k_scale):
+    """q and K of which one is near fp32's end; products up to 1e9 are one-hot weights."""
+    import torch
+
+    heads = (2, 2, 64)
+    c = Case(16, [(0, 70)], heads)
+    c.q *= np.float32(q_scale)
+    c.k *= np.float32(k_scale)
+    c.upload(True)
+    out = torch.full((70, 128), float("nan"), device="cuda")
+    c.pool.prefill_append(c.layer, to_gpu(c.q), to_gpu(c.k), to_gpu(c.v), out, *heads)
+    c.put()
+    c.check(out, "magnitudes")
+
+
 # ------------------------------------------------------------------ prefill
 
 @pytest.mark.parametrize("spans", [[(0, 1)], [(0, 16), (0, 0), (0, 17)], [(0, 200), (63, 65), (5, 1)], [(129, 70)]])
