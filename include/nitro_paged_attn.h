@@ -170,8 +170,10 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  *   A pool holds less than 512 GiB and is used on the device that was current when it was
  * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  Its
  * workspace for splits stays where it is until the pool goes, so a captured
- * nitro_paged_attn_decode may be replayed after launches that needed more; as for an fp32
- * pool, launches that overlap on one pool race on it.  nitro_kvpool_data has nothing to
+ * nitro_paged_attn_decode may be replayed after launches that needed more, also over a
+ * later upload of as many sequences and the same max_pages, whatever their lengths
+ * (prefill calls: of as many rows, in any number of chunks); as for an fp32 pool,
+ * launches that overlap on one pool race on it.  nitro_kvpool_data has nothing to
  * give (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape reports kv_dim = n_kv_heads *
  * head_dim. */
 int nitro_kvpool_create_q8(int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,

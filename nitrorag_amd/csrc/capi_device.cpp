@@ -620,8 +620,10 @@ void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out,
     KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh, d.shared_pages);
     if (a.num_splits > 1) {
         pool->q8_partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
-        if (pool->q8_counters.reserve((size_t)d.batch * n_kv_heads * sh.groups))
+        if (pool->q8_counters.reserve((size_t)d.batch * n_kv_heads * sh.groups)) {
             hip_check(hipMemset(pool->q8_counters.now.ptr, 0, pool->q8_counters.now.count * sizeof(int32_t)), "hipMemset");
+            hip_check(hipStreamSynchronize(nullptr), "hipStreamSynchronize");  // s need not wait for the null stream
+        }
     }
     a.tables = d.tables.ptr;
     a.positions = d.pos.ptr;
@@ -635,21 +637,24 @@ void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out,
     pool->last_stream = s;
 }
 
-// The rows of the uploaded decode or prefill batch.
+// The rows of the uploaded decode or prefill batch, a prefill's by whole pages from
+// 2^19 values on where chunks have 16 rows or more: a wave takes its pages' rows
+// together, a longer way than the rows' own waves have.  By rows and by pages, in us, 8
+// heads of 128: 256 rows in chunks of 64 4.7 and 6.8, 512 rows 6.5 and 6.8, 1024 10.3
+// and 6.8, 4096 29 and 12.6; in chunks of 8 512 rows 7.0 and 10.5, 1024 11.0 and 10.9,
+// 4096 30 and 18.9; 8 heads of 64, chunks of 64: 512 rows 4.6 and 5.2, 1024 6.4 and 5.4.
 KvQ8Rows q8_rows(const nitro_kvpool* pool, bool prefill) {
     const DecodeBatch& d = pool->decode;
     const PrefillBatch& p = pool->prefill;
-    return prefill ? KvQ8Rows{p.slots.ptr, p.row_pos.ptr, p.total_rows} : KvQ8Rows{d.slots.ptr, d.pos.ptr, d.batch};
-}
-KvQ8Chunks q8_chunks(const nitro_kvpool* pool, bool prefill) {
-    const PrefillBatch& p = pool->prefill;
-    return prefill ? KvQ8Chunks{p.seqs.ptr, p.work.ptr, p.work_items, p.work_block_m} : KvQ8Chunks{};
+    if (!prefill) return KvQ8Rows{d.slots.ptr, d.pos.ptr, d.batch, false};
+    const bool together = (long long)p.total_rows * pool->kv_dim >= 1 << 19 && p.total_rows / 16 >= p.batch;
+    return KvQ8Rows{p.slots.ptr, p.row_pos.ptr, p.total_rows, together};
 }
 
 // Appends the batch's rows (fr, fi: after rotating q and k).
 void append_q8(nitro_kvpool* pool, int layer, bool prefill, float* q, float* k, const float* v, const float* fr,
                const float* fi, int n_heads, hipStream_t s) {
-    hip_check(launch_kv_q8_append(kv_q8_layer(pool, layer), q8_rows(pool, prefill), q8_chunks(pool, prefill), q, k, v, fr,
+    hip_check(launch_kv_q8_append(kv_q8_layer(pool, layer), q8_rows(pool, prefill), q, k, v, fr,
                                   fi, n_heads, s),
               "kv_q8_append launch");
     pool->last_stream = s;
@@ -864,7 +869,7 @@ static int kv_read(nitro_kvpool* pool, int32_t layer, float* k, float* v, bool p
         require((prefill ? pool->prefill.batch : pool->decode.batch) > 0, ERR_NO_BATCH,
                 prefill ? "no prefill batch uploaded" : "no decode batch uploaded");
         hipStream_t s = as_stream(stream);
-        hip_check(launch_kv_q8_read(kv_q8_layer(pool, layer), q8_rows(pool, prefill), q8_chunks(pool, prefill), k, v, s),
+        hip_check(launch_kv_q8_read(kv_q8_layer(pool, layer), q8_rows(pool, prefill), k, v, s),
                   "kv_q8_read launch");
         pool->last_stream = s;
     });
@@ -1164,7 +1169,7 @@ int nitro_prefill_batch_upload(nitro_kvpool* pool, const int32_t* tables, const 
         int32_t* h_wide = st.part(p.work_wide.ptr, n_wide);
         std::memcpy(h_tables, tables, nt * sizeof(int32_t));
         for (int b = 0; b < batch; b++) {
-            const PrefillSeq seq{start_pos[b], num_tokens[b], row_off[b], 0};
+            const PrefillSeq seq{start_pos[b], num_tokens[b], row_off[b], (int32_t)items.size()};
             std::memcpy(h_seqs + 4 * (size_t)b, &seq, sizeof(seq));
         }
         for (int b = 0; b < batch; b++)

@@ -215,7 +215,8 @@ struct DecodeBatch {
 // arrays cost a launch three cache lines: 406.6 us for 12 launches over 8 prompts,
 // 402.3 so).
 struct PrefillSeq {
-    int32_t start_pos, num_tokens, row_off, unused;
+    int32_t start_pos, num_tokens, row_off;
+    int32_t work_items;  // of the batch, the same for each (a launch that was captured over another batch reads it)
 };
 
 struct PrefillBatch {

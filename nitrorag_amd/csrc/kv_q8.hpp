@@ -31,28 +31,24 @@ struct KvQ8 {
 };
 
 // New rows of a step: row r lies at position pos[r] in slot slots[r] (page * 16
-// + position % 16).
+// + position % 16).  together: they are mostly chunks, consecutive rows of one
+// sequence, and taken by whole pages (any rows would come out the same).
 struct KvQ8Rows {
     const int32_t* slots;
     const int32_t* pos;
     int32_t rows;
+    bool together;
 };
 
 struct PrefillSeq;
-// The same rows as chunks of sequences, in items of item_rows consecutive rows.
-struct KvQ8Chunks {
-    const PrefillSeq* seqs = nullptr;
-    const int32_t* work = nullptr;  // pairs (seq, first row of the item in its chunk)
-    int32_t work_items = 0, item_rows = 0;
-};
 
 // Appends k, v [rows][kv_heads * head_dim].  With freq_real, q [rows][n_heads *
-// head_dim] and k are first rotated in place.  chunks: the rows are also these.
-hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& chunks, float* q, float* k,
+// head_dim] and k are first rotated in place.
+hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k,
                                const float* v, const float* freq_real, const float* freq_imag, int n_heads,
                                hipStream_t stream);
 // k, v = the values that those slots hold.
-hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& chunks, float* k, float* v,
+hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v,
                              hipStream_t stream);
 
 // Keys that a wave takes at a time: four pages.

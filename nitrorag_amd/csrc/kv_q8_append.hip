@@ -31,6 +31,7 @@ namespace {
 
 constexpr int THREADS = 256;
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f2 __attribute__((ext_vector_type(2), aligned(4)));
 
 constexpr float LEAST = 0x1p-100f;
 
@@ -71,8 +72,9 @@ __device__ __forceinline__ float head_max(float x) {
     return x;
 }
 
-__device__ __forceinline__ f4 rotated(f4 x, const float* fr, const float* fi) {
-    const double c0 = fr[0], s0 = fi[0], c1 = fr[1], s1 = fi[1];
+__device__ __forceinline__ f2 pair(const float* p) { return *reinterpret_cast<const f2*>(p); }
+__device__ __forceinline__ f4 rotated(f4 x, f2 fr, f2 fi) {
+    const double c0 = fr.x, s0 = fi.x, c1 = fr.y, s1 = fi.y;
     const double x0 = x.x, x1 = x.y, x2 = x.z, x3 = x.w;
     f4 r;
     r.x = (float)(x0 * c0 - x1 * s0);
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(THREADS) void kv_q8_append_kernel(KvQ8 c, KvQ8Rows 
             if (!query) vx = *reinterpret_cast<const f4*>(v + ((int64_t)row * c.kv_heads + h) * c.head_dim + dim);
             if (ROPE) {
                 const int64_t at = (int64_t)pos * (c.head_dim / 2) + dim / 2;
-                x = rotated(x, freq_real + at, freq_imag + at);
+                x = rotated(x, pair(freq_real + at), pair(freq_imag + at));
                 *reinterpret_cast<f4*>(x_at) = x;
             }
         }
@@ -235,91 +237,102 @@ __device__ __forceinline__ float page_max(float x) {  // over dg
     return max_across_32(max_across_16(x));
 }
 
-// Where a wave's page lies: its rows are first .. first + count - 1 of the packed
-// ones, tokens t0 .. t0 + count - 1 of the page.
+// Rows of one page: first .. first + count - 1 of the packed ones, tokens t0 .. t0 +
+// count - 1 of the page; pos: the first one's position.
 struct PageRows {
-    int first, count, t0, page;
+    int first, count, t0, page, pos;
 };
-// Page `which` (0 .. item_rows / 16) of an item: the pages whose first row of the
-// chunk is one of the item's rows.  count = 0: the item has no such page.
-__device__ __forceinline__ PageRows page_rows(const KvQ8Rows& rows, const KvQ8Chunks& ch, int item, int which) {
-    const PrefillSeq seq = ch.seqs[ch.work[2 * item]];
-    const int q0 = ch.work[2 * item + 1];
-    const int page = (q0 == 0 ? seq.start_pos : seq.start_pos + q0 + 15) / 16 + which;
-    const int from = max(page * 16 - seq.start_pos, 0);  // in the chunk
-    PageRows p{0, 0, 0, 0};
-    if (from >= min(seq.num_tokens, q0 + ch.item_rows)) return p;
-    p.first = seq.row_off + from;
-    const int slot = rows.slots[p.first];
-    p.t0 = slot & 15;
-    p.page = slot >> 4;
-    p.count = min(16 - p.t0, seq.num_tokens - from);
-    return p;
+// The pages that begin (with the page, or with a chunk) in rows 64 block .. + 64 are
+// dealt to five waves: four pages where all are whole, a fifth where chunks meet.
+constexpr int PAGE_BLOCK = 64, PAGE_WAVES = 5;
+// f(lane, PageRows) for each page of wave `rest` % 5 of block `rest` / 5, the same in all
+// lanes.  Found from the rows' slots and positions alone, so that a captured launch
+// works on any batch of as many rows.
+template <class F>
+__device__ __forceinline__ void each_page(const KvQ8Rows& rows, int64_t rest, F f) {
+    const int64_t base = rest / PAGE_WAVES * PAGE_BLOCK;
+    if (base >= rows.rows) return;
+    const int lane = threadIdx.x & 63, row = (int)base + lane;
+    const bool in = row < rows.rows, in_after = lane < 16 && row + PAGE_BLOCK < rows.rows;
+    // (all loads at once)
+    const int here = in ? row : 0, later = in_after ? row + PAGE_BLOCK : here;
+    const int at[4] = {here, max(here - 1, 0), later, max(later - 1, 0)};
+    int slots[4], pos[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) slots[i] = rows.slots[at[i]], pos[i] = rows.pos[at[i]];
+    // does a row go on where the one before it ends?
+    auto follows = [&](int i) {
+        return (slots[i] & 15) != 0 && slots[i] == slots[i + 1] + 1 && pos[i] == pos[i + 1] + 1;
+    };
+    const uint64_t next = __builtin_amdgcn_ballot_w64(in && row > 0 && follows(0));
+    const uint64_t after = __builtin_amdgcn_ballot_w64(in_after && follows(2));
+    uint64_t starts = __builtin_amdgcn_ballot_w64(in) & ~next;
+    for (int i = (int)(rest % PAGE_WAVES); i > 0; i--) starts &= starts - 1;
+    while (starts) {
+        int self = lane;
+        asm volatile("" : "+v"(self));  // (what follows from the lane is made anew, not kept in registers)
+        const int i = __builtin_ctzll(starts);
+        const uint64_t run = (next >> i >> 1) | (after << (63 - i));  // (15 follow at most)
+        const int slot = __builtin_amdgcn_readlane(slots[0], i);
+        f(self, PageRows{(int)base + i, 1 + __builtin_ctzll(~run), slot & 15, slot >> 4,
+                         __builtin_amdgcn_readlane(pos[0], i)});
+        for (int n = 0; n < PAGE_WAVES; n++) starts &= starts - 1;
+    }
 }
 
 typedef int i4 __attribute__((ext_vector_type(4)));
 
-// J = hdp / 64, rounded up.  Workgroups past page_blocks rotate q.
+// J = hdp / 64, rounded up.
 template <int J, bool ROPE>
-__global__ __launch_bounds__(THREADS) void kv_q8_append_pages_kernel(KvQ8 c, KvQ8Rows rows, KvQ8Chunks ch,
-                                                                     float* __restrict__ q, float* __restrict__ k,
-                                                                     const float* __restrict__ v,
-                                                                     const float* __restrict__ freq_real,
-                                                                     const float* __restrict__ freq_imag, int n_heads,
-                                                                     unsigned page_blocks) {
-    if (ROPE && blockIdx.x >= page_blocks) {
-        const int per_row = n_heads * c.head_dim / 4;  // float4
-        const int64_t total = (int64_t)rows.rows * per_row;
-        for (int64_t i = (int64_t)(blockIdx.x - page_blocks) * THREADS + threadIdx.x; i < total;
-             i += (int64_t)(gridDim.x - page_blocks) * THREADS) {
-            const int row = (int)(i / per_row), dim = (int)(i - (int64_t)row * per_row) * 4 % c.head_dim;
-            const int64_t at = (int64_t)rows.pos[row] * (c.head_dim / 2) + dim / 2;
-            f4* x = reinterpret_cast<f4*>(q + 4 * i);
-            *x = rotated(*x, freq_real + at, freq_imag + at);
-        }
-        return;
-    }
-    const int pages = ch.item_rows / 16 + 1;
-    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
-    const int h = (int)(unit % c.kv_heads);
-    const int64_t rest = unit / c.kv_heads;
-    if (rest >= (int64_t)ch.work_items * pages) return;
-    const PageRows p = page_rows(rows, ch, (int)(rest / pages), (int)(rest % pages));
-    if (p.count == 0) return;
-    const int lane = threadIdx.x & 63, tq = lane & 3, dg = lane >> 2;
-
+__device__ __forceinline__ void append_page(const KvQ8& c, const PageRows& p, int h, int lane, float* __restrict__ k,
+                                            const float* __restrict__ v, const float* __restrict__ freq_real,
+                                            const float* __restrict__ freq_imag) {
+    const int tq = lane & 3, dg = lane >> 2;
     f4 kx[J][4], vx[J][4];
-    float ka[4] = {0.f, 0.f, 0.f, 0.f}, va[4] = {0.f, 0.f, 0.f, 0.f}, bad[4] = {0.f, 0.f, 0.f, 0.f};
+    f2 fr[J][4], fi[J][4];
     bool here[4];
+    // (lanes without a row of their own load the page's last one: no branches between the loads)
+    int row[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        here[r] = (unsigned)(4 * tq + r - p.t0) < (unsigned)p.count;
+        row[r] = min(max(4 * tq + r - p.t0, 0), p.count - 1);
+        here[r] = row[r] == 4 * tq + r - p.t0;
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int dim = 64 * j + 4 * dg;
+#pragma unroll
+        for (int r = 0; r < 4; r++) kx[j][r] = vx[j][r] = f4{0.f, 0.f, 0.f, 0.f}, fr[j][r] = fi[j][r] = f2{0.f, 0.f};
+        if (dim < c.head_dim) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int64_t at = ((int64_t)(p.first + row[r]) * c.kv_heads + h) * c.head_dim + dim;
+                kx[j][r] = *reinterpret_cast<const f4*>(k + at);
+                vx[j][r] = *reinterpret_cast<const f4*>(v + at);
+                if (ROPE) {
+                    const int64_t f = (int64_t)(p.pos + row[r]) * (c.head_dim / 2) + dim / 2;
+                    fr[j][r] = pair(freq_real + f);
+                    fi[j][r] = pair(freq_imag + f);
+                }
+            }
+        }
+    }
+    float ka[4] = {0.f, 0.f, 0.f, 0.f}, va[4] = {0.f, 0.f, 0.f, 0.f}, bad[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const int dim = 64 * j + 4 * dg;
-            kx[j][r] = vx[j][r] = f4{0.f, 0.f, 0.f, 0.f};
-            if (here[r] && dim < c.head_dim) {
+            const bool in = here[r] && dim < c.head_dim;
+            if (ROPE) {
+                kx[j][r] = rotated(kx[j][r], fr[j][r], fi[j][r]);
                 const int64_t at = ((int64_t)(p.first + 4 * tq + r - p.t0) * c.kv_heads + h) * c.head_dim + dim;
-                kx[j][r] = *reinterpret_cast<const f4*>(k + at);
-                vx[j][r] = *reinterpret_cast<const f4*>(v + at);
+                if (in) *reinterpret_cast<f4*>(k + at) = kx[j][r];
             }
+            const f4 zero = {0.f, 0.f, 0.f, 0.f};
+            kx[j][r] = here[r] ? kx[j][r] : zero;
+            vx[j][r] = here[r] ? vx[j][r] : zero;
         }
-    }
-    if (ROPE) {
-        const int64_t pos = rows.pos[p.first] - p.t0;  // of token 0
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int j = 0; j < J; j++) {
-                const int dim = 64 * j + 4 * dg;
-                if (here[r] && dim < c.head_dim) {
-                    const int64_t f = (pos + 4 * tq + r) * (c.head_dim / 2) + dim / 2;
-                    kx[j][r] = rotated(kx[j][r], freq_real + f, freq_imag + f);
-                    const int64_t at = ((int64_t)(p.first + 4 * tq + r - p.t0) * c.kv_heads + h) * c.head_dim + dim;
-                    *reinterpret_cast<f4*>(k + at) = kx[j][r];
-                }
-            }
-    }
     float ks[4], vs[4], ki[4], vi[4];
     bool good[4];
 #pragma unroll
@@ -375,17 +388,36 @@ __global__ __launch_bounds__(THREADS) void kv_q8_append_pages_kernel(KvQ8 c, KvQ
     }
 }
 
-template <int J>
-__global__ __launch_bounds__(THREADS) void kv_q8_read_pages_kernel(KvQ8 c, KvQ8Rows rows, KvQ8Chunks ch,
-                                                                   float* __restrict__ k, float* __restrict__ v) {
-    const int pages = ch.item_rows / 16 + 1;
-    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
+// Workgroups past page_blocks rotate q.
+template <int J, bool ROPE>
+__global__ __launch_bounds__(THREADS) void kv_q8_append_pages_kernel(KvQ8 c, KvQ8Rows rows, float* __restrict__ q,
+                                                                     float* __restrict__ k, const float* __restrict__ v,
+                                                                     const float* __restrict__ freq_real,
+                                                                     const float* __restrict__ freq_imag, int n_heads,
+                                                                     unsigned page_blocks) {
+    if (ROPE && blockIdx.x >= page_blocks) {
+        const int per_row = n_heads * c.head_dim / 4;  // float4
+        const int64_t total = (int64_t)rows.rows * per_row;
+        for (int64_t i = (int64_t)(blockIdx.x - page_blocks) * THREADS + threadIdx.x; i < total;
+             i += (int64_t)(gridDim.x - page_blocks) * THREADS) {
+            const int row = (int)(i / per_row), dim = (int)(i - (int64_t)row * per_row) * 4 % c.head_dim;
+            const int64_t at = (int64_t)rows.pos[row] * (c.head_dim / 2) + dim / 2;
+            f4* x = reinterpret_cast<f4*>(q + 4 * i);
+            *x = rotated(*x, pair(freq_real + at), pair(freq_imag + at));
+        }
+        return;
+    }
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)(unit % c.kv_heads);
-    const int64_t rest = unit / c.kv_heads;
-    if (rest >= (int64_t)ch.work_items * pages) return;
-    const PageRows p = page_rows(rows, ch, (int)(rest / pages), (int)(rest % pages));
-    if (p.count == 0) return;
-    const int lane = threadIdx.x & 63, tq = lane & 3, dg = lane >> 2;
+    each_page(rows, unit / c.kv_heads, [&](int lane, const PageRows& p) {
+        append_page<J, ROPE>(c, p, h, lane, k, v, freq_real, freq_imag);
+    });
+}
+
+template <int J>
+__device__ __forceinline__ void read_page(const KvQ8& c, const PageRows& p, int h, int lane, float* __restrict__ k,
+                                          float* __restrict__ v) {
+    const int tq = lane & 3, dg = lane >> 2;
     if (p.page < 0 || p.page >= c.num_pages) {
         if (lane == 0 && h == 0) atomicAdd(c.bad_pages, p.count);
         return;
@@ -419,27 +451,36 @@ __global__ __launch_bounds__(THREADS) void kv_q8_read_pages_kernel(KvQ8 c, KvQ8R
     }
 }
 
+template <int J>
+__global__ __launch_bounds__(THREADS) void kv_q8_read_pages_kernel(KvQ8 c, KvQ8Rows rows, float* __restrict__ k,
+                                                                   float* __restrict__ v) {
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = (int)(unit % c.kv_heads);
+    each_page(rows, unit / c.kv_heads, [&](int lane, const PageRows& p) { read_page<J>(c, p, h, lane, k, v); });
+}
+
 unsigned groups(int64_t units, int lph) {
     const int64_t per = THREADS / lph, g = (units + per - 1) / per;
     return (unsigned)(g < 1 ? 1 : g > 65536 ? 65536 : g);
 }
-// Workgroups that take the pages of a batch's chunks.
-int64_t page_groups(const KvQ8& c, const KvQ8Chunks& ch) {
-    return ((int64_t)ch.work_items * (ch.item_rows / 16 + 1) * c.kv_heads + THREADS / 64 - 1) / (THREADS / 64);
+// Workgroups that take a batch by its pages.
+int64_t page_groups(const KvQ8& c, const KvQ8Rows& r) {
+    const int64_t waves = ((int64_t)r.rows + PAGE_BLOCK - 1) / PAGE_BLOCK * PAGE_WAVES * c.kv_heads;
+    return (waves + THREADS / 64 - 1) / (THREADS / 64);
 }
 
 template <int J>
-void append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* q, float* k, const float* v, const float* fr,
+void append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k, const float* v, const float* fr,
             const float* fi, int n_heads, hipStream_t s) {
     constexpr int LPH = J == 1 ? 16 : J == 2 ? 32 : 64;
-    if (ch.work_items) {
-        const unsigned pages = (unsigned)page_groups(c, ch);
+    if (r.together) {
+        const unsigned pages = (unsigned)page_groups(c, r);
         const unsigned turn = fr ? groups((int64_t)r.rows * n_heads * c.head_dim / 4, 1) : 0;
         if (fr)
-            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, true>), dim3(pages + turn), dim3(THREADS), 0, s, c, r, ch, q,
+            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, true>), dim3(pages + turn), dim3(THREADS), 0, s, c, r, q,
                                k, v, fr, fi, n_heads, pages);
         else
-            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, false>), dim3(pages), dim3(THREADS), 0, s, c, r, ch, q, k, v,
+            hipLaunchKernelGGL((kv_q8_append_pages_kernel<J, false>), dim3(pages), dim3(THREADS), 0, s, c, r, q, k, v,
                                fr, fi, n_heads, pages);
         return;
     }
@@ -453,10 +494,10 @@ void append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* q, fl
 }
 
 template <int J>
-void read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* k, float* v, hipStream_t s) {
+void read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v, hipStream_t s) {
     constexpr int LPH = J == 1 ? 16 : J == 2 ? 32 : 64;
-    if (ch.work_items)
-        hipLaunchKernelGGL((kv_q8_read_pages_kernel<J>), dim3((unsigned)page_groups(c, ch)), dim3(THREADS), 0, s, c, r, ch,
+    if (r.together)
+        hipLaunchKernelGGL((kv_q8_read_pages_kernel<J>), dim3((unsigned)page_groups(c, r)), dim3(THREADS), 0, s, c, r,
                            k, v);
     else
         hipLaunchKernelGGL((kv_q8_read_kernel<LPH>), dim3(groups((int64_t)r.rows * c.kv_heads, LPH)), dim3(THREADS), 0, s,
@@ -464,27 +505,27 @@ void read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* k, floa
 }
 
 // The pages' workgroups have a grid index each.
-bool fits(const KvQ8& c, const KvQ8Chunks& ch) {
-    return c.head_dim >= 4 && c.head_dim <= 256 && c.head_dim % 4 == 0 && ch.item_rows % 16 == 0 &&
-           page_groups(c, ch) <= INT32_MAX - 65536;
+bool fits(const KvQ8& c, const KvQ8Rows& r) {
+    return c.head_dim >= 4 && c.head_dim <= 256 && c.head_dim % 4 == 0 &&
+           page_groups(c, r) <= INT32_MAX - 65536;
 }
 
 }  // namespace
 
-hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* q, float* k,
+hipError_t launch_kv_q8_append(const KvQ8& c, const KvQ8Rows& r, float* q, float* k,
                                const float* v, const float* freq_real, const float* freq_imag, int n_heads,
                                hipStream_t stream) {
-    if (!fits(c, ch)) return hipErrorInvalidValue;
+    if (!fits(c, r)) return hipErrorInvalidValue;
     auto* const f = c.hdp <= 64 ? append<1> : c.hdp <= 128 ? append<2> : c.hdp <= 192 ? append<3> : append<4>;
-    f(c, r, ch, q, k, v, freq_real, freq_imag, n_heads, stream);
+    f(c, r, q, k, v, freq_real, freq_imag, n_heads, stream);
     return hipGetLastError();
 }
 
-hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, const KvQ8Chunks& ch, float* k, float* v,
+hipError_t launch_kv_q8_read(const KvQ8& c, const KvQ8Rows& r, float* k, float* v,
                              hipStream_t stream) {
-    if (!fits(c, ch)) return hipErrorInvalidValue;
+    if (!fits(c, r)) return hipErrorInvalidValue;
     auto* const f = c.hdp <= 64 ? read<1> : c.hdp <= 128 ? read<2> : c.hdp <= 192 ? read<3> : read<4>;
-    f(c, r, ch, k, v, stream);
+    f(c, r, k, v, stream);
     return hipGetLastError();
 }
 

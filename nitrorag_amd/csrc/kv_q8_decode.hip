@@ -2,8 +2,8 @@
 // split over workgroups (the products and the softmax: kv_q8_attn.hpp).
 //
 // Bound by bytes: 2 * head_dim + 8 per key and K/V head.  64 x 4096 tokens at 32 x 128
-// take 328 us (6.74 TB/s, what this card streams; 56% of the cycles on vector
-// instructions), one sequence of 131072 at 32/8 x 128 50 us (5.5 TB/s: start, two tile
+// take 328 us (6.74 TB/s, what this card streams; vector instructions in a third of the
+// SIMDs' cycles), one sequence of 131072 at 32/8 x 128 50 us (5.5 TB/s: start, two tile
 // rounds' latency and the join of 64 splits are 9 us), 24 of 512 to 8192 43 us (the
 // same, and splits of unequal length), 32 of 16 to 1024 at 12 x 64 11 us and one of
 // 256 5 us (latency: launch, table entry, K/V, products, join).
@@ -94,8 +94,8 @@ constexpr int JOIN = 16;  // partials whose loads go out together
 
 // A workgroup takes one split of one sequence's keys for up to 16 query heads of a
 // K/V head; its waves take the split's tiles in turn.  Waves per SIMD are what the
-// registers allow without spills (at head size 128, 183 of them: three waves with 13
-// spilled took 404 us where two take 337).
+// registers allow without spills (at head size 128 208; an earlier form had 183, and
+// three waves with 13 of them spilled took 404 us where two took 337).
 template <int CH, bool STREAM>
 __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_decode_kernel(KvQ8Decode a) {
     extern __shared__ float s_part[];  // [waves][cols][pstride], then of a join [cols][parts] factors and [cols] sums
@@ -125,15 +125,20 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     auto page = [&](int i) {  // (atomic: a load that stays where it is written)
         return __hip_atomic_load(trow + min(i, a.max_pages - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
     };
-    const int t0 = split * a.tiles_per_split;
-    const int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
+    int tps = a.tiles_per_split, t0 = split * tps;
+    int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
     const auto row = load_row<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, g);
-    const int ctx = max(0, min(a.positions[b] + 1, a.ctx_limit));
+    const int ctx = max(0, min(a.positions[b], a.ctx_limit - 1) + 1);
     const int tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
-    const int parts = max(1, (tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+    if (tiles > a.num_splits * tps) {  // a captured launch, replayed over a later batch with a longer sequence
+        tps = (tiles + a.num_splits - 1) / a.num_splits;
+        t0 = split * tps;
+        kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
+    }
+    const int parts = max(1, (tiles + tps - 1) / tps);
     if (split >= parts) return;
     if (ctx == 0 && hg == 0 && kv_h == 0 && threadIdx.x == 0) atomicAdd(a.c.bad_pages, 1);  // a position below 0
-    const int t1 = min(tiles, t0 + a.tiles_per_split);
+    const int t1 = min(tiles, t0 + tps);
 
     State<CH> st;
 #pragma unroll

@@ -57,21 +57,9 @@ __device__ __forceinline__ void attend_pairs(State<CH>& st, const Query<(CH + 3)
     pair(std::false_type());  // (on its own: a load that may be missing costs waits for all of them)
 }
 
-// A wave takes 16 query rows of one head as its columns; the workgroup's waves take
-// consecutive ones and read the same K/V at about the same time.  (Rows of a wave
-// dealt out to two or four waves by their keys, so that a launch with few rows has
-// more to balance: never faster, 24.4 and 29.7 us against 24.2 for 8 prompts at 12 x
-// 64, 147 and 158 against 145 for four chunks at 32/8 x 128.)
+// Query rows first .. + 16 of an item, one head.
 template <int CH>
-__global__ __launch_bounds__(256, CH <= 4 ? 3 : CH <= 8 ? 2 : 1) void kv_q8_prefill_kernel(KvQ8Prefill a) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // The items come longest first.  Workgroups go round the CUs in order of their
-    // index, so every second round goes backwards: the CU that has the longest of one
-    // round has the shortest of the next.
-    const int round = blockIdx.x / a.num_cus, place = blockIdx.x - round * a.num_cus;
-    const int in_round = min(a.num_cus, (int)gridDim.x - round * a.num_cus);
-    const int w = round * a.num_cus + (round % 2 ? in_round - 1 - place : place);
-    const int h = w % a.n_heads, item = w / a.n_heads;
+__device__ __forceinline__ void attend_item(const KvQ8Prefill& a, int item, int h, int wave, int lane) {
     const int b = a.work[2 * item];
     const PrefillSeq seq = a.seqs[b];
     const int col = lane & 15, g = lane >> 4, hd = a.c.head_dim;
@@ -100,6 +88,31 @@ __global__ __launch_bounds__(256, CH <= 4 ? 3 : CH <= 8 ? 2 : 1) void kv_q8_pref
     for (int t = 0; t < CH; t++) {
         const int dim = 16 * t + 4 * g;
         if (dim < hd) *reinterpret_cast<f4*>(out + dim) = st.o[t] * inv;
+    }
+}
+
+// A wave takes 16 query rows of one head as its columns; the workgroup's waves take
+// consecutive ones and read the same K/V at about the same time.  (Rows of a wave
+// dealt out to two or four waves by their keys, so that a launch with few rows has
+// more to balance: never faster, 24.4 and 29.7 us against 24.2 for 8 prompts at 12 x
+// 64, 147 and 158 against 145 for four chunks at 32/8 x 128.)
+template <int CH>
+__global__ __launch_bounds__(256, CH <= 4 ? 3 : CH <= 8 ? 2 : 1) void kv_q8_prefill_kernel(KvQ8Prefill a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // The items come longest first.  Workgroups go round the CUs in order of their
+    // index, so every second round goes backwards: the CU that has the longest of one
+    // round has the shortest of the next.  As many workgroups as items and heads, but
+    // for a captured launch that is replayed over a later batch.
+    const int total = a.seqs[0].work_items * a.n_heads;
+    for (int block = blockIdx.x; block < total; block += gridDim.x) {
+        const int round = block / a.num_cus, place = block - round * a.num_cus;
+        const int in_round = min(a.num_cus, total - round * a.num_cus);
+        const int w = round * a.num_cus + (round % 2 ? in_round - 1 - place : place);
+        const int item = w / a.n_heads;
+        int here = lane;
+        asm volatile("" : "+v"(here));  // (what follows from the lane is made anew, not kept in registers)
+        attend_item<CH>(a, item, w - item * a.n_heads, wave, here);
+        if (total - block <= (int)gridDim.x) break;
     }
 }
 

@@ -102,6 +102,7 @@ void reserve_rows(nitro_model* m, const nitro_kvpool* pool, int rows, bool last_
             for (size_t i = 0; i < at.size(); i++) at[i] = (int32_t)i;
             hip_check(hipMemcpy(m->kv_at.ptr, at.data(), at.size() * sizeof(int32_t), hipMemcpyHostToDevice),
                       "hipMemcpy(row numbers)");
+            hip_check(hipStreamSynchronize(nullptr), "hipStreamSynchronize");
             m->kv_at_rows = (int)at.size();
         }
     }

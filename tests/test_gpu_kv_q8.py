@@ -17,6 +17,10 @@ HEADS = [(2, 2, 64), (4, 2, 128), (6, 1, 36), (32, 1, 4), (17, 1, 20), (8, 1, 25
          (5, 5, 160)]
 
 
+# head counts with which a prefill of 150 rows is taken by whole pages
+PAGEWISE = [(900, 900, 4), (200, 100, 36), (128, 64, 64), (50, 50, 80), (60, 30, 128), (23, 23, 160), (14, 14, 252), (14, 14, 256)]
+
+
 def say(*a):
     print(*a, flush=True)
 
@@ -94,12 +98,14 @@ class Case:
 
 @pytest.mark.parametrize("rope", [False, True])
 @pytest.mark.parametrize("prefill", [False, True])
-@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("heads", HEADS + PAGEWISE)
 def test_append_and_read(heads, prefill, rope):
     import torch
 
     say("append", heads, "prefill" if prefill else "decode", "rope" if rope else "")
-    spans = [(0, 1), (5, 40), (16, 16), (31, 17), (0, 0), (40, 2)] if prefill else [(0, 1), (15, 1), (16, 1), (37, 1), (63, 1)]
+    spans = [(0, 1), (15, 1), (16, 1), (37, 1), (63, 1)]
+    if prefill:
+        spans = [(0, 1), (5, 40), (16, 16), (31, 17), (0, 0), (40, 2), (14, 1), (15, 1), (8, 70), (3, 2)]
     c = Case(1, spans, heads)
     c.upload(prefill)
     q, k, v = to_gpu(c.q), to_gpu(c.k), to_gpu(c.v)
@@ -124,11 +130,11 @@ def test_append_and_read(heads, prefill, rope):
     assert c.pool.take_device_errors() == 0
 
 
-@pytest.mark.parametrize("prefill", [False, True])
-def test_append_of_unusual_rows(prefill):
+@pytest.mark.parametrize("prefill,heads", [(False, 2), (True, 2), (True, 400)])
+def test_append_of_unusual_rows(prefill, heads):
     """Zeros, values below the least scale, the largest finite ones, ties, infinities and NaN."""
-    say("append unusual rows", prefill)
-    c = Case(2, [(3, 24)] if prefill else [(i, 1) for i in range(24)], (4, 2, 64))
+    say("append unusual rows", prefill, heads)
+    c = Case(2, [(3, 24)] if prefill else [(i, 1) for i in range(24)], (2 * heads, heads, 64))
     k, v = c.heads(c.k), c.heads(c.v)
     k[0] = 0
     v[1] = 0
@@ -421,6 +427,109 @@ def test_captured_decode_outlives_a_larger_launch():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (64, 64, 64)])
+@pytest.mark.parametrize("rope", [False, True])
+def test_captured_prefill_follows_uploads(rope, heads):
+    """Captured prefill calls replayed over later batches of as many rows, cut into fewer and more chunks
+    than the captured ones: each replay works on the batch uploaded last, as eager calls do."""
+    import torch
+
+    import nitrorag_amd as na
+
+    say("captured prefill, later uploads", heads, rope)
+    H, G, hd = heads
+    rows, width, pages = 192, 9, 64
+    rng = np.random.default_rng(21)
+    batches = [(rng.permutation(pages)[:len(n) * width].astype(np.int32).reshape(len(n), width), start, n)
+               for start, n in (([0, 3], [64, 128]), ([40, 16], [96, 96]), ([9, 0, 24, 79], [7, 0, 120, 65]),
+                                ([70, 5], [70, 122]), ([0, 15, 30, 5, 8, 7], [1, 2, 3, 121, 1, 64]))]
+    assert all(sum(n) == rows for _, _, n in batches)
+    data = rng.integers(0, 256, (pages, 1, G, kv_q8.record_bytes(hd)), dtype=np.uint8)
+    scales = np.abs(rng.standard_normal((pages, 1, G, 32))).astype(np.float32)
+    data[..., 32 * hd:] = scales.view(np.uint8)
+    clean = to_gpu(data)
+    cache = clean.clone()
+    pool = na.KVPool.wrap_q8(cache, hd)
+    q0, k0, v = (to_gpu(rng.standard_normal((rows, n * hd)).astype(np.float32)) for n in (H, G, G))
+    cos, sin = (to_gpu(x) for x in freqs(16 * width, hd))
+    state = q, k, out, kr, vr = [torch.empty_like(x) for x in (q0, k0, q0, k0, v)]
+
+    def reset():
+        cache.copy_(clean), q.copy_(q0), k.copy_(k0)
+        for x in (out, kr, vr):
+            x.fill_(float("nan"))
+
+    def step():
+        if rope:
+            pool.rope_kv_append_prefill(0, q, k, v, cos, sin, *heads)
+        else:
+            pool.kv_append_prefill(0, k, v)
+        pool.kv_read_prefill(0, kr, vr)
+        pool.prefill(0, q, out, *heads)
+
+    pool.upload_prefill_batch(*batches[-1])  # sizes every buffer
+    for captured in (0, 4):
+        pool.upload_prefill_batch(*batches[captured])
+        reset()
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for i in (0, 1, 4, 2, 3, 0):
+            pool.upload_prefill_batch(*batches[i])
+            reset()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [x.clone() for x in (cache, *state)]
+            assert torch.isfinite(out).all()
+            reset()
+            step()
+            torch.cuda.synchronize()
+            for name, g, w in zip(("cache", "q", "k", "out", "read k", "read v"), got, (cache, *state)):
+                assert torch.equal(g, w), f"captured {captured}, replayed over {i}: {name}"
+        del graph
+    assert pool.take_device_errors() == 0
+
+
+@pytest.mark.parametrize("heads", [(2, 2, 64), (8, 1, 128)])
+def test_captured_decode_follows_uploads(heads):
+    """A captured decode replayed over a later batch of the same tables with longer sequences (its splits
+    are then longer) and over its own."""
+    import torch
+
+    say("captured decode, later uploads", heads)
+    for short in (40, 700):
+        c = Case(22, [(3000, 1), (2047, 1), (64, 1)], heads)
+        c.fill()
+        c.put()
+        c.cache.copy_(to_gpu(c.ref.data))
+        q = to_gpu(c.q)
+        out = torch.empty_like(q)
+        for pos in ([3000, 2047, 64], [short, 20, 64]):  # the workspace, then what is captured
+            c.pool.upload_decode_batch(c.tables, pos)
+            c.pool.decode(c.layer, q, out, *heads)
+        torch.cuda.synchronize()
+        first = out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.pool.decode(c.layer, q, out, *heads)
+        for i in range(3):
+            out.fill_(float("nan"))
+            c.upload(False)
+            graph.replay()
+            torch.cuda.synchronize()
+            c.check(out, f"captured at {short}, replay {i}")
+            c.pool.upload_decode_batch(c.tables, [short, 20, 64])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, first)
+            c.upload(False)
+            c.pool.decode(c.layer, q, out, *heads)
+            c.check(out, f"eager after {i}")
+        del graph
 
 
 def test_on_another_stream():
