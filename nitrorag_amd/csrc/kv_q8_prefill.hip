@@ -2,12 +2,13 @@
 // row over the keys up to its own position (the products and the softmax:
 // kv_q8_attn.hpp).
 //
-// Bound by the vector instructions around the products, 344 per tile of 64 keys and 16
-// rows at head size 128 beside 48 matrix ones: they take 88% of the SIMDs' cycles, the
-// matrix cores are busy in 37%.  8192 tokens at 32 x 128: 975-1040 us (530-560
-// TFLOP/s of fp32-grade work; the cards' boxes differ), four chunks of 384 to 512
-// behind up to 4096 cached tokens at 32/8 x 128 130-138 us, 8 prompts of 128 to 1024
-// at 12 x 64 21-23 us.
+// Bound by the vector instructions around the products, 347 per tile of 64 keys and 16
+// rows at head size 128 beside 48 matrix ones: 79% of the SIMDs' cycles, the matrix
+// cores are busy in 38%.  8192 tokens at 32 x 128: 975-1040 us (530-560 TFLOP/s of
+// fp32-grade work; cards differ), four chunks of 384 to 512 behind up to 4096 cached
+// tokens at 32/8 x 128 130-138 us, 8 prompts of 128 to 1024 at 12 x 64 21-23 us.  (Four
+// tiles under one maximum rather than two: 8% fewer vector instructions, V a run of 16
+// dimensions at a time, 1029 us.)
 #include <hip/hip_runtime.h>
 
 #include "device_pool.hpp"
