@@ -550,6 +550,39 @@ def test_on_another_stream():
     c.check(out, "stream")
 
 
+def test_two_pools_on_two_streams():
+    """Split decodes and prefills of two pools that overlap: each pool has its own workspace."""
+    import torch
+
+    heads = (8, 2, 128)
+    cases = [Case(31, [(2999, 1), (1500, 1)], heads), Case(32, [(2000, 1), (2700, 1)], heads)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = []
+    for c in cases:
+        c.fill()
+        c.put()
+        c.cache.copy_(to_gpu(c.ref.data))
+        c.upload(False)
+        c.upload(True)
+        q = to_gpu(c.q)
+        outs = torch.empty_like(q), torch.empty_like(q)
+        c.pool.decode(c.layer, q, outs[0], *heads)  # sizes the workspace
+        c.pool.prefill(c.layer, q, outs[1], *heads)
+        jobs.append((c, q, outs))
+    torch.cuda.synchronize()
+    want = [[o.clone() for o in outs] for _, _, outs in jobs]
+    for _ in range(20):
+        for (c, q, outs), s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                c.pool.decode(c.layer, q, outs[0], *heads)
+                c.pool.prefill(c.layer, q, outs[1], *heads)
+    torch.cuda.synchronize()
+    for (c, _, outs), w in zip(jobs, want):
+        for o, e, what in zip(outs, w, ("decode", "prefill")):
+            assert torch.equal(o, e), what
+            c.check(o, what)
+
+
 def test_static_decode_and_bad_pages():
     """The allocation-free form gives the uploaded form's bits; page ids outside the pool are counted
     and their keys left out; a position below 0 gives zeros."""
