@@ -202,11 +202,13 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     const float* parts0 = a.partials + ((int64_t)b * a.num_splits * a.n_heads + h0) * a.pstride;
     // a wave per head: the splits' factors 2^(m - M) and the sum (lane i holds splits i, i + 64, ..)
     for (int c = wave; c < cols; c += a.waves) {
-        float M = -INFINITY, L = 0.0f;
-        for (int sp = lane; sp < parts; sp += 64) M = fmaxf(M, load_coherent(parts0 + sp * stride + c * a.pstride + hd).x);
+        auto m_and_l = [&](int sp) { return load_coherent(parts0 + sp * stride + c * a.pstride + hd); };
+        const float2 first = m_and_l(min(lane, parts - 1));
+        float M = first.x, L = 0.0f;
+        for (int sp = lane + 64; sp < parts; sp += 64) M = fmaxf(M, m_and_l(sp).x);
         M = wave_max(M);
         for (int sp = lane; sp < parts; sp += 64) {
-            const float2 ml = load_coherent(parts0 + sp * stride + c * a.pstride + hd);
+            const float2 ml = sp == lane ? first : m_and_l(sp);
             const float f = scale_of(ml.x, M);
             s_part[c * parts + sp] = f;
             L += ml.x == -INFINITY ? ml.y : ml.y * f;
@@ -228,9 +230,16 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
 #pragma unroll
             for (int i = 0; i < JOIN; i++) A0 = fmaf(x[i].x, f[sp + i], A0), A1 = fmaf(x[i].y, f[sp + i], A1);
         }
-        for (; sp < parts; sp++) {
-            const float2 x = load_coherent(from + sp * stride);
-            A0 = fmaf(x.x, f[sp], A0), A1 = fmaf(x.y, f[sp], A1);
+        // the rest four at a time (past the last: the last again, times 0)
+        for (; sp < parts; sp += 4) {
+            float2 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = load_coherent(from + min(sp + i, parts - 1) * stride);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float w = sp + i < parts ? f[sp + i] : 0.0f;
+                A0 = fmaf(x[i].x, w, A0), A1 = fmaf(x[i].y, w, A1);
+            }
         }
         float* out = a.out + ((int64_t)b * a.n_heads + h0 + c) * hd + d;
         const float L = s_part[cols * parts + c];
