@@ -546,12 +546,15 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
 
 // Launch shape of a decode over an 8-bit pool: four waves to a workgroup (two where
 // four waves' parts of all columns do not fit LDS), and the tiles per split that an
-// estimate of the launch's time finds best.  Its constants, in us: a tile takes a
-// wave t_alone where the memory is not what it waits for (measured 1.8 at head size
-// 64, 3.2 at 128: loads' latency and the products), t_busy where every resident wave
-// streams at 6.7 TB/s; a workgroup begins in 2.5, and a split that has to be joined
-// costs 5 more.  Where a launch has more workgroups than are resident, they follow
-// one another as they finish; the last ones run alone.
+// estimate of the launch's time finds best.  Its constants, in us: a tile takes a wave
+// t_alone where it has the memory to itself (loads' latency and the products), t_busy
+// where every resident wave streams at 6.7 TB/s; a workgroup begins in 3, and a join of
+// splits costs 4 more and 32e-6 for each byte that the last workgroup reads.  Between
+// the longest workgroup's tiles and the mean of all, half way.  Where a launch has more
+// workgroups than are resident, they follow one another as they finish; the last ones
+// run alone.  (Fitted to 24 batches, 1 to 64 sequences of 16 to 131072 tokens at head
+// sizes 36 to 256, each in splits of 4 to 96 tiles: the choice is 1.4% slower than the
+// best of those in the mean, 7% at most.)
 template <class Ctx>
 Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_heads, int n_kv_heads, int head_dim) {
     Q8DecodeShape best;
@@ -559,6 +562,7 @@ Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_hea
     best.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
     best.waves = kv_q8_decode_lds(n_heads, n_kv_heads, kv_q8_partial_floats(head_dim), 4, 1) <= KV_Q8_LDS ? 4 : 2;
     const double W = best.waves, columns = (double)n_kv_heads * best.groups;
+    const double part_bytes = (double)std::min(kv_mul, KV_Q8_COLUMNS) * hdp * sizeof(float);
     long long tiles = 0;
     int longest = 1;
     auto tiles_of = [&](int b) { return (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE; };
@@ -567,7 +571,7 @@ Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_hea
         longest = std::max(longest, tiles_of(b));
     }
     const double waves = 4.0 * kv_q8_decode_occupancy(hdp) * std::max(pool->num_cus, 1), resident = waves / W;
-    const double t_alone = hdp <= 64 ? 1.8 : hdp <= 128 ? 3.2 : 5.0;
+    const double t_alone = hdp <= 64 ? 1.1 : hdp <= 128 ? 1.2 : 3.2;
     const double t_busy = waves * KV_Q8_TILE * (2 * hdp + 8) / 6.7e6;
     double least = 1e30;
     for (int rounds = (longest + 256 * best.waves - 1) / (256 * best.waves);; rounds += 1 + rounds / 8) {
@@ -575,11 +579,12 @@ Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_hea
         long long items = 0;
         for (int b = 0; b < B; b++) items += (tiles_of(b) + tps - 1) / tps;
         const double load = (double)items * columns / resident;  // workgroups per place
-        const double begin = 2.5 + (tps < longest ? 5.0 : 0.0);
-        const double deep = std::min<double>(rounds, (longest + W - 1) / W);
-        const double cost = load <= 1 ? deep * std::max(t_alone, t_busy * load) + begin
-                                      : load * ((double)tiles / items / W * t_busy + begin) +
-                                            0.5 * (deep * t_alone + begin);
+        const int parts = (longest + tps - 1) / tps;
+        const double begin = 3.0 + (parts > 1 ? 4.0 + 32e-6 * parts * part_bytes : 0.0);
+        const double deep = std::min<double>(rounds, (longest + W - 1) / W), mean = (double)tiles / items / W;
+        const double cost =
+            load <= 1 ? 0.5 * (deep + mean) * (t_alone + (t_busy - t_alone) * std::pow(load, 1.25)) + begin
+                      : load * (mean * t_busy + 1.2) + 0.25 * deep * t_alone + begin;
         if (cost < least) {
             least = cost;
             best.tps = tps;

@@ -92,6 +92,43 @@ __device__ __forceinline__ float divided(float A, float L) { return L == 0.0f ? 
 
 constexpr int JOIN = 16;  // partials whose loads go out together
 
+// Tokens that sequence b's row attends.
+__device__ __forceinline__ int seen_by(const KvQ8Decode& a, int b) {
+    return max(0, min(a.positions[b], a.ctx_limit - 1) + 1);
+}
+// Tiles per split of a sequence.  (More than planned in a captured launch that is
+// replayed over a later batch with a longer sequence.)
+__device__ __forceinline__ int split_tiles(const KvQ8Decode& a, int tiles) {
+    return tiles > a.num_splits * a.tiles_per_split ? (tiles + a.num_splits - 1) / a.num_splits : a.tiles_per_split;
+}
+// The sequence and split of work item i, the sequences' splits one after the other; -1
+// past the last.  (Workgroups go round the CUs in order of their index: with an index
+// for every sequence and each split that the longest has, the CUs had more or less
+// work as those that a short one lacks fell.)
+__device__ __forceinline__ int item_of(const KvQ8Decode& a, int i, int lane, int& split) {
+    for (int base = 0; base < a.batch; base += 64) {
+        int n = 0;
+        if (base + lane < a.batch) {
+            const int tiles = (seen_by(a, base + lane) + KV_Q8_TILE - 1) / KV_Q8_TILE, tps = split_tiles(a, tiles);
+            n = max(1, (tiles + tps - 1) / tps);
+        }
+        int upto = n;  // splits of the sequences up to the lane's
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        const int total = __builtin_amdgcn_readlane(upto, 63);
+        if (i < total) {
+            const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= i));
+            split = i - __builtin_amdgcn_readlane(upto - n, at);
+            return base + at;
+        }
+        i -= total;
+    }
+    return -1;
+}
+
 // A workgroup takes one split of one sequence's keys for up to 16 query heads of a
 // K/V head; its waves take the split's tiles in turn.  Waves per SIMD are what the
 // registers allow without spills (at head size 128 208; an earlier form had 183, and
@@ -108,12 +145,13 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     w /= groups;
     const int kv_h = w % a.c.kv_heads;
     w /= a.c.kv_heads;
-    // Workgroups go round the CUs in order of their index, and the splits that a
-    // short sequence lacks end at once: an odd number of places per sequence keeps
-    // those from falling on the same CUs (24 sequences of 512 to 8192 tokens at 32/8
-    // heads of 128 in splits of 2048: 61 us with four places, 47 with five).
-    const int places = a.num_splits | 1;
-    const int split = w % places, b = w / places;
+    int split = w, b = 0;
+    if (a.num_splits == 1) {
+        split = 0, b = w;
+    } else if (a.batch > 1) {
+        b = item_of(a, w, lane, split);
+        if (b < 0) return;
+    }
     const int h0 = kv_h * kv_mul + hg * KV_Q8_COLUMNS;  // first query head
     const int cols = min(KV_Q8_COLUMNS, kv_mul - hg * KV_Q8_COLUMNS);
     const int hd = a.c.head_dim;
@@ -128,10 +166,9 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     int tps = a.tiles_per_split, t0 = split * tps;
     int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
     const auto row = load_row<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, g);
-    const int ctx = max(0, min(a.positions[b], a.ctx_limit - 1) + 1);
-    const int tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
-    if (tiles > a.num_splits * tps) {  // a captured launch, replayed over a later batch with a longer sequence
-        tps = (tiles + a.num_splits - 1) / a.num_splits;
+    const int ctx = seen_by(a, b), tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
+    if (tiles > a.num_splits * tps) {
+        tps = split_tiles(a, tiles);
         t0 = split * tps;
         kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
     }
@@ -262,7 +299,7 @@ void pick(int chunks, bool stream, F launch) {
 hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream) {
     const int kv_mul = a.n_heads / a.c.kv_heads;
     const int groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
-    const int64_t blocks = (int64_t)a.batch * (a.num_splits | 1) * a.c.kv_heads * groups;
+    const int64_t blocks = (int64_t)a.batch * a.num_splits * a.c.kv_heads * groups;
     const int chunks = a.c.hdp / 16;
     const size_t lds = kv_q8_decode_lds(a.n_heads, a.c.kv_heads, a.pstride, a.waves, a.num_splits);
     if (a.waves < 1 || a.waves > 4 || a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
