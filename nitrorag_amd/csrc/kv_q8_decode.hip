@@ -4,7 +4,7 @@
 // Bound by bytes: 2 * head_dim + 8 per key and K/V head.  64 x 4096 tokens at 32 x 128
 // take 328 us (6.74 TB/s, what this card streams; vector instructions in a third of the
 // SIMDs' cycles), one sequence of 131072 at 32/8 x 128 50 us (5.5 TB/s: start, two tile
-// rounds' latency and the join of 64 splits are 9 us), 24 of 512 to 8192 43 us (the
+// rounds' latency and the join of 64 splits are 9 us), 24 of 512 to 8192 42 us (the
 // same, and splits of unequal length), 32 of 16 to 1024 at 12 x 64 11 us and one of
 // 256 5 us (latency: launch, table entry, K/V, products, join).
 //
