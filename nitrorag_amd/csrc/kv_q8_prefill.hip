@@ -4,9 +4,9 @@
 //
 // Bound by the vector instructions around the products, 347 per tile of 64 keys and 16
 // rows at head size 128 beside 48 matrix ones: 79% of the SIMDs' cycles, the matrix
-// cores are busy in 38%.  8192 tokens at 32 x 128: 975-1040 us (530-560 TFLOP/s of
+// cores are busy in 38%.  8192 tokens at 32 x 128: 975-1060 us (520-560 TFLOP/s of
 // fp32-grade work; cards differ), four chunks of 384 to 512 behind up to 4096 cached
-// tokens at 32/8 x 128 130-138 us, 8 prompts of 128 to 1024 at 12 x 64 21-23 us.  (Four
+// tokens at 32/8 x 128 130-140 us, 8 prompts of 128 to 1024 at 12 x 64 21-23 us.  (Four
 // tiles under one maximum rather than two: 8% fewer vector instructions, V a run of 16
 // dimensions at a time, 1029 us.)
 #include <hip/hip_runtime.h>

@@ -182,6 +182,35 @@ def test_decode(heads, ctx):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("heads,ctx", [((4, 1, 64), [5000] + [1, 90, 300] * 43 + [4100, 7]),
+                                       ((2, 2, 128), [700, 1, 1, 64, 65, 3000] * 11 + [1]),
+                                       ((3, 1, 36), [1] * 64 + [2500] + [1] * 64)])
+def test_decode_of_many_unequal_sequences(heads, ctx):
+    """More sequences than a wave has lanes, a few of them split."""
+    import torch
+
+    from nitrorag_amd import _native as N
+
+    say("decode, many sequences", heads, len(ctx))
+    c = Case(41, [(n - 1, 1) for n in ctx], heads)
+    c.fill()
+    c.put()
+    c.cache.copy_(to_gpu(c.ref.data))
+    q = to_gpu(c.q)
+    c.upload(False)
+    out, again, fixed = (torch.full_like(q, float("nan")) for _ in range(3))
+    c.pool.decode(c.layer, q, out, *heads)
+    c.check(out, "decode")
+    c.pool.decode(c.layer, q, again, *heads)
+    assert torch.equal(out, again)
+    t, p = to_gpu(c.tables), to_gpu(np.array(ctx, np.int32) - 1)
+    assert N.lib().nitro_paged_attn_decode_static(
+        c.pool.handle, c.layer, q.data_ptr(), fixed.data_ptr(), t.data_ptr(), p.data_ptr(), len(ctx), c.tables.shape[1],
+        max(ctx), *heads, 1, torch.cuda.current_stream().cuda_stream) == N.OK
+    c.check(fixed, "static decode")
+    assert c.pool.take_device_errors() == 0
+
+
 @pytest.mark.parametrize("scale", [0.0, 1e-30, 30.0])
 def test_decode_of_flat_and_peaked_weights(scale):
     import torch
