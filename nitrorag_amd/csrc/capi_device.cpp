@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <numeric>
 #include <string>
 #include <unordered_map>
 #include <utility>
@@ -546,45 +547,65 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
 
 // Launch shape of a decode over an 8-bit pool: four waves to a workgroup (two where
 // four waves' parts of all columns do not fit LDS), and the tiles per split that an
-// estimate of the launch's time finds best.  Its constants, in us: a tile takes a wave
-// t_alone where it has the memory to itself (loads' latency and the products), t_busy
-// where every resident wave streams at 6.7 TB/s; a workgroup begins in 3, and a join of
-// splits costs 4 more and 32e-6 for each byte that the last workgroup reads.  Between
-// the longest workgroup's tiles and the mean of all, half way.  Where a launch has more
-// workgroups than are resident, they follow one another as they finish; the last ones
-// run alone.  (Fitted to 24 batches, 1 to 64 sequences of 16 to 131072 tokens at head
-// sizes 36 to 256, each in splits of 4 to 96 tiles: the choice is 1.4% slower than the
-// best of those in the mean, 7% at most.)
+// estimate of the launch's time finds best.  In us: the time in which the longest
+// workgroup's tiles follow one another, the one in which a CU reads what its workgroups
+// take (these go round the CUs in order) and the one in which all is read meet in a
+// power mean; a workgroup begins in 3.6, and a join costs 4.1 more and 34e-6 for each
+// byte that the last workgroup reads.  Where a launch has more workgroups than are
+// resident, they follow one another as they finish, and the last ones run alone.
+// (Constants fitted to 24 batches, 1 to 64 sequences of 16 to 131072 tokens at head
+// sizes 36 to 256, each in splits of 4 to 96 tiles: the choice is 0.7% slower than the
+// best of those in the mean, 4% at most.)
+// Sequences that are not split are taken longest first, every second round of CUs
+// backwards: a CU with one of the longest then has one of the shortest beside it.
 template <class Ctx>
 Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_heads, int n_kv_heads, int head_dim) {
     Q8DecodeShape best;
-    const int kv_mul = n_heads / n_kv_heads, hdp = kv_q8_padded(head_dim);
+    const int kv_mul = n_heads / n_kv_heads, hdp = kv_q8_padded(head_dim), num_cus = std::max(pool->num_cus, 1);
     best.groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
     best.waves = kv_q8_decode_lds(n_heads, n_kv_heads, kv_q8_partial_floats(head_dim), 4, 1) <= KV_Q8_LDS ? 4 : 2;
-    const double W = best.waves, columns = (double)n_kv_heads * best.groups;
+    const int W = best.waves, columns = n_kv_heads * best.groups;
     const double part_bytes = (double)std::min(kv_mul, KV_Q8_COLUMNS) * hdp * sizeof(float);
-    long long tiles = 0;
-    int longest = 1;
-    auto tiles_of = [&](int b) { return (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE; };
-    for (int b = 0; b < B; b++) {
-        tiles += tiles_of(b);
-        longest = std::max(longest, tiles_of(b));
+    std::vector<int> tiles(B);
+    long long all = 0;
+    for (int b = 0; b < B; b++) all += tiles[b] = (ctx(b) + KV_Q8_TILE - 1) / KV_Q8_TILE;
+    const int longest = std::max(1, *std::max_element(tiles.begin(), tiles.end()));
+    if (B <= KV_Q8_ORDERED && (long long)B * columns > num_cus &&
+        *std::min_element(tiles.begin(), tiles.end()) < longest) {
+        best.order.resize(B);
+        std::iota(best.order.begin(), best.order.end(), (uint8_t)0);
+        std::stable_sort(best.order.begin(), best.order.end(), [&](int x, int y) { return tiles[x] > tiles[y]; });
     }
-    const double waves = 4.0 * kv_q8_decode_occupancy(hdp) * std::max(pool->num_cus, 1), resident = waves / W;
-    const double t_alone = hdp <= 64 ? 1.1 : hdp <= 128 ? 1.2 : 3.2;
-    const double t_busy = waves * KV_Q8_TILE * (2 * hdp + 8) / 6.7e6;
+    const int resident = 4 * kv_q8_decode_occupancy(hdp) * num_cus / W;
+    const double tile_bytes = KV_Q8_TILE * (2.0 * hdp + 8);
+    const double t_alone = hdp <= 64 ? 0.8 : hdp <= 128 ? 0.5 : 2.4;
+    const double t_all = all * columns * tile_bytes / 8.0e6;  // every CU reads throughout
+    // Items that share a CU (each stands for one workgroup per column): index by index
+    // over `across` places.
+    const int across = std::max(1, (num_cus + columns / 2) / columns);
+    std::vector<int> place(across);
     double least = 1e30;
-    for (int rounds = (longest + 256 * best.waves - 1) / (256 * best.waves);; rounds += 1 + rounds / 8) {
-        const int tps = rounds * best.waves;
+    for (int rounds = (longest + 256 * W - 1) / (256 * W);; rounds += 1 + rounds / 8) {
+        const int tps = rounds * W, parts = (longest + tps - 1) / tps, deep = std::min(rounds, (longest + W - 1) / W);
         long long items = 0;
-        for (int b = 0; b < B; b++) items += (tiles_of(b) + tps - 1) / tps;
-        const double load = (double)items * columns / resident;  // workgroups per place
-        const int parts = (longest + tps - 1) / tps;
-        const double begin = 3.0 + (parts > 1 ? 4.0 + 32e-6 * parts * part_bytes : 0.0);
-        const double deep = std::min<double>(rounds, (longest + W - 1) / W), mean = (double)tiles / items / W;
-        const double cost =
-            load <= 1 ? 0.5 * (deep + mean) * (t_alone + (t_busy - t_alone) * std::pow(load, 1.25)) + begin
-                      : load * (mean * t_busy + 1.2) + 0.25 * deep * t_alone + begin;
+        for (int b = 0; b < B; b++) items += (tiles[b] + tps - 1) / tps;
+        double cost = 3.6 + (parts > 1 ? 4.1 + 34e-6 * parts * part_bytes : 0.0);
+        const double load = (double)items * columns / resident;
+        if (load <= 1) {
+            std::fill(place.begin(), place.end(), 0);
+            int i = 0;
+            for (int x = 0; x < B; x++) {
+                const bool sorted = parts == 1 && !best.order.empty();
+                for (int left = tiles[sorted ? best.order[x] : x]; left > 0; left -= tps, i++)
+                    place[sorted && i / across % 2 ? across - 1 - i % across : i % across] += (std::min(left, tps) + W - 1) / W;
+            }
+            const double t_cu = *std::max_element(place.begin(), place.end()) * W * tile_bytes / 48e3;
+            const double n = 2.75;
+            cost += std::pow(std::pow(deep * t_alone, n) + std::pow(t_cu, n) + std::pow(t_all, n), 1 / n);
+        } else {
+            const double t_busy = resident * tile_bytes / 6.7e6;  // of a tile of each wave
+            cost += load * (all * t_busy / items + 1.4) + 0.25 * deep * t_alone;
+        }
         if (cost < least) {
             least = cost;
             best.tps = tps;
@@ -592,6 +613,7 @@ Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_hea
         if (tps >= longest) break;
     }
     best.splits = (longest + best.tps - 1) / best.tps;
+    if (best.splits > 1) best.order.clear();
     return best;
 }
 
@@ -607,6 +629,8 @@ KvQ8Decode q8_decode_args(const nitro_kvpool* pool, int layer, const float* q, f
     a.num_splits = sh.splits;
     a.pstride = kv_q8_partial_floats(a.c.head_dim);
     a.stream_kv = sh.groups == 1 && !shared_pages;
+    a.ordered = sh.order.empty() ? 0 : std::max(pool->num_cus, 1);
+    std::copy(sh.order.begin(), sh.order.end(), a.order);
     a.qscale = (float)(1.4426950408889634 / std::sqrt((double)a.c.head_dim));
     return a;
 }

@@ -246,6 +246,7 @@ namespace nitro {
 // Launch shape of a decode over an 8-bit pool.
 struct Q8DecodeShape {
     int waves = 0, tps = 0, groups = 0, splits = 0;  // waves per workgroup, tiles per split, head groups, splits at most
+    std::vector<uint8_t> order;                      // of unsplit sequences, where they are taken in one of their own
 };
 }  // namespace nitro
 

@@ -57,6 +57,9 @@ constexpr int KV_Q8_TILE = 64;
 // columns of its matrix instructions).
 constexpr int KV_Q8_COLUMNS = 16;
 
+// Sequences of a decode launch that are taken in an order of their own at most.
+constexpr int KV_Q8_ORDERED = 128;
+
 struct KvQ8Decode {
     KvQ8 c;
     const float* q;
@@ -69,6 +72,10 @@ struct KvQ8Decode {
     int32_t tiles_per_split, num_splits, waves, pstride;
     int32_t stream_kv;  // no record is read twice: loads that stay out of the caches
     float qscale;  // log2(e) / sqrt(head_dim)
+    // Not 0 (the number of CUs): unsplit sequences are taken in this order, every
+    // second round of CUs backwards.  Any order of them is right.
+    int32_t ordered;
+    uint8_t order[KV_Q8_ORDERED];
 };
 // Waves per SIMD of the decode kernel.
 constexpr int kv_q8_decode_occupancy(int hdp) { return hdp <= 64 ? 4 : hdp <= 128 ? 2 : 1; }

@@ -3,10 +3,10 @@
 //
 // Bound by bytes: 2 * head_dim + 8 per key and K/V head.  64 x 4096 tokens at 32 x 128
 // take 328 us (6.74 TB/s, what this card streams; vector instructions in a third of the
-// SIMDs' cycles), one sequence of 131072 at 32/8 x 128 50 us (5.5 TB/s: start, two tile
-// rounds' latency and the join of 64 splits are 9 us), 24 of 512 to 8192 42 us (the
-// same, and splits of unequal length), 32 of 16 to 1024 at 12 x 64 11 us and one of
-// 256 5 us (latency: launch, table entry, K/V, products, join).
+// SIMDs' cycles), one sequence of 131072 at 32/8 x 128 48 us (5.8 TB/s: start and the
+// join of 32 splits are 7 us), 24 of 512 to 8192 41 us (the same, and splits that do not
+// fill the CUs evenly), 32 of 16 to 1024 at 12 x 64 9 us and one of 256 5 us (latency:
+// launch, table entry, K/V, products, join).
 //
 // A product's 16 columns are the query heads of one K/V head, so K and V are read once
 // for up to 16 of them; with fewer the other columns compute nothing, which the matrix
@@ -141,13 +141,17 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     const int kv_mul = a.n_heads / a.c.kv_heads;
     const int groups = (kv_mul + KV_Q8_COLUMNS - 1) / KV_Q8_COLUMNS;
     int w = blockIdx.x;
+    if (a.ordered) {
+        const int round = w / a.ordered, in_round = min(a.ordered, (int)gridDim.x - round * a.ordered);
+        if (round % 2) w = round * a.ordered + in_round - 1 - (w - round * a.ordered);
+    }
     const int hg = w % groups;
     w /= groups;
     const int kv_h = w % a.c.kv_heads;
     w /= a.c.kv_heads;
     int split = w, b = 0;
     if (a.num_splits == 1) {
-        split = 0, b = w;
+        split = 0, b = a.ordered ? a.order[w] : w;
     } else if (a.batch > 1) {
         b = item_of(a, w, lane, split);
         if (b < 0) return;
@@ -302,7 +306,7 @@ hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream) {
     const int64_t blocks = (int64_t)a.batch * a.num_splits * a.c.kv_heads * groups;
     const int chunks = a.c.hdp / 16;
     const size_t lds = kv_q8_decode_lds(a.n_heads, a.c.kv_heads, a.pstride, a.waves, a.num_splits);
-    if (a.waves < 1 || a.waves > 4 || a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
+    if ((a.ordered && (a.num_splits != 1 || a.batch > KV_Q8_ORDERED)) || a.waves < 1 || a.waves > 4 || a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
         blocks > INT32_MAX || lds > KV_Q8_LDS)
         return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(64 * a.waves);

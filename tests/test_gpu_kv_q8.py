@@ -184,9 +184,11 @@ def test_decode(heads, ctx):
 
 @pytest.mark.parametrize("heads,ctx", [((4, 1, 64), [5000] + [1, 90, 300] * 43 + [4100, 7]),
                                        ((2, 2, 128), [700, 1, 1, 64, 65, 3000] * 11 + [1]),
-                                       ((3, 1, 36), [1] * 64 + [2500] + [1] * 64)])
+                                       ((3, 1, 36), [1] * 64 + [2500] + [1] * 64),
+                                       ((12, 12, 64), [1000, 16, 300, 65, 1] * 7),
+                                       ((48, 24, 32), [5, 700, 80] * 43)])
 def test_decode_of_many_unequal_sequences(heads, ctx):
-    """More sequences than a wave has lanes, a few of them split."""
+    """More sequences than a wave has lanes, a few of them split; unsplit ones, longest first."""
     import torch
 
     from nitrorag_amd import _native as N
@@ -523,7 +525,7 @@ def test_captured_prefill_follows_uploads(rope, heads):
     assert pool.take_device_errors() == 0
 
 
-@pytest.mark.parametrize("heads", [(2, 2, 64), (8, 1, 128)])
+@pytest.mark.parametrize("heads", [(2, 2, 64), (8, 1, 128), (100, 100, 32)])
 def test_captured_decode_follows_uploads(heads):
     """A captured decode replayed over a later batch of the same tables with longer sequences (its splits
     are then longer) and over its own."""
