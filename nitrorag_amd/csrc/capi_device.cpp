@@ -592,12 +592,20 @@ Q8DecodeShape plan_q8_decode(const nitro_kvpool* pool, int B, Ctx ctx, int n_hea
         double cost = 3.6 + (parts > 1 ? 4.1 + 34e-6 * parts * part_bytes : 0.0);
         const double load = (double)items * columns / resident;
         if (load <= 1) {
+            const bool sorted = parts == 1 && !best.order.empty();
             std::fill(place.begin(), place.end(), 0);
-            int i = 0;
+            int at = 0, step = 1;
+            auto add = [&](int n) {
+                place[at] += n;
+                if (sorted && (at + step < 0 || at + step == across))
+                    step = -step;
+                else
+                    at = at + step == across ? 0 : at + step;
+            };
             for (int x = 0; x < B; x++) {
-                const bool sorted = parts == 1 && !best.order.empty();
-                for (int left = tiles[sorted ? best.order[x] : x]; left > 0; left -= tps, i++)
-                    place[sorted && i / across % 2 ? across - 1 - i % across : i % across] += (std::min(left, tps) + W - 1) / W;
+                int left = tiles[sorted ? best.order[x] : x];
+                for (; left > tps; left -= tps) add(rounds);
+                if (left > 0) add((left + W - 1) / W);
             }
             const double t_cu = *std::max_element(place.begin(), place.end()) * W * tile_bytes / 48e3;
             const double n = 2.75;
