@@ -169,7 +169,8 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
     };
     int tps = a.tiles_per_split, t0 = split * tps;
     int kp = page(4 * (t0 + wave) + (col >> 2)), vp = page(4 * (t0 + wave) + g);
-    const auto row = load_row<(CH + 3) / 4>(col < cols ? a.q + ((int64_t)b * a.n_heads + h0 + col) * hd : nullptr, hd, g);
+    const float* q_at = a.q + ((int64_t)b * a.n_heads + h0 + col) * hd;
+    const auto row = load_row<(CH + 3) / 4>(col < cols ? q_at : nullptr, hd, g);
     const int ctx = seen_by(a, b), tiles = (ctx + KV_Q8_TILE - 1) / KV_Q8_TILE;
     if (tiles > a.num_splits * tps) {
         tps = split_tiles(a, tiles);
@@ -185,8 +186,8 @@ __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_de
 #pragma unroll
     for (int t = 0; t < CH; t++) st.o[t] = f4{0.f, 0.f, 0.f, 0.f};
     if (t0 + wave < t1) {
-        attend<CH, STREAM>(st, row, a.qscale, a.c, a.c.cache + a.c.layer_off + (int64_t)kv_h * a.c.record, t0 + wave, t1, a.waves,
-                           lane, kp, vp, page, [&](int t) { return ctx - t * KV_Q8_TILE - 16 * g; });
+        const uint8_t* base = a.c.cache + a.c.layer_off + (int64_t)kv_h * a.c.record;
+        attend<CH, STREAM>(st, row, a.qscale, a.c, base, t0 + wave, t1, a.waves, lane, kp, vp, page, [&](int t) { return ctx - t * KV_Q8_TILE - 16 * g; });
     }
 
     // The waves' parts meet in LDS.
@@ -306,7 +307,8 @@ hipError_t launch_kv_q8_decode(const KvQ8Decode& a, hipStream_t stream) {
     const int64_t blocks = (int64_t)a.batch * a.num_splits * a.c.kv_heads * groups;
     const int chunks = a.c.hdp / 16;
     const size_t lds = kv_q8_decode_lds(a.n_heads, a.c.kv_heads, a.pstride, a.waves, a.num_splits);
-    if ((a.ordered && (a.num_splits != 1 || a.batch > KV_Q8_ORDERED)) || a.waves < 1 || a.waves > 4 || a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
+    if ((a.ordered && (a.num_splits != 1 || a.batch > KV_Q8_ORDERED)) || a.waves < 1 || a.waves > 4 ||
+        a.pstride < a.c.head_dim + 2 || a.pstride % 4 || chunks < 1 || chunks > 16 ||
         blocks > INT32_MAX || lds > KV_Q8_LDS)
         return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(64 * a.waves);

@@ -18,7 +18,8 @@ HEADS = [(2, 2, 64), (4, 2, 128), (6, 1, 36), (32, 1, 4), (17, 1, 20), (8, 1, 25
 
 
 # head counts with which a prefill of 150 rows is taken by whole pages
-PAGEWISE = [(900, 900, 4), (200, 100, 36), (128, 64, 64), (50, 50, 80), (60, 30, 128), (23, 23, 160), (14, 14, 252), (14, 14, 256)]
+PAGEWISE = [(900, 900, 4), (200, 100, 36), (128, 64, 64), (50, 50, 80), (60, 30, 128), (23, 23, 160), (14, 14, 252),
+            (14, 14, 256)]
 
 
 def say(*a):
