@@ -168,14 +168,17 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  * below 2^-96 may be zero.  Two rows of one batch that go to the same slot leave a mixture
  * of both there, as in an fp32 pool.
  *   A pool holds less than 512 GiB and is used on the device that was current when it was
- * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  Its
- * workspace for splits stays where it is until the pool goes, so a captured
- * nitro_paged_attn_decode may be replayed after launches that needed more, also over a
- * later upload of as many sequences and the same max_pages, whatever their lengths
- * (prefill calls: of as many rows, in any number of chunks); as for an fp32 pool,
- * launches that overlap on one pool race on it.  nitro_kvpool_data has nothing to
- * give (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape reports kv_dim = n_kv_heads *
- * head_dim. */
+ * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  As for
+ * an fp32 pool, launches that overlap on one pool race on its workspace for splits.
+ * nitro_kvpool_data has nothing to give (NITRO_ERR_UNSUPPORTED); nitro_kvpool_shape
+ * reports kv_dim = n_kv_heads * head_dim.
+ *   Captured calls: the workspace for splits stays where it is until the pool goes, so a
+ * captured nitro_paged_attn_decode may be replayed after launches that needed more.
+ * Captured calls work on the batch uploaded last, whatever its lengths: decode and
+ * nitro_kv_append calls where it has as many sequences and the same max_pages, prefill
+ * calls where it has as many rows and the same max_pages, in any number of chunks - as
+ * long as no upload since the capture needed more room for the batch than the pool had
+ * for it (nitro_kvpool_reserve_batches). */
 int nitro_kvpool_create_q8(int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
                            nitro_kvpool** out);
 int nitro_kvpool_wrap_q8(void* cache, int32_t num_pages, int32_t num_layers, int32_t n_kv_heads, int32_t head_dim,
@@ -200,6 +203,16 @@ int nitro_kv_read_prefill(nitro_kvpool* pool, int32_t layer, float* k, float* v,
  * rows from the caches measured faster. */
 int nitro_decode_batch_upload(nitro_kvpool* pool, const int32_t* tables, const int32_t* positions,
                               int32_t batch, int32_t max_pages, void* stream);
+
+/* Room for decode batches of up to `sequences` sequences, and for prefill batches of up
+ * to `sequences` chunks and `rows` rows in all (0: none), with tables up to max_pages
+ * wide.  No counterpart in the reference: it is for callers that capture launches.  A
+ * captured launch reads a batch's device arrays where they were then.  Uploads of batches
+ * within this room, or within that of an earlier upload, write to those arrays; one that
+ * needs more moves all of that kind (decode or prefill), and a launch captured before goes
+ * on reading the batch that its old arrays hold, which are kept until the pool goes.
+ * Where this call moves arrays, their batch has to be uploaded again.  Any pool. */
+int nitro_kvpool_reserve_batches(nitro_kvpool* pool, int32_t sequences, int32_t max_pages, int32_t rows);
 
 /* KV append for the decode batch — src/model_q8.cpp:616-623 (and the
  * single-sequence append :279-287): k, v are device [batch][kv_dim]; row

@@ -86,6 +86,7 @@ SIGNATURES = {
     "nitro_kv_read_prefill": [_vp, _i32, _fp, _fp, _vp],
     "nitro_kvpool_destroy": [_vp],
     "nitro_kvpool_data": [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
+    "nitro_kvpool_reserve_batches": [_vp, _i32, _i32, _i32],
     "nitro_kvpool_shape": [_vp, _i32p, _i32p, _i32p],
     "nitro_decode_batch_upload": [_vp, _i32p, _i32p, _i32, _i32, _vp],
     "nitro_kv_append": [_vp, _i32, _fp, _fp, _vp],

@@ -172,6 +172,12 @@ class KVPool:
         N.call("nitro_kvpool_data", self._h, ctypes.byref(k), ctypes.byref(v))
         return k.value, v.value
 
+    def reserve_batches(self, sequences: int, max_pages: int, rows: int = 0) -> None:
+        """Room for decode batches of up to `sequences` sequences and prefill batches of up to
+        `sequences` chunks and `rows` rows, tables up to max_pages wide: launches captured
+        after it follow later uploads within that room.  Batches are uploaded after it."""
+        N.call("nitro_kvpool_reserve_batches", self._h, sequences, max_pages, rows)
+
     # ---------------------------------------------------------------- decode
     def upload_decode_batch(self, tables, positions, stream=None) -> None:
         t = _host_i32(tables)

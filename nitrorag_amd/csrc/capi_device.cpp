@@ -953,6 +953,21 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
     });
 }
 
+int nitro_kvpool_reserve_batches(nitro_kvpool* pool, int32_t sequences, int32_t max_pages, int32_t rows) {
+    return guarded([&] {
+        require_pool(pool);
+        require(sequences > 0 && max_pages > 0 && rows >= 0, ERR_INVALID_ARGUMENT,
+                "sequences and max_pages must be positive, rows not negative");
+        if (pool->q8) (void)kv_q8_layer(pool, 0);  // the current device is the pool's
+        const size_t tables = (size_t)sequences * max_pages;
+        auto work_words = [&](int item_rows) { return 2 * ((size_t)rows / item_rows + sequences); };
+        if (pool->decode.reserve(tables, sequences)) pool->decode.batch = 0;
+        if (rows > 0 && pool->prefill.reserve(tables, sequences, rows, work_words(prefill_block_m(0)),
+                                              work_words(PREFILL_WIDE_ROWS)))
+            pool->prefill.batch = 0;
+    });
+}
+
 int nitro_decode_batch_upload(nitro_kvpool* pool, const int32_t* tables, const int32_t* positions,
                               int32_t batch, int32_t max_pages, void* stream) {
     return guarded([&] {
@@ -1190,12 +1205,7 @@ int nitro_prefill_batch_upload(nitro_kvpool* pool, const int32_t* tables, const 
 
         const size_t nt = (size_t)batch * max_pages;
         const size_t n_work = items.size() * 2, n_wide = wide.size() * 2;
-        p.tables.reserve(nt);
-        p.seqs.reserve(batch);
-        p.slots.reserve(total);
-        p.row_pos.reserve(total);
-        p.work.reserve(n_work);
-        p.work_wide.reserve(n_wide);
+        p.reserve(nt, batch, total, n_work, n_wide);
         hipStream_t s = as_stream(stream);
         Staging& st = pool->prefill_staging;
         st.acquire(nt + 4 * (size_t)batch + 2 * (size_t)total + n_work + n_wide, 6);

@@ -8,6 +8,8 @@
 #include <cstdint>
 #include <memory>
 #include <string>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "kv_q8.hpp"
@@ -78,6 +80,47 @@ struct KeptBuffer {
         return true;
     }
 };
+
+// Device blocks that a launch captured earlier may still read, freed with their owner.
+struct KeptBlocks {
+    std::vector<void*> blocks;
+    KeptBlocks() = default;
+    KeptBlocks(const KeptBlocks&) = delete;
+    KeptBlocks& operator=(const KeptBlocks&) = delete;
+    ~KeptBlocks() {
+        for (void* p : blocks) (void)hipFree(p);
+    }
+};
+
+// A larger block for a buffer that belongs to a set.  The arrays of a batch move
+// together, when one of them is outgrown, and their old blocks are kept: what was
+// captured over them then works on the batch they hold, never on freed memory nor on
+// an old table under a new batch's row numbers.  (One that is large enough moves at its
+// size, so what is kept stays a few times the arrays themselves.)
+template <class T>
+struct Moved {
+    DeviceBuffer<T>& buffer;
+    DeviceBuffer<T> fresh;
+    Moved(std::pair<DeviceBuffer<T>*, size_t> need) : buffer(*need.first) {
+        const size_t have = buffer.count;
+        fresh.reserve(need.second <= have ? have : grown_capacity(need.second, have));
+    }
+    void take(KeptBlocks& kept) {
+        if (buffer.ptr) kept.blocks.push_back(buffer.ptr);
+        buffer.ptr = std::exchange(fresh.ptr, nullptr);
+        buffer.count = fresh.count;
+    }
+};
+// True where a buffer was too small for its size: all of them have then moved (or, where
+// memory ran out, none).
+template <class... T>
+bool reserve_together(KeptBlocks& kept, std::pair<DeviceBuffer<T>*, size_t>... need) {
+    if (((need.first->ptr && need.second <= need.first->count) && ...)) return false;
+    std::tuple<Moved<T>...> moved(need...);
+    kept.blocks.reserve(kept.blocks.size() + sizeof...(T));  // nothing throws from here on
+    std::apply([&](auto&... m) { (m.take(kept), ...); }, moved);
+    return true;
+}
 
 // The arrays of one upload: array p is words[p] words from word 4 * first[p] of
 // pinned host memory (each starts on 16 bytes), bound for dst[p].
@@ -183,10 +226,9 @@ struct DecodeBatch {
     // of other shapes.
     DeviceBuffer<int32_t> tables, pos;
     DeviceBuffer<int32_t> slots;     // per row: page * 16 + position % 16 (where its K/V row goes)
-    void reserve(size_t table_words, size_t rows) {
-        tables.reserve(table_words);
-        pos.reserve(rows);
-        slots.reserve(rows);
+    KeptBlocks kept;
+    bool reserve(size_t table_words, size_t rows) {
+        return reserve_together(kept, std::pair(&tables, table_words), std::pair(&pos, rows), std::pair(&slots, rows));
     }
     // The decode work list last built for this batch, and what it was built for
     // (work_items = 0: longer than the kernel arguments hold).
@@ -230,6 +272,12 @@ struct PrefillBatch {
     int32_t work_items = 0;
     int32_t work_block_m = 0;         // query rows per work item the list was built for
     DeviceBuffer<int32_t> work_wide;  // the same for items of PREFILL_WIDE_ROWS rows
+    KeptBlocks kept;
+    bool reserve(size_t table_words, size_t chunks, size_t rows, size_t work_words, size_t wide_words) {
+        return reserve_together(kept, std::pair(&tables, table_words), std::pair(&seqs, chunks), std::pair(&slots, rows),
+                                std::pair(&row_pos, rows), std::pair(&work, work_words),
+                                std::pair(&work_wide, wide_words));
+    }
     int32_t work_items_wide = 0;
     int32_t max_pos = 0;              // largest position of any row
     // No table entry but a chunk row's own names the page that row lands on:
