@@ -657,11 +657,7 @@ void launch_q8_decode(nitro_kvpool* pool, int layer, const float* q, float* out,
     KvQ8Decode a = q8_decode_args(pool, layer, q, out, n_heads, sh, d.shared_pages);
     if (a.num_splits > 1) {
         pool->q8_partials.reserve((size_t)d.batch * a.num_splits * n_heads * a.pstride);
-        if (pool->q8_counters.reserve((size_t)d.batch * n_kv_heads * sh.groups)) {
-            const DeviceBuffer<int32_t>& n = pool->q8_counters.now;
-            hip_check(hipMemset(n.ptr, 0, n.count * sizeof(int32_t)), "hipMemset");
-            hip_check(hipStreamSynchronize(nullptr), "hipStreamSynchronize");  // s need not wait for the null stream
-        }
+        pool->q8_counters.reserve((size_t)d.batch * n_kv_heads * sh.groups, true);
     }
     a.tables = d.tables.ptr;
     a.positions = d.pos.ptr;

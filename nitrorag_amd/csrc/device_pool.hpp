@@ -70,10 +70,17 @@ template <class T>
 struct KeptBuffer {
     DeviceBuffer<T> now;
     std::vector<std::unique_ptr<DeviceBuffer<T>>> outgrown;
-    bool reserve(size_t n) {
+    // zeroed: a new block is filled with zeros, whole, before it is taken (a fill that
+    // fails leaves the old one in place) and before any stream may use it.
+    bool reserve(size_t n, bool zeroed = false) {
         if (n <= now.count && now.ptr) return false;
         auto bigger = std::make_unique<DeviceBuffer<T>>();
         bigger->reserve(n > 2 * now.count ? n : 2 * now.count);
+        if (zeroed) {
+            hip_check(hipMemset(bigger->ptr, 0, bigger->count * sizeof(T)), "hipMemset");
+            hip_check(hipStreamSynchronize(nullptr), "hipStreamSynchronize");
+        }
+        if (now.ptr) outgrown.reserve(outgrown.size() + 1);
         std::swap(bigger->ptr, now.ptr);
         std::swap(bigger->count, now.count);
         if (bigger->ptr) outgrown.push_back(std::move(bigger));

@@ -1,7 +1,8 @@
-// The device arrays of a pool's batches as they are outgrown, over a stand-in for the
+// The device arrays of a pool's batches and its counters as they are outgrown, over a stand-in for the
 // device allocator that notes what was freed (host code only; test_host_batch_arrays.py).
 #include <cstdio>
 #include <cstdlib>
+#include <cstring>
 #include <set>
 
 #include "device_pool.hpp"
@@ -9,6 +10,7 @@
 namespace {
 std::set<void*> live, freed;
 int left = -1;  // allocations that still succeed (-1: all)
+bool fills = true;
 }  // namespace
 
 extern "C" {
@@ -16,6 +18,7 @@ hipError_t hipMalloc(void** p, size_t n) {
     if (left == 0) return hipErrorOutOfMemory;
     if (left > 0) left--;
     *p = std::malloc(n);
+    std::memset(*p, 0xAA, n);
     live.insert(*p);
     return hipSuccess;
 }
@@ -26,6 +29,12 @@ hipError_t hipFree(void* p) {
     }
     return hipSuccess;
 }
+hipError_t hipMemset(void* p, int value, size_t n) {
+    if (!fills) return hipErrorStreamCaptureUnsupported;
+    std::memset(p, value, n);
+    return hipSuccess;
+}
+hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
 hipError_t hipGetLastError(void) { return hipSuccess; }
 const char* hipGetErrorString(hipError_t) { return "error"; }
 }
@@ -78,6 +87,36 @@ int main() {
             CHECK(live.count(const_cast<void*>(before[i])));
             CHECK(after[i] != before[i]);
         }
+    }
+    CHECK(live.empty());
+    {
+        // arrival counters: zeros from the first launch on, also after one whose fill failed
+        nitro::KeptBuffer<int32_t> counters;
+        fills = false;
+        for (int i = 0; i < 2; i++) {
+            bool thrown = false;
+            try {
+                counters.reserve(64, true);
+            } catch (const nitro::Error&) {
+                thrown = true;
+            }
+            CHECK(thrown && !counters.now.ptr);
+        }
+        fills = true;
+        CHECK(counters.reserve(64, true) && !counters.reserve(64, true));
+        for (size_t i = 0; i < counters.now.count; i++) CHECK(counters.now.ptr[i] == 0);
+        int32_t* first = counters.now.ptr;
+        first[3] = 7;
+        fills = false;
+        try {
+            counters.reserve(1 << 20, true);
+            CHECK(false);
+        } catch (const nitro::Error&) {
+        }
+        CHECK(counters.now.ptr == first && counters.outgrown.empty());
+        fills = true;
+        CHECK(counters.reserve(1 << 20, true) && counters.now.ptr != first && live.count(first) && first[3] == 7);
+        for (size_t i = 0; i < counters.now.count; i++) CHECK(counters.now.ptr[i] == 0);
     }
     CHECK(live.empty());
     std::printf("ok\n");
