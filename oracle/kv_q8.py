@@ -69,6 +69,13 @@ class Cache:
                 at = 32 * self.hdp + base + 4 * t
                 rec[:, at:at + 4] = s[:, None].view(np.uint8)
 
+    def scales(self, layer, table, tokens):
+        """K and V scales of a sequence's first `tokens` tokens, float64 [tokens][kv_heads]."""
+        at = np.arange(tokens)
+        rec = self.data[np.asarray(table)[at // PAGE], layer]
+        s = np.ascontiguousarray(rec[:, :, 32 * self.hdp:]).view(np.float32).astype(np.float64)
+        return s[at, :, at % PAGE], s[at, :, PAGE + at % PAGE]
+
     def values(self, layer, table, tokens):
         """K and V of a sequence's first `tokens` tokens, float64 [tokens][kv_heads][head_dim]."""
         k = np.empty((tokens, self.data.shape[2], self.hd))
@@ -138,3 +145,59 @@ def attention(q, positions, k, v):
             tiles = (n + 63) // 64
             bound[r, h] = np.abs(vh).max() * (2 * weight + 64 * 6e-8 + (2 * tiles + 20) * 2.0 ** -24) + 1e-30
     return out, bound
+
+
+UNITS = 8355000.0  # of a row's largest entry (q) and a group of keys' largest weight
+
+
+def typical_error(q, positions, k, v, k_scales, v_scales, group, units=UNITS):
+    """attention(), and the root mean square of each output row's error norm [rows][heads]
+    as the kernels' roundings make it: q and weights in 24-bit fixed point, the integers'
+    sums rounded to 256 units, everything else in fp32.  `group` keys share a weight's unit
+    (64 in decode, 128 in prefill).
+
+    Each rounding to a step d is taken as uniform in +-d/2 (variance d^2/12; for fp32,
+    relative, 2^-48/3) and independent of the others; u_j = v_j - out is what a relative
+    change of weight p_j moves the output by, times p_j.
+      q        entries off by a step a/units (a: the row's largest; the product before it is
+               rounded costs a quarter more): moves along sum_j p_j k_ji u_j / sqrt(hd)
+      scores   a step of 256 a/units * ks_j / sqrt(hd) each; two fp32 roundings of s_j, one
+               of its distance from the maximum; a factor common to all of a row (four
+               roundings), which moves along sum_j p_j s_j u_j
+      weights  2^-23 of exp2, a rounding of p vs; a step W/units, W = max p vs of the group,
+               times the codes v_j/vs_j
+      sums     a step 256 W/units per group and dimension; the group's own factor (2^-23,
+               in the output alone) and its place in the softmax (2^-22); two roundings for
+               each group of what is summed so far; the sum of the weights and the division"""
+    rows, heads, hd = q.shape
+    out, typical = np.empty((rows, heads, hd)), np.empty((rows, heads))
+    per = heads // k.shape[1]
+    eps2 = 2.0 ** -48 / 3
+    for r in range(rows):
+        n = int(positions[r]) + 1
+        starts = np.arange(0, n, group)
+        for h in range(heads):
+            g = h // per
+            kh, vh, ks, vs = k[:n, g], v[:n, g], k_scales[:n, g], v_scales[:n, g]
+            x = q[r, h].astype(np.float64)
+            a = np.abs(x).max()
+            s = kh @ x / np.sqrt(hd)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            o = p @ vh
+            u = vh - o
+            u2, v2 = (u * u).sum(-1), (vh * vh).sum(-1)
+            step = a / units
+            var = step ** 2 * (5 / 48) / hd * (((kh * p[:, None]).T @ u) ** 2).sum()
+            each = (256 * step * ks) ** 2 / (12 * hd) + eps2 * (2 * s * s + (s - s.max()) ** 2)
+            var += (p * p * (each + 4 * eps2) * u2).sum() + (p * p * v2).sum() * eps2
+            var += 16 * 2.0 ** -48 * (((p * (s - p @ s)) @ u) ** 2).sum()
+            W = np.maximum.reduceat(p * vs, starts) / units
+            codes2 = v2 / np.where(vs > 0, vs, 1) ** 2
+            var += (np.add.reduceat(codes2, starts) / 12 + hd * 256 ** 2 / 12) @ (W * W)
+            own, moved = (np.add.reduceat(p[:, None] * z, starts) for z in (vh, u))
+            var += 2.0 ** -46 * (own ** 2).sum() + 2.0 ** -44 * (moved ** 2).sum()
+            var += 2 * eps2 * (np.cumsum(own, 0) ** 2).sum()
+            var += eps2 * (20 + 2 * len(starts)) * (o * o).sum()
+            out[r, h], typical[r, h] = o, np.sqrt(var)
+    return out, typical
