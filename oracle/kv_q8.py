@@ -122,13 +122,16 @@ def attention(q, positions, k, v):
     """q [rows][heads][hd] at `positions` over keys 0..position; with a bound on what
     fp32 arithmetic with 24-bit fixed point may be off, elementwise [rows][heads][1].
 
-    The bound: an entry of q is off by at most 6e-8 of its row's largest (half a unit
-    of 1/8355000), so a score is off by that times the key's 1-norm; fp32 rounds it
-    about six times (conversions, the two factors, the sum of the digits, the
+    The bound: an entry of q is off by at most 6e-8 of its row's largest a (half a unit
+    of a/8355000), so a score is off by that times the key's 1-norm; its joined integer
+    by half of 256 units times the key's scale, at most 128 a/8355000 * max|k|/127 =
+    1.21e-7 a max|k|; fp32 rounds it about six times (conversions, the two factors, the
     difference from the maximum).  A weight is then off by that, relative, and 2^-22
-    (exp2, its sum).  As numerator and denominator: twice.  The weights' own
-    fixed point: at most 64 half units per tile of the tile's largest, whose sum over
-    tiles is at most the denominator.  Joining the tiles: two roundings each."""
+    (exp2, its sum).  As numerator and denominator: twice.  The weights' own fixed
+    point: half a unit (6e-8) of the largest of those that share it, at most 128 of them
+    (prefill's two tiles), and the sum of those largest ones is at most the denominator;
+    the joined integers of an output half of 256 units once for them, 1.21e-7 of it.
+    Joining the tiles: two roundings each."""
     rows, heads, hd = q.shape
     out, bound = np.empty((rows, heads, hd)), np.empty((rows, heads, 1))
     per = heads // k.shape[1]
@@ -140,10 +143,11 @@ def attention(q, positions, k, v):
             s = kh @ x / np.sqrt(hd)
             p = np.exp(s - s.max())
             out[r, h] = p @ vh / p.sum()
-            off = np.abs(x).max() * 6e-8 * np.abs(kh).sum(-1).max() / np.sqrt(hd) + 6 * 2.0 ** -24 * np.abs(s).max()
+            off = np.abs(x).max() * (6e-8 * np.abs(kh).sum(-1).max() + 1.21e-7 * np.abs(kh).max()) / np.sqrt(hd)
+            off += 6 * 2.0 ** -24 * np.abs(s).max()
             weight = off + 2.0 ** -22
             tiles = (n + 63) // 64
-            bound[r, h] = np.abs(vh).max() * (2 * weight + 64 * 6e-8 + (2 * tiles + 20) * 2.0 ** -24) + 1e-30
+            bound[r, h] = np.abs(vh).max() * (2 * weight + 128 * 6e-8 + 1.21e-7 + (2 * tiles + 20) * 2.0 ** -24) + 1e-30
     return out, bound
 
 

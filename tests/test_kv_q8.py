@@ -59,3 +59,21 @@ def test_plain_form_places_every_byte():
     kc = kv_q8.quantise(k, v)[0]
     token, d = 7, 18
     assert cache.data[2, 1, 0, ((token // 4 * 2 + d // 16) * 4 + token % 4) * 16 + d % 16] == kc[token, 0, d].view(np.uint8)
+
+
+def test_the_bound_counts_every_rounding():
+    """It holds the sum of them: 128 weights that share a unit of the first one's, each off by
+    half of it in the direction of the largest value; the integers of a score and of an output
+    joined half of 256 units off; q's steps; six fp32 roundings of a score and one of exp2, for
+    numerator and denominator; two for each of two tiles."""
+    hd, n = 4, 128
+    k, v = np.zeros((n, 1, hd)), np.ones((n, 1, hd))
+    k[0] = 1
+    for far in (5.0, 8.0, 12.0):
+        q = np.full((1, 1, hd), far / hd * np.sqrt(hd), np.float32)  # the first score is `far`, the others 0
+        bound = kv_q8.attention(q, [n - 1], k, v)[1][0, 0, 0]
+        p = np.exp(-far)
+        total = 1 + (n - 1) * p
+        scores = 6e-8 * float(q.max()) * hd / np.sqrt(hd) + 128 / 8355000 * float(q.max()) / 127 / np.sqrt(hd)
+        weights = n * 0.5 / 8355000 / total + 128 / 127 / 8355000 / total
+        assert bound >= 2 * (scores + 6 * 2.0 ** -24 * far + 2.0 ** -22) + weights + 4 * 2.0 ** -24
