@@ -155,7 +155,7 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  * code = rint(x * inv), inv = 127 / a (both quotients fp32, the product exact, ties
  * to even); the value is code * scale.  Rows with a < 2^-100 are held as zeros.  A
  * head's row of K or V with an infinity or a NaN in it is held as NaN, K and V both:
- * every output that attends the token is NaN, no other one is.  Attention works on
+ * every output that attends the token is NaN, and for it no other one is.  Attention works on
  * the values held, the step's own rows among them.
  *   Storage: num_pages * num_layers * n_kv_heads records [page][layer][kv_head] of
  * nitro_kvpool_q8_record_bytes(head_dim) = 32 * hdp + 128 bytes, hdp = head_dim
@@ -164,8 +164,10 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  * create_q8 owns zero-filled memory, wrap_q8 borrows a caller's (16-byte aligned).
  * In records that a caller writes itself, scales are not negative; a token with one that
  * is not finite counts as NaN.
- *   Attention takes q and K up to 1e36 in magnitude; parts of its output that come from V
- * below 2^-96 may be zero.  Two rows of one batch that go to the same slot leave a mixture
+ *   Attention takes finite q and K up to 1e36 in magnitude whose scores fp32 holds: a row
+ * with a score |q.k| * log2(e) / sqrt(head_dim) past its range may be NaN, no other row is.
+ * A head's q with no magnitude of 2^-100 or more counts as zeros.  Parts of the output that
+ * come from V below 2^-96 may be zero.  Two rows of one batch that go to the same slot leave a mixture
  * of both there, as in an fp32 pool.
  *   A pool holds less than 512 GiB and is used on the device that was current when it was
  * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  As for

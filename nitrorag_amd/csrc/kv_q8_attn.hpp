@@ -262,13 +262,23 @@ struct Weights {
 template <int CH, int H>
 __device__ __forceinline__ Weights<H> weigh(State<CH>& st, f4 (&s)[H][4], float top, float scale, const float (&scales)[H]) {
     const float base = top == -INFINITY ? 0.0f : top * scale;  // no key (or only NaN ones) in the tiles
-    float sum = 0.0f, big = 0.0f;
+    float sum = 0.0f, big = 0.0f, shift = base;
+    // base is rounded and s * scale below is not: they differ by up to 2^-24 of base at the
+    // maximum itself.  A small difference is the tiles' common factor (m carries it); a large
+    // one leaves exp2's range, so there the maximum is taken off first (infinite: NaN).
+    const bool far = fabsf(base) >= 0x1p26f;
+    if (__builtin_amdgcn_ballot_w64(far)) {
+        shift = far ? base - base : base;
+#pragma unroll
+        for (int h = 0; h < H; h++)
+            each_token([&](auto n) { s[h][n / 4][n % 4] -= far ? top : 0.0f; });
+    }
 #pragma unroll
     for (int h = 0; h < H; h++) {
         const float vs = fabsf(scales[h]) < INFINITY ? scales[h] : 0.0f;
         each_token([&](auto n) {
             constexpr int t = n / 4, r = n % 4;
-            const float p = exp2_fast(fmaf(s[h][t][r], scale, -base));
+            const float p = exp2_fast(fmaf(s[h][t][r], scale, -shift));
             sum += p;
             s[h][t][r] = p * of_token<n>(vs);
             big = fmaxf(big, s[h][t][r]);

@@ -155,3 +155,63 @@ def test_joins_of_many_splits(heads, tokens):
     want, typical = kv_q8.typical_error(q.reshape(1, H, hd), [tokens - 1], k, v, *ref.scales(0, table[0], tokens), 64)
     check_error(out.cpu().numpy().reshape(1, H, hd), want, typical, "join")
     assert pool.take_device_errors() == 0
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_the_range_of_scores(prefill):
+    """Scores up to fp32's end, of either sign, are one-hot weights; a row whose scores pass it
+    leaves the others as they were; a q below 2^-100 counts as zeros."""
+    import torch
+
+    heads = (2, 2, 64)
+    say("range of scores", prefill)
+    c = Tight(66, [(0, 130)], heads)
+    K = c.heads(c.k)
+    K *= np.float32(1e3)
+    K[..., 0] = 3000 + 7 * c.rng.permutation(130)[:, None]
+    c.put()
+    c.cache.copy_(to_gpu(c.ref.data))
+    k, v = c.ref.values(c.layer, c.tables[0], 130)
+    plain = c.q.copy()
+    Q = c.heads(c.q)
+    far = {}
+    for i, power in enumerate((2, 3, 4, 5, 6, 7, 8, 9, 10, 15, 20, 30, 32)):
+        far[30 + 3 * i] = power + 1.0
+        Q[30 + 3 * i] *= np.float32(10.0 ** (power + 1))
+        for row, sign in ((31 + 3 * i, 1), (32 + 3 * i, -1)):  # scores of one sign
+            far[row] = sign
+            Q[row] = 0
+            Q[row, :, 0] = sign * np.float32(10.0 ** power)
+    Q[80] *= np.float32(1e36)   # scores past 1e39
+    Q[85] *= np.float32(2e-31)  # below 2^-100 (8e-31)
+    outs = []
+    for q in (plain, c.q):
+        out = torch.full((130, 128), float("nan"), device="cuda")
+        if prefill:
+            c.upload(True)
+            c.pool.prefill(c.layer, to_gpu(q), out, *heads)
+        else:
+            c.pool.upload_decode_batch(np.repeat(c.tables, 130, 0), c.pos)
+            c.pool.decode(c.layer, to_gpu(q), out, *heads)
+        outs.append(c.heads(out.cpu().numpy()))
+    same = np.ones(130, bool)
+    same[[80, 85, *far]] = False
+    assert np.isfinite(outs[0]).all()
+    np.testing.assert_array_equal(outs[1][same], outs[0][same])
+    seen = 0
+    for row in far:
+        for h in range(2):
+            s = k[:row + 1, h] @ Q[row, h].astype(np.float64) / 8
+            first, second = np.sort(s)[[-1, -2]]
+            # (a score is off by the steps of q and of the joined integer, and six roundings)
+            off = np.abs(Q[row, h]).max() * (6e-8 * np.abs(k[:row + 1, h]).sum(-1).max() + 1.21e-7 * np.abs(k).max()) / 8
+            if first - second < 40 + 2 * (off + 6 * 2.0 ** -24 * np.abs(s).max()):
+                continue
+            seen += 1
+            # one weight of 1 beside 130 of e^-40: its step, the joined integer's, three roundings
+            want = v[int(np.argmax(s)), h]
+            assert np.abs(outs[1][row, h] - want).max() <= np.abs(want).max() * 5e-7, (row, far[row], h)
+    assert seen >= 60, seen
+    for h in range(2):
+        mean = v[:86, h].mean(0)
+        assert np.abs(outs[1][85, h] - mean).max() <= np.abs(v[:86, h]).max() * 128 * 6e-8
