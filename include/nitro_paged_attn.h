@@ -161,7 +161,8 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  * nitro_kvpool_q8_record_bytes(head_dim) = 32 * hdp + 128 bytes, hdp = head_dim
  * rounded up to 16: K codes [4][hdp/16][4][16] (token 4a + r, dimension 16c + i at
  * [a][c][r][i]), V codes [hdp][16] (dimension, token), K scales [16], V scales [16].
- * create_q8 owns zero-filled memory, wrap_q8 borrows a caller's (16-byte aligned).
+ * create_q8 owns zero-filled memory, wrap_q8 borrows a caller's (16-byte aligned, of the
+ * current device).
  * In records that a caller writes itself, scales are not negative; a token with one that
  * is not finite counts as NaN.
  *   Attention takes finite q and K up to 1e36 in magnitude whose scores fp32 holds: a row

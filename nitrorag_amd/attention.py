@@ -136,6 +136,8 @@ class KVPool:
             raise TypeError("cache must be a GPU tensor")
         if cache.dtype is not torch.uint8 or not cache.is_contiguous():
             raise TypeError("cache must be contiguous uint8")
+        if cache.device.index != torch.cuda.current_device():  # the pool's from now on
+            raise ValueError(f"cache is on {cache.device}, which is not the current device")
         if cache.dim() != 4 or cache.shape[3] != kv_record_bytes(head_dim):
             raise ValueError(f"cache must be [pages][layers][kv_heads][{kv_record_bytes(head_dim)}]")
         self, h = cls.__new__(cls), ctypes.c_void_p()
