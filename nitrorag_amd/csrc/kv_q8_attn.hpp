@@ -262,23 +262,20 @@ struct Weights {
 template <int CH, int H>
 __device__ __forceinline__ Weights<H> weigh(State<CH>& st, f4 (&s)[H][4], float top, float scale, const float (&scales)[H]) {
     const float base = top == -INFINITY ? 0.0f : top * scale;  // no key (or only NaN ones) in the tiles
-    float sum = 0.0f, big = 0.0f, shift = base;
     // base is rounded and s * scale below is not: they differ by up to 2^-24 of base at the
-    // maximum itself.  A small difference is the tiles' common factor (m carries it); a large
-    // one leaves exp2's range, so there the maximum is taken off first (infinite: NaN).
-    const bool far = fabsf(base) >= 0x1p26f;
-    if (__builtin_amdgcn_ballot_w64(far)) {
-        shift = far ? base - base : base;
-#pragma unroll
-        for (int h = 0; h < H; h++)
-            each_token([&](auto n) { s[h][n / 4][n % 4] -= far ? top : 0.0f; });
-    }
+    // maximum itself.  A small difference is the tiles' common factor (m carries it), a large
+    // one would leave exp2's range: past 2^26 both are brought down to it, by a power of two.
+    // (Scores that far are 2^-24 of themselves exact at best, so two that differ are then
+    // still 4 apart, and those that are clearly less keep no weight.)
+    const int down = min(26 - __builtin_amdgcn_frexp_expf(base), 0);
+    const float near = __builtin_amdgcn_ldexpf(scale, down), shift = __builtin_amdgcn_ldexpf(base, down);
+    float sum = 0.0f, big = 0.0f;
 #pragma unroll
     for (int h = 0; h < H; h++) {
         const float vs = fabsf(scales[h]) < INFINITY ? scales[h] : 0.0f;
         each_token([&](auto n) {
             constexpr int t = n / 4, r = n % 4;
-            const float p = exp2_fast(fmaf(s[h][t][r], scale, -shift));
+            const float p = exp2_fast(fmaf(s[h][t][r], near, -shift));
             sum += p;
             s[h][t][r] = p * of_token<n>(vs);
             big = fmaxf(big, s[h][t][r]);
