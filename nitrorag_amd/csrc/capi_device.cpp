@@ -555,7 +555,9 @@ void launch_decode(nitro_kvpool* pool, int layer, const float* q, float* out, co
 // resident, they follow one another as they finish, and the last ones run alone.
 // (Constants fitted to 24 batches, 1 to 64 sequences of 16 to 131072 tokens at head
 // sizes 36 to 256, each in splits of 4 to 96 tiles: the choice is 0.7% slower than the
-// best of those in the mean, 4% at most.)
+// best of those in the mean, 4% at most.  t_alone, of one tile after another in a wave,
+// is such a fit and no measurement of a tile.  Resident workgroups are counted by the
+// waves that the builds are compiled for; at head size 80 registers allow a third.)
 // Sequences that are not split are taken longest first, every second round of CUs
 // backwards: a CU with one of the longest then has one of the shortest beside it.
 template <class Ctx>

@@ -131,8 +131,10 @@ __device__ __forceinline__ int item_of(const KvQ8Decode& a, int i, int lane, int
 
 // A workgroup takes one split of one sequence's keys for up to 16 query heads of a
 // K/V head; its waves take the split's tiles in turn.  Waves per SIMD are what the
-// registers allow without spills (at head size 128 208; an earlier form had 183, and
-// three waves with 13 of them spilled took 404 us where two took 337).
+// registers allow without spills (at head size 128 210; an earlier form had 183, and
+// three waves with 13 of them spilled took 404 us where two took 337).  At head sizes
+// 132 to 176 the build keeps a K operand in scratch, 80 bytes a lane: 16 sequences of
+// 1024 at 16/8 x 160 take 18.6 us where 16/8 x 192 take 14.8.
 template <int CH, bool STREAM>
 __global__ __launch_bounds__(256, kv_q8_decode_occupancy(16 * CH)) void kv_q8_decode_kernel(KvQ8Decode a) {
     extern __shared__ float s_part[];  // [waves][cols][pstride], then of a join [cols][parts] factors and [cols] sums

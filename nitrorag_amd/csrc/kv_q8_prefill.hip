@@ -2,13 +2,16 @@
 // row over the keys up to its own position (the products and the softmax:
 // kv_q8_attn.hpp).
 //
-// Bound by the vector instructions around the products, 347 per tile of 64 keys and 16
+// Bound by the vector instructions around the products, 350 per tile of 64 keys and 16
 // rows at head size 128 beside 48 matrix ones: 79% of the SIMDs' cycles, the matrix
 // cores are busy in 38%.  8192 tokens at 32 x 128: 975-1060 us (520-560 TFLOP/s of
 // fp32-grade work; cards differ), four chunks of 384 to 512 behind up to 4096 cached
 // tokens at 32/8 x 128 130-140 us, 8 prompts of 128 to 1024 at 12 x 64 21-23 us.  (Four
 // tiles under one maximum rather than two: 8% fewer vector instructions, V a run of 16
-// dimensions at a time, 1029 us.)
+// dimensions at a time, 1029 us.)  Builds that hold part of their operands in scratch,
+// in bytes a lane: head sizes 20-32 52, 36-48 112, 100-112 56, 132-176 432, 212-224 48,
+// 228-240 140.  2048 tokens at 16/8 heads of 112, 128, 160 and 192 take 48, 47, 156 and
+// 86 us.
 #include <hip/hip_runtime.h>
 
 #include "device_pool.hpp"
