@@ -168,8 +168,9 @@ int nitro_kvpool_shape(const nitro_kvpool* pool, int32_t* num_pages, int32_t* nu
  *   Attention takes finite q and K up to 1e36 in magnitude whose scores fp32 holds: a row
  * with a score |q.k| * log2(e) / sqrt(head_dim) past its range may be NaN, no other row is.
  * A head's q with no magnitude of 2^-100 or more counts as zeros.  Parts of the output that
- * come from V below 2^-96 may be zero.  Two rows of one batch that go to the same slot leave a mixture
- * of both there, as in an fp32 pool.
+ * come from V below 2^-96 may be zero, and V times the number of keys is to stay in fp32's
+ * range (weights of up to 1 are summed before they are divided).  Two rows of one batch that
+ * go to the same slot leave a mixture of both there, as in an fp32 pool.
  *   A pool holds less than 512 GiB and is used on the device that was current when it was
  * made: calls with another one current are refused (NITRO_ERR_INVALID_ARGUMENT).  As for
  * an fp32 pool, launches that overlap on one pool race on its workspace for splits.
