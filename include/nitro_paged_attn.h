@@ -367,6 +367,53 @@ int nitro_q8_matmul(const void* w, const float* x, float* out, int32_t batch, in
 #define NITRO_Q8_LAUNCH_QKV 3
 int nitro_q8_tile_rows(int32_t launch, int32_t batch, int32_t n, int32_t d, int32_t d_kv, int32_t* rows);
 
+/* ------------------------- rows held in 8 bits -----------------------------
+ * No counterpart in the reference, whose activations are fp32 throughout: what a
+ * layer's products read held in 8 bits, as their weights are, and products of such
+ * rows.  Where products bound a step (prompts, large batches) they take a fraction of
+ * nitro_q8_matmul's time; the price is the rows' rounding.
+ *   A row y of n fp32 numbers is held as n int8 codes and one fp32 scale: with a =
+ * max |y|, scale = a / 127 and code = rint(y * inv), inv = 127 / a (both quotients
+ * fp32, the product exact, ties to even); the value is code * scale.  Rows with a <
+ * 2^-100 are held as zeros.  A row with an infinity or a NaN in it gets a NaN for its
+ * scale and zeros for codes: all that is computed from it is NaN, and nothing else is.
+ *   codes: device int8 [rows][n]; scales: device fp32 [rows].  Rows of any n > 0. */
+
+/* codes, scales = rms_norm (src/model_q8.cpp:128-140) of x [rows][n], held:
+ *   h = x + residual (fp32; residual may be NULL)
+ *   y = h * weight / sqrt(mean(h^2) + eps), computed in 64 bits and rounded once
+ * sum (NULL: not written) receives h and may be x or residual; eps > 0. */
+int nitro_rms_norm_row8(const float* x, const float* residual, const float* weight, double eps, float* sum,
+                        int8_t* codes, float* scales, int32_t rows, int32_t n, void* stream);
+/* codes, scales = the rows of x held; x = the values that rows hold. */
+int nitro_row8_quantize(const float* x, int8_t* codes, float* scales, int32_t rows, int32_t n, void* stream);
+int nitro_row8_read(const int8_t* codes, const float* scales, float* x, int32_t rows, int32_t n, void* stream);
+
+/* A Q8_0 matrix laid out for such rows: w is device BlockQ8 rows (d rows of n / 32
+ * blocks, 4-byte aligned), n a multiple of 32; a copy of 1.125 bytes a weight is made
+ * (the caller may free w).  With w_gate, of the same shape, the pair computes
+ * act(w_gate . x) * (w . x).  Used on the device that was current at its creation. */
+typedef struct nitro_q8_weights nitro_q8_weights;
+int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_t d, nitro_q8_weights** out);
+int nitro_q8_weights_destroy(nitro_q8_weights* weights);
+
+enum {
+    NITRO_ACT_NONE = 0,
+    NITRO_ACT_RELU = 1,
+    NITRO_ACT_SILU = 2,      /* x / (1 + exp(-x)) */
+    NITRO_ACT_GELU = 3,      /* x * Phi(x), Phi the normal distribution's */
+    NITRO_ACT_GELU_TANH = 4  /* x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3) */
+};
+/* out[b][i] = act(p[b][i] + bias[i]) + residual[b][i], b < rows, i < d, with
+ *   p[b][i] = scales[b] * sum_j ws[i][j] * sum_t wq[i][32j + t] * codes[b][32j + t];
+ * of a gated pair out = act(p_gate + bias[i]) * (p + bias[d + i]) + residual.
+ * codes [rows][n] 16-byte aligned, bias [d] ([2][d] of a pair) or NULL, residual and out
+ * [rows][d] fp32 (residual NULL, or out itself).  The sums over t are exact integers,
+ * those over j fp32, in an order that depends on rows, n and d only.  Allocates nothing;
+ * calls on one matrix may overlap. */
+int nitro_row8_matmul(const nitro_q8_weights* weights, const int8_t* codes, const float* scales, const float* bias,
+                      const float* residual, float* out, int32_t rows, int32_t activation, void* stream);
+
 /* ------------------------ transformer step (model) -------------------------
  * The forward passes of src/model_q8.cpp around the attention path, on the
  * device: embedding, per layer rms_norm -> wq/wk/wv (Q8) -> RoPE + KV append

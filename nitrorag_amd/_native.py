@@ -103,6 +103,12 @@ SIGNATURES = {
                                      _vp],
     "nitro_q8_matmul": [_vp, _fp, _fp, _i32, _i32, _i32, _i32, _vp],
     "nitro_q8_tile_rows": [_i32, _i32, _i32, _i32, _i32, _i32p],
+    "nitro_rms_norm_row8": [_fp, _fp, _fp, ctypes.c_double, _fp, _vp, _fp, _i32, _i32, _vp],
+    "nitro_row8_quantize": [_fp, _vp, _fp, _i32, _i32, _vp],
+    "nitro_row8_read": [_vp, _fp, _fp, _i32, _i32, _vp],
+    "nitro_q8_weights_create": [_vp, _vp, _i32, _i32, ctypes.POINTER(_vp)],
+    "nitro_q8_weights_destroy": [_vp],
+    "nitro_row8_matmul": [_vp, _vp, _fp, _fp, _fp, _fp, _i32, _i32, _vp],
     "nitro_model_create": [_vp, ctypes.c_uint64, ctypes.POINTER(_vp)],
     "nitro_model_destroy": [_vp],
     "nitro_model_config": [_vp, _i32p],

@@ -25,8 +25,9 @@ LIB = os.path.join(HERE, "libnitro_paged_attn.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("NITRO_OFFLOAD_ARCH", "gfx950")
 DEVICE_SOURCES = ["paged_attn_decode.hip", "paged_attn_prefill.hip", "kv_append.hip", "q8_matmul.hip", "q8_gemm.hip",
-                  "kv_q8_append.hip", "kv_q8_decode.hip", "kv_q8_prefill.hip", "model_kernels.hip", "scheduler_kernels.hip"]
-HIP_HOST_SOURCES = ["capi_device.cpp", "model.cpp", "scheduler_step.cpp"]
+                  "kv_q8_append.hip", "kv_q8_decode.hip", "kv_q8_prefill.hip", "row8.hip", "row8_matmul.hip",
+                  "model_kernels.hip", "scheduler_kernels.hip"]
+HIP_HOST_SOURCES = ["capi_device.cpp", "capi_row8.cpp", "model.cpp", "scheduler_step.cpp"]
 HOST_SOURCES = ["paged_memory.cpp", "capi_host.cpp", "scheduler.cpp", "rpc.cpp"]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}", "-Wall"]
