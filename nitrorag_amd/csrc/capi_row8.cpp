@@ -75,7 +75,7 @@ int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_
         require(w != nullptr, ERR_INVALID_ARGUMENT, "null weights");
         require(n > 0 && d > 0, ERR_INVALID_ARGUMENT, "n and d must be positive");
         require(n % 32 == 0, ERR_INVALID_ARGUMENT, "n must be a multiple of 32 (Q8 block)");
-        require(n <= 1 << 30 && d <= 1 << 30, ERR_UNSUPPORTED, "more than 2^30 rows or columns");
+        require(n <= 1 << 30 && d <= 1 << 29, ERR_UNSUPPORTED, "more than 2^30 columns or 2^29 rows");
         require(aligned(w, 4) && aligned(w_gate, 4), ERR_INVALID_ARGUMENT, "weights must be 4-byte aligned");
         auto m = std::make_unique<nitro_q8_weights>();
         m->n = n, m->d = d, m->gated = w_gate != nullptr, m->device = current_device();

@@ -22,34 +22,9 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Entries 4v .. 4v + 3 of a row of n (zeros past its end).
-__device__ __forceinline__ f32x4 load4(const float* row, int v, int n) {
-    if (4 * v + 3 < n) return *reinterpret_cast<const f32x4_any*>(row + 4 * v);
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 3; e++)
-        if (4 * v + e < n) x[e] = row[4 * v + e];
-    return x;
-}
-__device__ __forceinline__ void store4(float* row, int v, int n, f32x4 x) {
-    if (4 * v + 3 < n) {
-        *reinterpret_cast<f32x4_any*>(row + 4 * v) = x;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; e++)
-        if (4 * v + e < n) row[4 * v + e] = x[e];
-}
-// c: entries 4v .. 4v + 3's codes, a byte each.
-__device__ __forceinline__ void store_codes(int8_t* row, int v, int n, uint32_t c) {
-    if (4 * v + 3 < n) {
-        *reinterpret_cast<u32_any*>(row + 4 * v) = c;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; e++)
-        if (4 * v + e < n) row[4 * v + e] = (int8_t)(c >> (8 * e));
-}
+__device__ __forceinline__ f32x4 load4(const float* row, int at) { return *reinterpret_cast<const f32x4_any*>(row + at); }
+__device__ __forceinline__ void store4(float* row, int at, f32x4 x) { *reinterpret_cast<f32x4_any*>(row + at) = x; }
+__device__ __forceinline__ void store4(int8_t* row, int at, uint32_t codes) { *reinterpret_cast<u32_any*>(row + at) = codes; }
 
 __device__ __forceinline__ double joined(double a, double b) { return a + b; }
 __device__ __forceinline__ uint32_t joined(uint32_t a, uint32_t b) { return a > b ? a : b; }
@@ -69,10 +44,10 @@ __device__ __forceinline__ V over_row(V x, V* parts) {
     return x;
 }
 
-__device__ __forceinline__ f32x4 normed(f32x4 h, const float* weight, int v, int n, double r) {
-    const f32x4 w = load4(weight, v, n);
+__device__ __forceinline__ float normed(float h, float weight, double r) { return (float)((double)h * r * (double)weight); }
+__device__ __forceinline__ f32x4 normed(f32x4 h, f32x4 w, double r) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) h[e] = (float)((double)h[e] * r * (double)w[e]);
+    for (int e = 0; e < 4; e++) h[e] = normed(h[e], w[e], r);
     return h;
 }
 __device__ __forceinline__ double squares(f32x4 h, double s) {
@@ -80,9 +55,10 @@ __device__ __forceinline__ double squares(f32x4 h, double s) {
     for (int e = 0; e < 4; e++) s = fma((double)h[e], (double)h[e], s);
     return s;
 }
+__device__ __forceinline__ uint32_t largest(float y, uint32_t top) { return joined(top, __float_as_uint(y) & 0x7fffffffu); }
 __device__ __forceinline__ uint32_t largest(f32x4 y, uint32_t top) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) top = joined(top, __float_as_uint(y[e]) & 0x7fffffffu);
+    for (int e = 0; e < 4; e++) top = largest(y[e], top);
     return top;
 }
 
@@ -91,58 +67,71 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
     if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
     return __uint_as_float(top) < 0x1p-100f ? 0.0f : __uint_as_float(top) / 127.0f;
 }
+// (0: zeros for codes)
 __device__ __forceinline__ float inverse_of(uint32_t top) {
     return top >= 0x7f800000u || __uint_as_float(top) < 0x1p-100f ? 0.0f : 127.0f / __uint_as_float(top);
 }
-// The codes of four entries, a byte each (inv = 0: zeros).
+// The code in the lowest byte: the fma rounds the exact product to an integer, once (a sum
+// with 1.5 * 2^23 has whole units).
+__device__ __forceinline__ uint32_t code_of(float y, float inv) {
+    return __float_as_uint(fmaf(inv == 0.0f ? 0.0f : y, inv, 12582912.0f));
+}
 __device__ __forceinline__ uint32_t codes_of(f32x4 y, float inv) {
-    uint32_t c = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const double p = (double)(inv == 0.0f ? 0.0f : y[e]) * (double)inv;
-        c |= ((uint32_t)(int)rint(p) & 255u) << (8 * e);
-    }
-    return c;
+    const uint32_t low = __builtin_amdgcn_perm(code_of(y[1], inv), code_of(y[0], inv), 0x0c0c0400u);
+    const uint32_t high = __builtin_amdgcn_perm(code_of(y[3], inv), code_of(y[2], inv), 0x0c0c0400u);
+    return low | high << 16;
 }
 
 // T lanes to a row (256 / T rows to a workgroup, or one), the row in V groups of four
-// entries per lane.
+// entries per lane; the last n % 4 entries are one more of the first lanes each.
 template <int T, int V, bool NORM>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a) {
     constexpr int ROWS = T < 256 ? 256 / T : 1;
     __shared__ double sums[T / 64];
     __shared__ uint32_t tops[T / 64];
-    const int lane = threadIdx.x % T, n = a.n, groups = (n + 3) / 4;
-    const int row = blockIdx.x * ROWS + threadIdx.x / T;
+    const int lane = threadIdx.x % T, n = a.n, end = n & ~3;
+    const int row = blockIdx.x * ROWS + (ROWS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0);
     if (row >= a.rows) return;  // (only where a wave has a row: no barrier there)
     const size_t at = (size_t)row * n;
+    const float* const x = a.x + at;
+    int8_t* const codes = a.codes + at;
+    const bool last = lane < n - end;
     f32x4 h[V];
+    float tail = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         h[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (lane + i * T < groups) h[i] = load4(a.x + at, lane + i * T, n);
+        if (4 * (lane + i * T) < end) h[i] = load4(x, 4 * (lane + i * T));
     }
+    if (last) tail = x[end + lane];
     if constexpr (NORM) {
         if (a.residual) {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (lane + i * T < groups) h[i] += load4(a.residual + at, lane + i * T, n);
+                if (4 * (lane + i * T) < end) h[i] += load4(a.residual + at, 4 * (lane + i * T));
+            if (last) tail += a.residual[at + end + lane];
         }
         if (a.sum) {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (lane + i * T < groups) store4(a.sum + at, lane + i * T, n, h[i]);
+                if (4 * (lane + i * T) < end) store4(a.sum + at, 4 * (lane + i * T), h[i]);
+            if (last) a.sum[at + end + lane] = tail;
         }
-        double s = 0.0;
+        double s = (double)tail * (double)tail;
 #pragma unroll
-        for (int i = 0; i < V; i++) s = squares(h[i], s);
-        s = over_row<T>(s, sums);
-        const double r = 1.0 / sqrt(s / n + a.eps);
+        for (int i = 0; i < V; i++) {
+            s = squares(h[i], s);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (64-bit values of four groups at a time)
+        }
+        const double r = 1.0 / sqrt(over_row<T>(s, sums) / n + a.eps);
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (lane + i * T < groups) h[i] = normed(h[i], a.weight, lane + i * T, n, r);
+        for (int i = 0; i < V; i++) {
+            if (4 * (lane + i * T) < end) h[i] = normed(h[i], load4(a.weight, 4 * (lane + i * T)), r);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (last) tail = normed(tail, a.weight[end + lane], r);
     }
-    uint32_t top = 0;
+    uint32_t top = largest(tail, 0);
 #pragma unroll
     for (int i = 0; i < V; i++) top = largest(h[i], top);
     top = over_row<T>(top, tops);
@@ -150,7 +139,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a
     const float inv = inverse_of(top);
 #pragma unroll
     for (int i = 0; i < V; i++)
-        if (lane + i * T < groups) store_codes(a.codes + at, lane + i * T, n, codes_of(h[i], inv));
+        if (4 * (lane + i * T) < end) store4(codes, 4 * (lane + i * T), codes_of(h[i], inv));
+    if (last) codes[end + lane] = (int8_t)code_of(tail, inv);
 }
 
 // Rows of any width, a workgroup each, read again for every use.
@@ -159,34 +149,43 @@ __global__ __launch_bounds__(1024) void row8_long_kernel(Row8Norm a) {
     constexpr int T = 1024;
     __shared__ double sums[T / 64];
     __shared__ uint32_t tops[T / 64];
-    const int lane = threadIdx.x, n = a.n, groups = (n + 3) / 4;
+    const int lane = threadIdx.x, n = a.n, end = n & ~3;
     const size_t at = (size_t)blockIdx.x * n;
     const float* x = a.x + at;
     const float* residual = a.residual ? a.residual + at : nullptr;
+    int8_t* const codes = a.codes + at;
+    const bool last = lane < n - end;
+    float tail = last ? x[end + lane] : 0.0f;
     double r = 0.0;
     if constexpr (NORM) {
-        double s = 0.0;
-        for (int v = lane; v < groups; v += T) {
-            f32x4 h = load4(x, v, n);
-            if (residual) h += load4(residual, v, n);
-            if (a.sum) store4(a.sum + at, v, n, h);
+        if (last && residual) tail += residual[end + lane];
+        if (last && a.sum) a.sum[at + end + lane] = tail;
+        double s = (double)tail * (double)tail;
+#pragma unroll 4
+        for (int v = 4 * lane; v < end; v += 4 * T) {
+            f32x4 h = load4(x, v);
+            if (residual) h += load4(residual, v);
+            if (a.sum) store4(a.sum + at, v, h);
             s = squares(h, s);
         }
         if (a.sum) x = a.sum + at, residual = nullptr;  // (it may lie over either; a lane reads what it wrote)
         r = 1.0 / sqrt(over_row<T>(s, sums) / n + a.eps);
+        if (last) tail = normed(tail, a.weight[end + lane], r);
     }
-    uint32_t top = 0;
+    uint32_t top = largest(tail, 0);
     for (int pass = 0; pass < 2; pass++) {
         const float inv = inverse_of(top);
-        for (int v = lane; v < groups; v += T) {
-            f32x4 h = load4(x, v, n);
-            if (residual) h += load4(residual, v, n);
-            if constexpr (NORM) h = normed(h, a.weight, v, n, r);
+#pragma unroll 4
+        for (int v = 4 * lane; v < end; v += 4 * T) {
+            f32x4 h = load4(x, v);
+            if (residual) h += load4(residual, v);
+            if constexpr (NORM) h = normed(h, load4(a.weight, v), r);
             if (pass == 0) top = largest(h, top);
-            else store_codes(a.codes + at, v, n, codes_of(h, inv));
+            else store4(codes, v, codes_of(h, inv));
         }
         if (pass == 0) top = over_row<T>(top, tops);
     }
+    if (last) codes[end + lane] = (int8_t)code_of(tail, inverse_of(top));
     if (lane == 0) a.scales[blockIdx.x] = scale_of(top);
 }
 
@@ -204,21 +203,18 @@ __global__ __launch_bounds__(256) void row8_read_kernel(const int8_t* __restrict
 #pragma unroll
     for (int i = 0; i < READ / 256; i++) {
         const int at = first + i * 256 + lane * 4;
-        c[i] = 0;
-        if (at + 3 < n) {
-            c[i] = *reinterpret_cast<const u32_any*>(from + at);
-        } else {
-            for (int e = 0; e < 3; e++)
-                if (at + e < n) c[i] |= (uint32_t)(uint8_t)from[at + e] << (8 * e);
-        }
+        c[i] = at + 3 < n ? *reinterpret_cast<const u32_any*>(from + at) : 0;
     }
 #pragma unroll
     for (int i = 0; i < READ / 256; i++) {
+        const int at = first + i * 256 + lane * 4;
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = q8_value(c[i], e) * scale;
-        store4(to, first / 4 + i * 64 + lane, n, v);
+        if (at + 3 < n) store4(to, at, v);
     }
+    const int at = (n & ~3) + lane;  // the last n % 4
+    if (at < n && at >= first && at < first + READ) to[at] = (float)from[at] * scale;
 }
 
 template <int T, int V>
@@ -233,31 +229,50 @@ void launch_rows(const Row8Norm& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_row8_norm(const Row8Norm& a, hipStream_t stream) {
-    const int n = a.n;
-    if (n <= 256) launch_rows<64, 1>(a, stream);
-    else if (n <= 512) launch_rows<64, 2>(a, stream);
-    else if (n <= 1024) launch_rows<64, 4>(a, stream);
-    else if (a.rows <= 256 && n <= 4096) launch_rows<1024, 1>(a, stream);
-    else if (a.rows <= 256 && n <= 8192) launch_rows<1024, 2>(a, stream);
-    else if (a.rows <= 256 && n <= 16384) launch_rows<1024, 4>(a, stream);
-    else if (n <= 2048) launch_rows<256, 2>(a, stream);
-    else if (n <= 4096) launch_rows<256, 4>(a, stream);
-    else if (n <= 8192) launch_rows<256, 8>(a, stream);
-    else if (n <= 16384) launch_rows<256, 16>(a, stream);
-    else if (n <= 32768) launch_rows<1024, 8>(a, stream);
-    else if (n <= 65536) launch_rows<1024, 16>(a, stream);
-    else if (a.weight) hipLaunchKernelGGL((row8_long_kernel<true>), dim3(a.rows), dim3(1024), 0, stream, a);
-    else hipLaunchKernelGGL((row8_long_kernel<false>), dim3(a.rows), dim3(1024), 0, stream, a);
-    return hipGetLastError();
+// A wave to a row up to 1024 entries, then a workgroup, four groups of four to a lane;
+// where the CUs have a row each at most, as many lanes as there are groups (one row of
+// 4096: 3.7 us, with 256 lanes 4.6).  Past the registers of 1024 lanes a row is read again.
+hipError_t launch_row8_norm(const Row8Norm& whole, hipStream_t stream) {
+    constexpr int SLICE = 1 << 21;  // rows of a launch at most (a grid's threads count in 32 bits)
+    for (int r0 = 0; r0 < whole.rows; r0 += std::min(SLICE, whole.rows - r0)) {
+        Row8Norm a = whole;
+        const size_t at = (size_t)r0 * whole.n;
+        const int n = a.n;
+        a.rows = std::min(SLICE, whole.rows - r0);
+        a.x += at, a.codes += at, a.scales += r0;
+        if (a.residual) a.residual += at;
+        if (a.sum) a.sum += at;
+        const bool few = a.rows <= device_cus();
+        if (n <= 256) launch_rows<64, 1>(a, stream);
+        else if (n <= 512) launch_rows<64, 2>(a, stream);
+        else if (n <= 1024) launch_rows<64, 4>(a, stream);
+        else if (few && n <= 4096) launch_rows<1024, 1>(a, stream);
+        else if (few && n <= 8192) launch_rows<1024, 2>(a, stream);
+        else if (n <= 2048) launch_rows<256, 2>(a, stream);
+        else if (n <= 4096) launch_rows<256, 4>(a, stream);
+        else if (n <= 8192) launch_rows<512, 4>(a, stream);
+        else if (n <= 16384) launch_rows<1024, 4>(a, stream);
+        else if (n <= 32768 && !a.weight) hipLaunchKernelGGL((row8_norm_kernel<1024, 8, false>), dim3(a.rows), dim3(1024), 0, stream, a);
+        else if (a.weight) hipLaunchKernelGGL((row8_long_kernel<true>), dim3(a.rows), dim3(1024), 0, stream, a);
+        else hipLaunchKernelGGL((row8_long_kernel<false>), dim3(a.rows), dim3(1024), 0, stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_row8_read(const int8_t* codes, const float* scales, float* x, int rows, int n, hipStream_t stream) {
     const int per_row = (n + READ - 1) / READ;
-    const int64_t parts = (int64_t)rows * per_row;
-    hipLaunchKernelGGL(row8_read_kernel, dim3((unsigned)((parts + 3) / 4)), dim3(256), 0, stream, codes, scales, x, parts,
-                       per_row, n);
-    return hipGetLastError();
+    const int slice = std::max(1, (1 << 25) / per_row);  // rows of a launch
+    for (int r0 = 0; r0 < rows; r0 += std::min(slice, rows - r0)) {
+        const int64_t parts = (int64_t)std::min(slice, rows - r0) * per_row;
+        const size_t at = (size_t)r0 * n;
+        hipLaunchKernelGGL(row8_read_kernel, dim3((unsigned)((parts + 3) / 4)), dim3(256), 0, stream, codes + at, scales + r0,
+                           x + at, parts, per_row, n);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace nitro

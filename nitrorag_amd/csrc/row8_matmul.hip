@@ -33,19 +33,6 @@ __device__ __forceinline__ float activate(float x, int activation) {
     }
 }
 
-// The output at batch row b, row i of member m, from its sums (second: the gated one's).
-__device__ __forceinline__ float finish(const Row8Matmul& a, int m, int b, int i, float sum, float second, float xs) {
-    float p = sum * xs;
-    if (a.bias) p += a.bias[i];
-    p = activate(p, a.activation);
-    if (a.gated) {
-        float q = second * xs;
-        if (a.bias) q += a.bias[a.d[0] + i];
-        p *= q;
-    }
-    return p;
-}
-
 // The member that column tile ct of `cols` columns each belongs to, and ct within it.
 __device__ __forceinline__ int member_of(const Row8Matmul& a, int& ct, int cols) {
     int m = 0;
@@ -58,101 +45,189 @@ __device__ __forceinline__ int member_of(const Row8Matmul& a, int& ct, int cols)
     return m;
 }
 
-// ---------------------------------------------------------------- few rows
-// A workgroup owns RT tiles of 16 batch rows x CT tiles of 16 weight rows; its waves
-// split the blocks, each keeping sums of its own, and add them through LDS in wave order.
-constexpr int FEW_WAVES = 8;
+// ---------------------------------------------------------- split over waves
+// A workgroup owns RT x CT tiles of U batch rows x U weight rows (U = 16 or 32, the matrix
+// instruction's); its W waves split the blocks, each with sums of its own, which are
+// added through LDS in wave order.  No wave waits for another before that.
+//  - weights: straight from memory in operand order, 512 bytes a load;
+//  - x: 128 bytes of a row at a time (eight lanes to a row) into a region of LDS of the
+//    wave's own, and back in operand order.  (Loaded in operand order, 16 rows to a load,
+//    every eight bytes were a lookup of their own in the vector cache: 128 rows of 4096 x
+//    4096 23 us, 14 us so; 16 rows of 4096 x 11008 17 us, 11 us so.)
+// Bound by the weights' bytes for few rows (8 rows of a gated 4096 x 11008 pair 20.5 us,
+// 4.9 TB/s, where loads alone take 18 us), by latency for small matrices (3.3 us at 768 x
+// 2048), and by the vector unit, at half its rate, towards 512 rows.
+template <int U>
+struct Tile;
+template <>
+struct Tile<16> {
+    typedef long Operand;
+    static constexpr int SUMS = 4, MASK = 15;
+    typedef f4 Sums;
+    // Row (x) or column (weights) lane % 16, k = 8 * (lane / 16) .. + 8.
+    static __device__ __forceinline__ Operand x(const int8_t* row, int lane) {
+        return *reinterpret_cast<const long*>(row + 8 * (lane >> 4));
+    }
+    static __device__ __forceinline__ Operand w(const uint8_t* record, int lane) {
+        return *reinterpret_cast<const long*>(record + 64 + 8 * lane);
+    }
+    static __device__ __forceinline__ void multiply(Operand x, Operand w, int (&p)[SUMS]) {
+        const i4 r = __builtin_amdgcn_mfma_i32_16x16x32_i8(x, w, i4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SUMS; i++) p[i] = r[i];
+    }
+    // Where the sum of (row, column) lies: its place among a lane's, and the lane.
+    static __device__ __forceinline__ int sum_at(int row) { return row % 4; }
+    static __device__ __forceinline__ int lane_at(int row, int col) { return row / 4 * 16 + col; }
+};
+template <>
+struct Tile<32> {
+    typedef i4 Operand;
+    static constexpr int SUMS = 16, MASK = 31;
+    typedef f16v Sums;
+    // Row or column lane % 32, k = 16 * (lane / 32) .. + 16.
+    static __device__ __forceinline__ Operand x(const int8_t* row, int lane) {
+        return *reinterpret_cast<const i4*>(row + 16 * (lane >> 5));
+    }
+    static __device__ __forceinline__ Operand w(const uint8_t* record, int lane) {
+        const uint8_t* p = record + 64 + 256 * (lane >> 5) + 8 * (lane & 15);
+        const int2 lo = *reinterpret_cast<const int2*>(p), hi = *reinterpret_cast<const int2*>(p + 128);
+        return i4{lo.x, lo.y, hi.x, hi.y};
+    }
+    static __device__ __forceinline__ void multiply(Operand x, Operand w, int (&p)[SUMS]) {
+        i16 zero;
+#pragma unroll
+        for (int i = 0; i < 16; i++) zero[i] = 0;
+        const i16 r = __builtin_amdgcn_mfma_i32_32x32x32_i8(x, w, zero, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SUMS; i++) p[i] = r[i];
+    }
+    static __device__ __forceinline__ int sum_at(int row) { return row / 8 * 4 + row % 4; }
+    static __device__ __forceinline__ int lane_at(int row, int col) { return row / 4 % 2 * 32 + col; }
+};
 
-template <int RT, int CT, bool GATED>
-__global__ __launch_bounds__(64 * FEW_WAVES) void row8_few_kernel(Row8Matmul a) {
-    extern __shared__ float parts[];  // [wave][RT * CT][64][4]
-    constexpr int COLS = 16 * CT / (GATED ? 2 : 1);  // outputs
+template <int U, int RT, int CT, int W, int OCC, bool GATED>
+__global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a) {
+    typedef Tile<U> T;
+    constexpr int ROWS = U * RT, COLS = U * CT / (GATED ? 2 : 1);  // of the output
+    constexpr int ROUND = 4, PITCH = ROUND * Q8_BLOCK + 16;  // blocks a round; bytes of a row in LDS
+    constexpr int LOADS = ROWS / 8;                          // of 8 rows of x
+    constexpr int PART = RT * CT * T::SUMS * 64, XBYTES = W * ROWS * PITCH, SBYTES = W * PART * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[XBYTES > SBYTES ? XBYTES : SBYTES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lr = lane & 15, lg = lane >> 4;
     int ct = blockIdx.x;
     const int member = member_of(a, ct, COLS);
     const int d = a.d[member], n = a.n, nb = n / Q8_BLOCK, tiles = (d + 15) / 16;
-    const int b0 = blockIdx.y * 16 * RT;
+    const int b0 = blockIdx.y * ROWS;
 
+    // Weight tiles of 16 rows, the last one for those past the end; with a gate, tile 2t is
+    // the gate's and 2t + 1 the other matrix's.
     const uint8_t* w[CT];
 #pragma unroll
     for (int t = 0; t < CT; t++) {
-        const int tile = min(ct * (COLS / 16) + (GATED ? t / 2 : t), tiles - 1);
+        const int tile = min((ct * COLS + U * (GATED ? t / 2 : t) + (lane & T::MASK)) / 16, tiles - 1);
         w[t] = a.w[GATED ? t % 2 : member] + (size_t)tile * nb * Q8_TILE_BYTES;
     }
-    const int8_t* x[RT];
+    const int8_t* x[LOADS];
+    const int xk = lane % 8 * 16;
 #pragma unroll
-    for (int r = 0; r < RT; r++) x[r] = a.codes + (size_t)min(b0 + 16 * r + lr, a.rows - 1) * n + 8 * lg;
+    for (int r = 0; r < LOADS; r++) x[r] = a.codes + (size_t)min(b0 + 8 * r + lane / 8, a.rows - 1) * n;
+    int8_t* const mine = reinterpret_cast<int8_t*>(lds) + wave * ROWS * PITCH;
 
-    f4 acc[RT][CT];
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = 0; t < CT; t++) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
-
-    // Blocks first .. end, U to a round, the next round's loads ahead of this one's use.
-    // A block past the end repeats the last one, times 0.
-    constexpr int U = CT * (1 + RT) <= 4 ? 4 : 2;
-    const int first = (int)((int64_t)nb * wave / FEW_WAVES), end = (int)((int64_t)nb * (wave + 1) / FEW_WAVES);
-    struct Round {
-        long wq[U][CT];
-        float ws[U][CT];
-        long xq[U][RT];
-    } ra, rb;
-    auto load = [&](Round& R, int blk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = min(blk + u, nb - 1);
-#pragma unroll
-            for (int t = 0; t < CT; t++) {
-                const uint8_t* p = w[t] + (size_t)k * Q8_TILE_BYTES;
-                R.wq[u][t] = *reinterpret_cast<const long*>(p + 64 + 8 * lane);
-                R.ws[u][t] = *reinterpret_cast<const float*>(p + 4 * lr);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; r++) R.xq[u][r] = *reinterpret_cast<const long*>(x[r] + (size_t)k * Q8_BLOCK);
-        }
-    };
-    auto use = [&](const Round& R, int blk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int t = 0; t < CT; t++) {
-                const float s = blk + u < end ? R.ws[u][t] : 0.0f;
-#pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    const i4 p = __builtin_amdgcn_mfma_i32_16x16x32_i8(R.xq[u][r], R.wq[u][t], i4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[r][t][i] = fmaf(s, (float)p[i], acc[r][t][i]);
-                }
-            }
-    };
-    load(ra, first);
-    for (int blk = first; blk < end; blk += 2 * U) {
-        load(rb, blk + U);
-        use(ra, blk);
-        load(ra, blk + 2 * U);
-        use(rb, blk + U);
-    }
+    typename T::Sums acc[RT][CT];
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int t = 0; t < CT; t++)
-            *reinterpret_cast<f4*>(&parts[((wave * RT * CT + r * CT + t) * 64 + lane) * 4]) = acc[r][t];
+#pragma unroll
+            for (int i = 0; i < T::SUMS; i++) acc[r][t][i] = 0.0f;
+
+    // Rounds first .. end, the next round's loads ahead of this one's use.  A block past
+    // the end repeats the last one, times 0.
+    const int rounds = (nb + ROUND - 1) / ROUND;
+    const int first = (int)((int64_t)rounds * wave / W), end = (int)((int64_t)rounds * (wave + 1) / W);
+    struct Weights {
+        typename T::Operand q[ROUND][CT];
+        float s[ROUND][CT];
+    } wa, wb;
+    i4 xn[LOADS];
+    auto load = [&](Weights& R, int round) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < LOADS; r++)
+            xn[r] = *reinterpret_cast<const i4*>(x[r] + min(round * (ROUND * Q8_BLOCK) + xk, n - 16));
+#pragma unroll
+        for (int u = 0; u < ROUND; u++) {
+            const int k = min(round * ROUND + u, nb - 1);
+#pragma unroll
+            for (int t = 0; t < CT; t++) {
+                const uint8_t* record = w[t] + (size_t)k * Q8_TILE_BYTES;
+                R.q[u][t] = T::w(record, lane);
+                R.s[u][t] = *reinterpret_cast<const float*>(record + 4 * (lane & 15));
+            }
+        }
+    };
+    // Lanes read what other lanes of the wave wrote, and write where others read: no
+    // access may pass another between them.
+    auto exchange = []() __attribute__((always_inline)) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto use = [&](const Weights& R, Weights& next, int round) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < LOADS; r++) *reinterpret_cast<i4*>(mine + (8 * r + lane / 8) * PITCH + xk) = xn[r];
+        exchange();
+        load(next, round + 1);
+#pragma unroll
+        for (int u = 0; u < ROUND; u++) {
+            typename T::Operand xq[RT];
+#pragma unroll
+            for (int r = 0; r < RT; r++) xq[r] = T::x(mine + (U * r + (lane & T::MASK)) * PITCH + u * Q8_BLOCK, lane);
+#pragma unroll
+            for (int t = 0; t < CT; t++) {
+                const float s = round * ROUND + u < nb ? R.s[u][t] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    int p[T::SUMS];
+                    T::multiply(xq[r], R.q[u][t], p);
+#pragma unroll
+                    for (int i = 0; i < T::SUMS; i++) acc[r][t][i] = fmaf(s, (float)p[i], acc[r][t][i]);
+                }
+            }
+        }
+        exchange();
+    };
+    if (first < end) {
+        load(wa, first);
+#pragma unroll 1
+        for (int round = first; round < end; round += 2) {
+            use(wa, wb, round);
+            if (round + 1 < end) use(wb, wa, round + 1);
+        }
+    }
+    float* const parts = reinterpret_cast<float*>(lds);  // [wave][tile][sum][lane]
     __syncthreads();
-    // Lane l has rows 4 * (l / 16) + i, column l % 16 of a tile.
-    for (int e = threadIdx.x; e < 16 * RT * COLS; e += 64 * FEW_WAVES) {
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int t = 0; t < CT; t++)
+#pragma unroll
+            for (int i = 0; i < T::SUMS; i++) parts[wave * PART + ((r * CT + t) * T::SUMS + i) * 64 + lane] = acc[r][t][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < ROWS * COLS; e += 64 * W) {
         const int row = e / COLS, col = e % COLS;
-        const int at = (row / 16 * CT + (GATED ? col / 16 * 2 : col / 16)) * 256 + (row % 16 / 4 * 16 + col % 16) * 4 + row % 4;
+        const int tile = row / U * CT + (GATED ? col / U * 2 : col / U);
+        const int at = (tile * T::SUMS + T::sum_at(row % U)) * 64 + T::lane_at(row % U, col % U);
         float s = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int v = 0; v < FEW_WAVES; v++) {
-            s += parts[v * RT * CT * 256 + at];
-            if constexpr (GATED) s2 += parts[v * RT * CT * 256 + at + 256];
+        for (int v = 0; v < W; v++) {
+            s += parts[v * PART + at];
+            if constexpr (GATED) s2 += parts[v * PART + at + T::SUMS * 64];
         }
         const int b = b0 + row, i = ct * COLS + col;
         if (b < a.rows && i < d) {
-            float y = finish(a, member, b, i, s, s2, a.scales[b]);
+            const float xs = a.scales[b];
+            float y = activate(s * xs + (a.bias ? a.bias[i] : 0.0f), a.activation);
+            if constexpr (GATED) y *= s2 * xs + (a.bias ? a.bias[d + i] : 0.0f);
             const size_t o = (size_t)b * d + i;
             if (a.residual) y += a.residual[o];
             a.out[member][o] = y;
@@ -166,15 +241,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void row8_few_kernel(Row8Matmul a) 
 // row l % 32).  Two blocks of x and of the weights lie in LDS, two buffers, a barrier for
 // each two.  x lies as four planes (a block's halves) of 16 bytes a row, so that lanes read
 // consecutive rows; the weights as in the tile layout, runs of 8 k.
-template <int MT, int NT, bool GATED>
-__global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col_tiles) {
+template <int MT, int NT, int DEPTH, int OCC, bool GATED>
+__global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, int col_tiles) {
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
     constexpr int PLANE = BM * 16 + 32;  // (the planes' banks lie 32 bytes apart: a row's four runs are written together)
-    __shared__ __attribute__((aligned(16))) uint8_t xl[2][4 * PLANE];
-    __shared__ __attribute__((aligned(16))) uint8_t wl[2][2 * BN * 32];
-    __shared__ float sl[2][2 * BN];
+    constexpr int XB = 4 * PLANE, WB = 2 * BN * 32, BUF = XB + WB + 2 * BN * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF < 16384 ? 16384 : 2 * BUF];
+    const int tid = threadIdx.x;
+    auto xl = [&](int buf) __attribute__((always_inline)) { return lds + buf * BUF; };
+    auto wl = [&](int buf) __attribute__((always_inline)) { return lds + buf * BUF + XB; };
+    auto sl = [&](int buf) __attribute__((always_inline)) { return reinterpret_cast<float*>(lds + buf * BUF + XB + WB); };
     static_assert(!GATED || NT == 2, "a wave's two column tiles are the gate's and the other's");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = tid & 63, wave = tid >> 6;
     const int wm = wave & 1, wn = wave >> 1, lc = lane & 31, lh = lane >> 5;
 
     // Column tiles fastest, XCD i taking the i-th eighth of the work.
@@ -196,22 +274,22 @@ __global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col
     // Staging: x as MT units of 16 bytes a thread, weights NT, one scale (of 2 BN).
     const int8_t* xp[MT];
     int xk, xdst[MT];
-    xk = threadIdx.x % 4 * 16;
+    xk = tid % 4 * 16;
 #pragma unroll
     for (int u = 0; u < MT; u++) {
-        const int row = threadIdx.x / 4 + 64 * u;
+        const int row = tid / 4 + 64 * u;
         xp[u] = a.codes + (size_t)min(b0 + row, a.rows - 1) * n;
-        xdst[u] = threadIdx.x % 4 * PLANE + row * 16;
+        xdst[u] = tid % 4 * PLANE + row * 16;
     }
     const uint8_t* wp[NT];
     int wblk[NT];
 #pragma unroll
     for (int u = 0; u < NT; u++) {
-        const int e = threadIdx.x + 256 * u;
+        const int e = tid + 256 * u;
         wblk[u] = e / (2 * BN);
         wp[u] = tile_at(e / 32 % (BN / 16)) + 64 + e % 32 * 16;
     }
-    const int sblk = threadIdx.x / BN, srow = threadIdx.x % BN;
+    const int sblk = tid / BN, srow = tid % BN;
     const uint8_t* sp = tile_at(srow / 16) + 4 * (srow % 16);
 
     struct Stage {
@@ -225,16 +303,16 @@ __global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col
 #pragma unroll
         for (int u = 0; u < NT; u++)
             S.w[u] = *reinterpret_cast<const i4*>(wp[u] + (size_t)min(blk + wblk[u], nb - 1) * Q8_TILE_BYTES);
-        if (2 * BN == 256 || threadIdx.x < 2 * BN)
+        if (2 * BN == 256 || tid < 2 * BN)
             S.s = *reinterpret_cast<const float*>(sp + (size_t)min(blk + sblk, nb - 1) * Q8_TILE_BYTES);
     };
     auto put = [&](const Stage& S, int buf, int blk) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < MT; u++) *reinterpret_cast<i4*>(&xl[buf][xdst[u]]) = S.x[u];
+        for (int u = 0; u < MT; u++) *reinterpret_cast<i4*>(xl(buf) + xdst[u]) = S.x[u];
 #pragma unroll
-        for (int u = 0; u < NT; u++) *reinterpret_cast<i4*>(&wl[buf][(threadIdx.x + 256 * u) * 16]) = S.w[u];
+        for (int u = 0; u < NT; u++) *reinterpret_cast<i4*>(wl(buf) + (tid + 256 * u) * 16) = S.w[u];
         // (a block past the end repeats the last one, times 0)
-        if (2 * BN == 256 || threadIdx.x < 2 * BN) sl[buf][threadIdx.x] = blk + sblk < nb ? S.s : 0.0f;
+        if (2 * BN == 256 || tid < 2 * BN) sl(buf)[tid] = blk + sblk < nb ? S.s : 0.0f;
     };
 
     f16v acc[MT][NT];
@@ -245,6 +323,15 @@ __global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[m][t][i] = 0.0f;
 
+    // The products of one 32 x 32 tile and block, scaled in while the next tile's run.
+    i16 late;
+    float late_s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) late[i] = 0;
+    auto scale_in = [&](f16v& to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) to[i] = fmaf(late_s, (float)late[i], to[i]);
+    };
     auto compute = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -253,14 +340,14 @@ __global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const int j = wn * 2 * NT + 2 * t + lc / 16;
-                const uint8_t* p = &wl[buf][(h * (BN / 16) + j) * 512 + (2 * lh * 16 + lc % 16) * 8];
+                const uint8_t* p = wl(buf) + (h * (BN / 16) + j) * 512 + (2 * lh * 16 + lc % 16) * 8;
                 const int2 lo = *reinterpret_cast<const int2*>(p), hi = *reinterpret_cast<const int2*>(p + 128);
                 w[t] = i4{lo.x, lo.y, hi.x, hi.y};
-                s[t] = sl[buf][h * BN + wn * 32 * NT + 32 * t + lc];
+                s[t] = sl(buf)[h * BN + wn * 32 * NT + 32 * t + lc];
             }
 #pragma unroll
             for (int m = 0; m < MT; m++)
-                x[m] = *reinterpret_cast<const i4*>(&xl[buf][(2 * h + lh) * PLANE + (wm * 32 * MT + 32 * m + lc) * 16]);
+                x[m] = *reinterpret_cast<const i4*>(xl(buf) + (2 * h + lh) * PLANE + (wm * 32 * MT + 32 * m + lc) * 16);
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -269,28 +356,41 @@ __global__ __launch_bounds__(256, 2) void row8_gemm_kernel(Row8Matmul a, int col
 #pragma unroll
                     for (int i = 0; i < 16; i++) zero[i] = 0;
                     const i16 p = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[m], w[t], zero, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) acc[m][t][i] = fmaf(s[t], (float)p[i], acc[m][t][i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    scale_in(m ? acc[m - 1][t] : t ? acc[MT - 1][t - 1] : acc[MT - 1][NT - 1]);
+                    late = p, late_s = s[t];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
         }
     };
     const int steps = (nb + 1) / 2;
-    Stage st;
-    load(st, 0);
-    put(st, 0, 0);
-    load(st, 2);
-#pragma unroll 1
-    for (int i = 0; i < steps; i++) {
+    auto step = [&](int i, Stage& S) __attribute__((always_inline)) {
         __syncthreads();  // step i is staged; the other buffer's readers are done
-        put(st, (i + 1) & 1, 2 * i + 2);
-        load(st, 2 * i + 4);
+        put(S, (i + 1) & 1, 2 * i + 2);
+        load(S, 2 * (i + 1 + DEPTH));
         compute(i & 1);
+    };
+    Stage sa, sb;
+    load(sa, 0);
+    if constexpr (DEPTH == 2) load(sb, 2);
+    put(sa, 0, 0);
+    load(sa, 2 * DEPTH);
+    if constexpr (DEPTH == 1) {
+#pragma unroll 1
+        for (int i = 0; i < steps; i++) step(i, sa);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i + 1 < steps; i += 2) {
+            step(i, sb);
+            step(i + 1, sa);
+        }
+        if (steps & 1) step(steps - 1, sb);
     }
+    scale_in(acc[MT - 1][NT - 1]);
 
     // Lane l holds row 8 * (i / 4) + 4 * (l / 32) + i % 4, column l % 32 of a tile.
     __syncthreads();
-    float* const mine = reinterpret_cast<float*>(&xl[0][0]) + wave * 1024 + lane;
-    static_assert(sizeof(xl) >= 4 * 1024 * sizeof(float), "a tile for each wave");
+    float* const mine = reinterpret_cast<float*>(lds) + wave * 1024 + lane;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int row0 = b0 + (wm * MT + m) * 32 + 4 * lh;
@@ -342,47 +442,118 @@ int col_tiles_of(const Row8Matmul& a, int cols) {
     return t;
 }
 
-template <int RT, int CT>
-void launch_few(const Row8Matmul& a, hipStream_t stream) {
-    const int cols = 16 * CT / (a.gated ? 2 : 1);
-    const dim3 grid((unsigned)col_tiles_of(a, cols), (unsigned)((a.rows + 16 * RT - 1) / (16 * RT)));
-    constexpr size_t lds = sizeof(float) * FEW_WAVES * RT * CT * 256;
-    if constexpr (CT % 2 == 0) {
-        if (a.gated) {
-            hipLaunchKernelGGL((row8_few_kernel<RT, CT, true>), grid, dim3(64 * FEW_WAVES), lds, stream, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((row8_few_kernel<RT, CT, false>), grid, dim3(64 * FEW_WAVES), lds, stream, a);
+// A kernel, its workgroup's tile, and what its time is estimated with: a wave's chain of
+// steps (`blocks` blocks each, the blocks split over `split` waves), of which one takes
+// `alone` us where few workgroups share a CU and `busy` us times their number where many
+// do, at most `resident` at once; `fixed` us for a launch, a third of it again for every
+// set of resident workgroups.
+struct Form {
+    int rows, cols, blocks, split, resident;
+    float fixed, alone, busy;
+    bool gates;  // its column tiles are even in number
+    bool tall;   // batch rows in the grid's first dimension
+    int threads;
+    void (*launch)(const Row8Matmul&, dim3, int, hipStream_t);
+};
+
+template <int U, int RT, int CT, int W, int OCC>
+constexpr Form split_form(int resident, float fixed, float alone, float busy) {
+    return {U * RT, U * CT, 4, W, resident, fixed, alone, busy, CT % 2 == 0, false, 64 * W,
+            [](const Row8Matmul& a, dim3 grid, int, hipStream_t stream) {
+                if constexpr (CT % 2 == 0) {
+                    if (a.gated) {
+                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, true>), grid, dim3(64 * W), 0, stream, a);
+                        return;
+                    }
+                }
+                hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, dim3(64 * W), 0, stream, a);
+            }};
 }
 
-template <int MT, int NT>
-void launch_gemm(const Row8Matmul& a, hipStream_t stream) {
-    const int cols = 64 * NT / (a.gated ? 2 : 1);
-    const int ct = col_tiles_of(a, cols);
-    const dim3 grid((unsigned)ct * (unsigned)((a.rows + 64 * MT - 1) / (64 * MT)));
-    if constexpr (NT == 2) {
-        if (a.gated) {
-            hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, true>), grid, dim3(256), 0, stream, a, ct);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, false>), grid, dim3(256), 0, stream, a, ct);
+template <int MT, int NT, int DEPTH, int OCC>
+constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
+    return {64 * MT, 64 * NT, 2, 1, resident, fixed, alone, busy, NT == 2, true, 256,
+            [](const Row8Matmul& a, dim3 grid, int col_tiles, hipStream_t stream) {
+                if constexpr (NT == 2) {
+                    if (a.gated) {
+                        hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, true>), grid, dim3(256), 0, stream, a, col_tiles);
+                        return;
+                    }
+                }
+                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, false>), grid, dim3(256), 0, stream, a, col_tiles);
+            }};
 }
+
+// Each timed over some 300 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384,
+// gated or not) as graph replays, and fitted to within 5 to 9% of its own times.  The
+// choice by these estimates takes 1.3% longer in the mean than the best of the forms each
+// time (at most 29%).
+constexpr Form FORMS[] = {
+    split_form<16, 1, 1, 4, 5>(9, 2.14f, 0.329f, 0.309f),
+    split_form<16, 1, 1, 8, 4>(3, 2.10f, 0.129f, 0.588f),
+    split_form<16, 1, 2, 4, 4>(5, 2.26f, 0.677f, 0.521f),
+    split_form<16, 1, 2, 8, 4>(3, 2.12f, 0.175f, 1.084f),
+    split_form<16, 2, 2, 8, 4>(2, 2.24f, 1.402f, 1.420f),
+    split_form<32, 1, 1, 4, 4>(4, 2.77f, 0.574f, 0.554f),
+    split_form<32, 2, 2, 4, 2>(1, 4.84f, 0.048f, 1.582f),
+    gemm_form<1, 1, 2, 4>(4, 2.91f, 0.418f, 0.196f),
+    gemm_form<1, 2, 2, 3>(2, 3.64f, 0.516f, 0.365f),
+    gemm_form<2, 2, 1, 3>(2, 5.60f, 0.805f, 0.569f),
+    gemm_form<4, 2, 1, 2>(2, 11.60f, 1.374f, 0.981f),
+};
+
+struct Grid {
+    int64_t x, y;
+    int col_tiles;
+};
+// (a grid's threads in x count in 32 bits, its workgroups in y in 16)
+bool grid_of(const Form& f, const Row8Matmul& a, Grid& g) {
+    g.col_tiles = col_tiles_of(a, a.gated ? f.cols / 2 : f.cols);
+    const int64_t row_tiles = ((int64_t)a.rows + f.rows - 1) / f.rows;
+    g.x = f.tall ? g.col_tiles * row_tiles : g.col_tiles, g.y = f.tall ? 1 : row_tiles;
+    return (f.gates || !a.gated) && g.y < 65536 && g.x * f.threads < (1ll << 32);
+}
+
+float estimate(const Form& f, const Row8Matmul& a, const Grid& g, int cus) {
+    const int64_t groups = (g.x * g.y + cus - 1) / cus;  // of the busiest CU
+    const int blocks = a.n / Q8_BLOCK, steps = (blocks + f.blocks - 1) / f.blocks;
+    const float chain = (float)((steps + f.split - 1) / f.split);
+    const float set = 0.3f * f.fixed;
+    const int64_t full = groups / f.resident, rest = groups % f.resident;
+    float t = f.fixed + full * (set + chain * std::max(f.alone, f.resident * f.busy));
+    if (rest) t += set + chain * std::max(f.alone, rest * f.busy);
+    return t;
+}
+
+// Rows of one launch at most.
+constexpr int SLICE = 1 << 20;
 
 }  // namespace
 
-hipError_t launch_row8_matmul(const Row8Matmul& a, hipStream_t stream) {
-    if (a.rows <= 16) {
-        a.gated ? launch_few<1, 2>(a, stream) : launch_few<1, 1>(a, stream);
-    } else if (a.rows <= 64) {
-        launch_few<2, 2>(a, stream);
-    } else if ((int64_t)a.rows * col_tiles_of(a, 1) < (int64_t)4 << 20) {
-        launch_gemm<2, 2>(a, stream);
-    } else {
-        launch_gemm<4, 2>(a, stream);
+hipError_t launch_row8_matmul(const Row8Matmul& whole, hipStream_t stream) {
+    const int cus = device_cus();
+    for (int r0 = 0; r0 < whole.rows; r0 += std::min(SLICE, whole.rows - r0)) {
+        Row8Matmul a = whole;
+        a.rows = std::min(SLICE, whole.rows - r0);
+        a.codes += (size_t)r0 * a.n;
+        a.scales += r0;
+        if (a.residual) a.residual += (size_t)r0 * a.d[0];
+        for (int m = 0; m < a.mats; m++) a.out[m] += (size_t)r0 * a.d[m];
+        const Form* best = nullptr;
+        Grid grid{};
+        float least = 0.0f;
+        for (const Form& f : FORMS) {
+            Grid g;
+            if (!grid_of(f, a, g)) continue;
+            const float t = estimate(f, a, g, cus);
+            if (!best || t < least) best = &f, least = t, grid = g;
+        }
+        if (!best) return hipErrorInvalidConfiguration;
+        best->launch(a, dim3((unsigned)grid.x, (unsigned)grid.y), grid.col_tiles, stream);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace nitro

@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _native as N
-from .attention import _dev, _stream_ptr
+from .attention import _dev, _stream_ptr, _torch_module
 from .q8 import BLOCK, BLOCK_BYTES
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -20,62 +20,61 @@ def _refuse(func: str, message: str):
     raise N.NitroError(N.INVALID_ARGUMENT, func, message)
 
 
-def _rows(func: str, codes, scales):
-    """(rows, n) of rows held in 8 bits."""
-    import torch
+def _here(func: str, t, dev: int):
+    if t.get_device() != dev:
+        _refuse(func, f"every tensor must be on the current device, cuda:{dev}")
 
+
+def _rows(func: str, codes, scales):
+    """(rows, n, current device) of rows held in 8 bits."""
+    torch = _torch_module()
+    dev = torch._C._cuda_getDevice()
     for t, dtype, name in ((codes, torch.int8, "codes"), (scales, torch.float32, "scales")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TypeError(f"{name} must be a GPU tensor")
         if t.dtype is not dtype or not t.is_contiguous():
             raise TypeError(f"{name} must be contiguous {str(dtype)[6:]}")
-    if codes.dim() != 2 or tuple(scales.shape) != (codes.shape[0],):
+        _here(func, t, dev)
+    if codes.dim() != 2 or scales.shape != codes.shape[:1]:
         _refuse(func, "codes must be [rows][n] and scales [rows]")
-    _here(func, codes, scales)
-    return codes.shape
+    rows, n = codes.shape
+    return rows, n, dev
 
 
-def _here(func: str, *tensors):
-    import torch
-
-    dev = torch.cuda.current_device()
-    if any(t is not None and t.get_device() != dev for t in tensors):
-        _refuse(func, f"every tensor must be on the current device, cuda:{dev}")
-
-
-def _f32(func: str, t, shape, name: str):
+def _f32(func: str, t, shape, name: str, dev: int):
     if t is None:
         return None
     p = _dev(t, name)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         _refuse(func, f"{name} must be {'x'.join(map(str, shape))}")
-    _here(func, t)
+    _here(func, t, dev)
     return p
 
 
 def rms_norm_row8(x, weight, codes, scales, residual=None, sum=None, eps: float = 1e-5, stream=None) -> None:
     """codes, scales = rms_norm(x + residual) * weight, held; sum receives x + residual
     (it may be x or residual)."""
-    rows, n = _rows("rms_norm_row8", codes, scales)
     f = "rms_norm_row8"
+    rows, n, dev = _rows(f, codes, scales)
+    shape = (rows, n)
     if x is None or weight is None:
         _refuse(f, "x and weight are required")
-    N.call("nitro_rms_norm_row8", _f32(f, x, (rows, n), "x"), _f32(f, residual, (rows, n), "residual"),
-           _f32(f, weight, (n,), "weight"), eps, _f32(f, sum, (rows, n), "sum"), codes.data_ptr(), scales.data_ptr(),
+    N.call("nitro_rms_norm_row8", _f32(f, x, shape, "x", dev), _f32(f, residual, shape, "residual", dev),
+           _f32(f, weight, (n,), "weight", dev), eps, _f32(f, sum, shape, "sum", dev), codes.data_ptr(), scales.data_ptr(),
            rows, n, _stream_ptr(stream))
 
 
 def row8_quantize(x, codes, scales, stream=None) -> None:
     """codes, scales = the rows of x, held."""
-    rows, n = _rows("row8_quantize", codes, scales)
-    N.call("nitro_row8_quantize", _f32("row8_quantize", x, (rows, n), "x"), codes.data_ptr(), scales.data_ptr(), rows, n,
+    rows, n, dev = _rows("row8_quantize", codes, scales)
+    N.call("nitro_row8_quantize", _f32("row8_quantize", x, (rows, n), "x", dev), codes.data_ptr(), scales.data_ptr(), rows, n,
            _stream_ptr(stream))
 
 
 def row8_read(codes, scales, x, stream=None) -> None:
     """x = the values that the rows hold."""
-    rows, n = _rows("row8_read", codes, scales)
-    N.call("nitro_row8_read", codes.data_ptr(), scales.data_ptr(), _f32("row8_read", x, (rows, n), "x"), rows, n,
+    rows, n, dev = _rows("row8_read", codes, scales)
+    N.call("nitro_row8_read", codes.data_ptr(), scales.data_ptr(), _f32("row8_read", x, (rows, n), "x", dev), rows, n,
            _stream_ptr(stream))
 
 
@@ -98,7 +97,7 @@ class Q8Weights:
                 _refuse("Q8Weights", f"weights must be rows of whole {BLOCK_BYTES}-byte blocks")
             if t.shape[0] != w.shape[0] or t.numel() != w.numel():
                 _refuse("Q8Weights", "the two matrices must have one shape")
-            _here("Q8Weights", t)
+            _here("Q8Weights", t, torch.cuda.current_device())
         self.d = w.shape[0]
         self.n = w.numel() // self.d // BLOCK_BYTES * BLOCK
         self.gated = up is not None
@@ -111,7 +110,7 @@ class Q8Weights:
         """out[rows][d] = act(rows . w^T + bias) + residual; of a pair act(rows . gate^T +
         bias[:d]) * (rows . up^T + bias[d:]) + residual.  residual may be out."""
         f = "Q8Weights.matmul"
-        rows, n = _rows(f, codes, scales)
+        rows, n, dev = _rows(f, codes, scales)
         if n != self.n:
             _refuse(f, f"the rows have {n} entries, the weights {self.n}")
         if activation not in ACTIVATIONS:
@@ -120,8 +119,8 @@ class Q8Weights:
             _refuse(f, "out is required")
         shape = (rows, self.d)
         N.call("nitro_row8_matmul", self._h, codes.data_ptr(), scales.data_ptr(),
-               _f32(f, bias, (self.d * (1 + self.gated),), "bias"), _f32(f, residual, shape, "residual"),
-               _f32(f, out, shape, "out"), rows, ACTIVATIONS[activation], _stream_ptr(stream))
+               _f32(f, bias, (self.d * (1 + self.gated),), "bias", dev), _f32(f, residual, shape, "residual", dev),
+               _f32(f, out, shape, "out", dev), rows, ACTIVATIONS[activation], _stream_ptr(stream))
 
     def close(self):
         if getattr(self, "_h", None):
