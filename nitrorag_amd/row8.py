@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _native as N
-from .attention import _dev, _stream_ptr, _torch_module
+from .attention import _torch_module
 from .q8 import BLOCK, BLOCK_BYTES
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -20,62 +20,61 @@ def _refuse(func: str, message: str):
     raise N.NitroError(N.INVALID_ARGUMENT, func, message)
 
 
-def _here(func: str, t, dev: int):
-    if t.get_device() != dev:
-        _refuse(func, f"every tensor must be on the current device, cuda:{dev}")
+def _ptr(func: str, t, dtype, shape, name: str, dev: int):
+    """The address of a contiguous tensor of that type and shape on the current device."""
+    try:
+        if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.shape == shape:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    if not isinstance(t, _torch_module().Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a GPU tensor")
+    if t.dtype is not dtype or not t.is_contiguous():
+        raise TypeError(f"{name} must be contiguous {str(dtype)[6:]}")
+    if t.shape != shape:
+        _refuse(func, f"{name} must be [{']['.join(map(str, shape))}]")
+    _refuse(func, f"{name} must be on the current device, cuda:{dev}")
 
 
-def _rows(func: str, codes, scales):
-    """(rows, n, current device) of rows held in 8 bits."""
+def _rows(func: str, codes, scales, stream):
+    """Of rows held in 8 bits: rows, n, the addresses of codes and scales; the current
+    device, the stream's address, and torch.float32."""
     torch = _torch_module()
     dev = torch._C._cuda_getDevice()
-    for t, dtype, name in ((codes, torch.int8, "codes"), (scales, torch.float32, "scales")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{name} must be a GPU tensor")
-        if t.dtype is not dtype or not t.is_contiguous():
-            raise TypeError(f"{name} must be contiguous {str(dtype)[6:]}")
-        _here(func, t, dev)
-    if codes.dim() != 2 or scales.shape != codes.shape[:1]:
-        _refuse(func, "codes must be [rows][n] and scales [rows]")
-    rows, n = codes.shape
-    return rows, n, dev
-
-
-def _f32(func: str, t, shape, name: str, dev: int):
-    if t is None:
-        return None
-    p = _dev(t, name)
-    if t.shape != shape:
-        _refuse(func, f"{name} must be {'x'.join(map(str, shape))}")
-    _here(func, t, dev)
-    return p
+    f32 = torch.float32
+    shape = getattr(codes, "shape", (0, 0))
+    if len(shape) != 2:
+        _refuse(func, "codes must be [rows][n]")
+    rows, n = shape
+    pc = _ptr(func, codes, torch.int8, shape, "codes", dev)
+    ps = _ptr(func, scales, f32, (rows,), "scales", dev)
+    return rows, n, pc, ps, dev, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, f32
 
 
 def rms_norm_row8(x, weight, codes, scales, residual=None, sum=None, eps: float = 1e-5, stream=None) -> None:
     """codes, scales = rms_norm(x + residual) * weight, held; sum receives x + residual
     (it may be x or residual)."""
     f = "rms_norm_row8"
-    rows, n, dev = _rows(f, codes, scales)
+    rows, n, pc, ps, dev, s, f32 = _rows(f, codes, scales, stream)
     shape = (rows, n)
-    if x is None or weight is None:
-        _refuse(f, "x and weight are required")
-    N.call("nitro_rms_norm_row8", _f32(f, x, shape, "x", dev), _f32(f, residual, shape, "residual", dev),
-           _f32(f, weight, (n,), "weight", dev), eps, _f32(f, sum, shape, "sum", dev), codes.data_ptr(), scales.data_ptr(),
-           rows, n, _stream_ptr(stream))
+    N.call("nitro_rms_norm_row8", _ptr(f, x, f32, shape, "x", dev),
+           None if residual is None else _ptr(f, residual, f32, shape, "residual", dev),
+           _ptr(f, weight, f32, (n,), "weight", dev), eps,
+           None if sum is None else _ptr(f, sum, f32, shape, "sum", dev), pc, ps, rows, n, s)
 
 
 def row8_quantize(x, codes, scales, stream=None) -> None:
     """codes, scales = the rows of x, held."""
-    rows, n, dev = _rows("row8_quantize", codes, scales)
-    N.call("nitro_row8_quantize", _f32("row8_quantize", x, (rows, n), "x", dev), codes.data_ptr(), scales.data_ptr(), rows, n,
-           _stream_ptr(stream))
+    f = "row8_quantize"
+    rows, n, pc, ps, dev, s, f32 = _rows(f, codes, scales, stream)
+    N.call("nitro_row8_quantize", _ptr(f, x, f32, (rows, n), "x", dev), pc, ps, rows, n, s)
 
 
 def row8_read(codes, scales, x, stream=None) -> None:
     """x = the values that the rows hold."""
-    rows, n, dev = _rows("row8_read", codes, scales)
-    N.call("nitro_row8_read", codes.data_ptr(), scales.data_ptr(), _f32("row8_read", x, (rows, n), "x", dev), rows, n,
-           _stream_ptr(stream))
+    f = "row8_read"
+    rows, n, pc, ps, dev, s, f32 = _rows(f, codes, scales, stream)
+    N.call("nitro_row8_read", pc, ps, _ptr(f, x, f32, (rows, n), "x", dev), rows, n, s)
 
 
 class Q8Weights:
@@ -84,20 +83,14 @@ class Q8Weights:
     act(gate . x) * (up . x).  The tensors may go afterwards."""
 
     def __init__(self, w, up=None):
-        import torch
-
-        for t in (w, up):
-            if t is None and t is not w:
-                continue
+        torch = _torch_module()
+        dev = torch.cuda.current_device()
+        for t in (w,) if up is None else (w, up):
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
                 raise TypeError("weights must be GPU tensors")
-            if t.dtype is not torch.uint8 or not t.is_contiguous():
-                raise TypeError("weights must be contiguous uint8")
             if t.dim() < 2 or t.numel() == 0 or t.numel() // t.shape[0] % BLOCK_BYTES:
                 _refuse("Q8Weights", f"weights must be rows of whole {BLOCK_BYTES}-byte blocks")
-            if t.shape[0] != w.shape[0] or t.numel() != w.numel():
-                _refuse("Q8Weights", "the two matrices must have one shape")
-            _here("Q8Weights", t, torch.cuda.current_device())
+            _ptr("Q8Weights", t, torch.uint8, w.shape, "weights", dev)
         self.d = w.shape[0]
         self.n = w.numel() // self.d // BLOCK_BYTES * BLOCK
         self.gated = up is not None
@@ -110,17 +103,18 @@ class Q8Weights:
         """out[rows][d] = act(rows . w^T + bias) + residual; of a pair act(rows . gate^T +
         bias[:d]) * (rows . up^T + bias[d:]) + residual.  residual may be out."""
         f = "Q8Weights.matmul"
-        rows, n, dev = _rows(f, codes, scales)
+        rows, n, pc, ps, dev, s, f32 = _rows(f, codes, scales, stream)
         if n != self.n:
             _refuse(f, f"the rows have {n} entries, the weights {self.n}")
-        if activation not in ACTIVATIONS:
+        act = ACTIVATIONS.get(activation)
+        if act is None:
             _refuse(f, f"activation must be one of {', '.join(ACTIVATIONS)}")
-        if out is None:
-            _refuse(f, "out is required")
-        shape = (rows, self.d)
-        N.call("nitro_row8_matmul", self._h, codes.data_ptr(), scales.data_ptr(),
-               _f32(f, bias, (self.d * (1 + self.gated),), "bias", dev), _f32(f, residual, shape, "residual", dev),
-               _f32(f, out, shape, "out", dev), rows, ACTIVATIONS[activation], _stream_ptr(stream))
+        d = self.d
+        shape = (rows, d)
+        N.call("nitro_row8_matmul", self._h, pc, ps,
+               None if bias is None else _ptr(f, bias, f32, (2 * d if self.gated else d,), "bias", dev),
+               None if residual is None else _ptr(f, residual, f32, shape, "residual", dev),
+               _ptr(f, out, f32, shape, "out", dev), rows, act, s)
 
     def close(self):
         if getattr(self, "_h", None):

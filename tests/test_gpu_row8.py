@@ -415,7 +415,7 @@ def test_refusals():
     bad = [
         (codes[:, :32].contiguous(), scales, out, {}), (codes, scales[:2], out, {}), (codes, scales, out[:2], {}),
         (codes, scales, out, {"bias": out[0, :7].contiguous()}), (codes, scales, out, {"residual": out[:2]}),
-        (codes, scales, out, {"activation": "tanh"}), (codes, scales, None, {})]
+        (codes, scales, out, {"activation": "tanh"}), (codes[0], scales, out, {})]
     for c, s, o, kw in bad:
         with pytest.raises(na.NitroError):
             weights.matmul(c, s, o, **kw)
@@ -423,7 +423,7 @@ def test_refusals():
     with pytest.raises(na.NitroError):
         weights.matmul(odd, scales, out)
     for c, s, o in ((codes.float(), scales, out), (codes, scales.double(), out), (codes, scales, out.t()), (codes.cpu(), scales, out),
-                    (codes, scales, out.cpu())):
+                    (codes, scales, out.cpu()), (codes, scales, None), (codes, None, out)):
         with pytest.raises(TypeError):
             weights.matmul(c, s, o)
     for wrong in (w.view(-1), w[:, :, :35].contiguous(), torch.zeros((0, 36), dtype=torch.uint8, device="cuda")):
