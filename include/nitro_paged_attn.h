@@ -352,6 +352,8 @@ int nitro_rope_kv_append_prefill(nitro_kvpool* pool, int32_t layer, float* q, fl
  * reference's 8-lane AVX2 order (results agree to fp32 rounding). */
 #define NITRO_Q8_FULL_ROWS 0
 #define NITRO_Q8_LAST_BLOCK 1
+/* Of a model's forwards only: full rows, and what the Q8 products read held in 8 bits. */
+#define NITRO_Q8_ROW8 2
 int nitro_q8_matmul(const void* w, const float* x, float* out, int32_t batch, int32_t n,
                     int32_t d, int32_t semantics, void* stream);
 
@@ -436,7 +438,10 @@ int nitro_row8_matmul(const nitro_q8_weights* weights, const int8_t* codes, cons
  * semantics selects the Q8 product (NITRO_Q8_*): forward_decode_batch and
  * forward_prefill_chunk compute their Q8 products with matmul_bulk
  * (NITRO_Q8_LAST_BLOCK reproduces them), forward_paged with matmul
- * (NITRO_Q8_FULL_ROWS).  The classifier is fp32 in both. */
+ * (NITRO_Q8_FULL_ROWS).  NITRO_Q8_ROW8, which the reference lacks, is full rows with each
+ * product's input held in 8 bits ("rows held in 8 bits" above): rms_norm's output, the
+ * attention's and SwiGLU's; its first forward of any size allocates the tile-layout copy.
+ * The classifier is fp32 in all. */
 typedef struct nitro_model nitro_model;
 int nitro_model_create(const void* blob, uint64_t bytes, nitro_model** out);
 int nitro_model_destroy(nitro_model* model);

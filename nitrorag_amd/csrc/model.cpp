@@ -13,6 +13,7 @@
 #include "capi_common.hpp"
 #include "device_pool.hpp"
 #include "nitro_paged_attn.h"
+#include "row8.hpp"
 
 using namespace nitro;
 
@@ -27,17 +28,21 @@ struct nitro_model {
     // the seven Q8 matrices again in the matrix-core tile layout (Q8Tiled),
     // each section holding every layer (rows are multiples of 16, so no tile
     // spans two layers); read only by products over more than 4 rows of full
-    // rows, and built by the first forward that runs one (ensure_tiled)
+    // rows and by products of 8-bit rows, and built by the first forward that runs one
+    // (ensure_tiled)
     uint8_t* tiled = nullptr;
     size_t tiled_bytes = 0;
     size_t t_wq = 0, t_wk = 0, t_wv = 0, t_wo = 0, t_w1 = 0, t_w2 = 0, t_w3 = 0;
     DeviceBuffer<float> x, attn, q, last, ss;
     DeviceBuffer<float> hb;                // SwiGLU's output as floats (where hsplit does not hold them)
     DeviceBuffer<uint8_t> xsplit, hsplit;  // x (times the next norm's weights) and that output in split form
+    bool has_split = false;                // some forward's products read split form
+    DeviceBuffer<int8_t> codes;            // rows held in 8 bits (NITRO_Q8_ROW8)
+    DeviceBuffer<float> scales;
     int max_rows = 0;                      // of any forward
     float* hb_floats() const { return hb.ptr ? hb.ptr : reinterpret_cast<float*>(hsplit.ptr); }
     DeviceBuffer<int32_t> tokens;
-    DeviceBuffer<float> kv_rows;   // over an 8-bit pool: a layer's new K rows, then its V rows, on their way there
+    DeviceBuffer<float> kv_rows;   // over an 8-bit pool, and of 8-bit rows: a layer's new K rows, then its V rows, on their way there
     DeviceBuffer<int32_t> kv_at;   // 0, 1, 2, ..: where the products put row r of them
     int kv_at_rows = 0;            // (filled so far)
     Staging staging;
@@ -66,7 +71,7 @@ hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // Builds the tile-layout copy of the Q8 matrices (1.125 bytes per weight) on
 // the first forward that reads it, so a model that never runs more than 4
-// rows of full-row products never holds it.  Allocates: a caller capturing
+// rows of full-row products, nor 8-bit rows, never holds it.  Allocates: a caller capturing
 // such forwards into a HIP graph runs one of them before the capture.
 void ensure_tiled(nitro_model* m, hipStream_t s) {
     if (m->tiled) return;
@@ -91,11 +96,16 @@ void ensure_tiled(nitro_model* m, hipStream_t s) {
 // rows as any forward had, and that memory serves SwiGLU's output as floats too
 // unless those have a buffer already.  Only a forward of more rows than any before
 // moves a buffer that exists (a captured forward holds their addresses).
-void reserve_rows(nitro_model* m, const nitro_kvpool* pool, int rows, bool last_block) {
+void reserve_rows(nitro_model* m, const nitro_kvpool* pool, int rows, int semantics) {
     m->max_rows = std::max(m->max_rows, rows);
     const size_t r = (size_t)m->max_rows;
+    const bool row8 = semantics == NITRO_Q8_ROW8;
+    if (row8 || m->codes.ptr) {
+        m->codes.reserve(r * (size_t)std::max(m->dim, m->hidden));
+        m->scales.reserve(r);
+    }
+    if (row8 || pool->q8 || m->kv_rows.ptr) m->kv_rows.reserve(2 * r * m->kv_dim);
     if (pool->q8) {
-        m->kv_rows.reserve(2 * r * m->kv_dim);
         if (m->kv_at.reserve(r)) m->kv_at_rows = 0;
         if (m->kv_at_rows < rows) {  // all of it, before any stream reads it
             std::vector<int32_t> at(m->kv_at.count);
@@ -111,7 +121,8 @@ void reserve_rows(nitro_model* m, const nitro_kvpool* pool, int rows, bool last_
     m->ss.reserve(r * (size_t)((m->dim + 15) / 16));
     m->q.reserve(r * m->dim);
     m->tokens.reserve(r);
-    if (m->tiled || (!last_block && rows > Q8_GEMV_MAX_BATCH)) {
+    m->has_split = m->has_split || (semantics == NITRO_Q8_FULL_ROWS && rows > Q8_GEMV_MAX_BATCH);
+    if (m->has_split) {
         const size_t sr = q8_split_usable(r, m->dim, m->hidden) ? r : (size_t)rows;
         if (q8_split_usable(sr, m->dim, m->hidden)) {
             m->xsplit.reserve(q8_split_bytes(sr, m->dim));
@@ -148,15 +159,79 @@ void upload_tokens(nitro_model* m, const int32_t* tokens, int rows, hipStream_t 
 // product left partial sums of squares for (src/model_q8.cpp:553-555,
 // :687-692).  The norm rides in the classifier launch where its flat kernel
 // takes the batch (x stays unnormalised); otherwise x is normalised in place
-// first.
-void final_logits(nitro_model* m, float* x, int first, int total, int rows, float* logits, hipStream_t s) {
+// first, as where no product left partials (of 8-bit rows).
+void final_logits(nitro_model* m, float* x, int first, int total, int rows, bool partials, float* logits, hipStream_t s) {
     const Q8Norm nm{m->f32(m->o_rms_final), m->ss.ptr + first, (m->dim + 15) / 16, total};
-    if (launch_f32_matmul_norm(m->f32(m->o_emb), x, nm, logits, rows, m->dim, m->vocab, s)) {
+    if (partials && launch_f32_matmul_norm(m->f32(m->o_emb), x, nm, logits, rows, m->dim, m->vocab, s)) {
         hip_check(hipGetLastError(), "classifier launch");
         return;
     }
     hip_check(launch_add_rmsnorm(x, nullptr, m->f32(m->o_rms_final), x, rows, m->dim, s), "rmsnorm launch");
     hip_check(launch_f32_matmul(m->f32(m->o_emb), x, logits, rows, m->dim, m->vocab, s), "classifier launch");
+}
+
+void check_semantics(int semantics) {
+    require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK || semantics == NITRO_Q8_ROW8,
+            ERR_INVALID_ARGUMENT, "unknown Q8 semantics");
+}
+
+// The layer loop with what the products read held in 8 bits.  Ten launches a layer: a row's
+// scale needs the whole row, so the norms, the attention's output and SwiGLU's output each
+// get a launch of their own that holds them, and RoPE + append follows its product.  Rows
+// [0, prefill) are the prefill batch's, the others the decode batch's.
+template <typename Attend>
+void layers_row8(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, int rows, int prefill, hipStream_t s,
+                 Attend attend) {
+    const int dim = m->dim, kv = m->kv_dim, hid = m->hidden;
+    ensure_tiled(m, s);
+    float* const k = m->kv_rows.ptr;
+    float* const v = k + (size_t)m->max_rows * kv;
+    float* const hb = m->hb_floats();
+    void* stream = s;
+    auto hold = [&](const float* x, const float* norm, int n) {
+        hip_check(launch_row8_norm({x, nullptr, norm, nullptr, m->codes.ptr, m->scales.ptr, rows, n, 1e-5}, s), "row8 launch");
+    };
+    auto multiply = [&](Row8Matmul a, int n, const char* what) {
+        a.codes = m->codes.ptr, a.scales = m->scales.ptr;
+        a.rows = rows, a.n = n;
+        hip_check(launch_row8_matmul(a, s), what);
+    };
+    auto append = [&](int l) {
+        auto rope = [&](auto entry, size_t first) {
+            require(entry(pool, l, m->q.ptr + first * dim, k + first * kv, v + first * kv, m->f32(m->o_freq_real),
+                          m->f32(m->o_freq_imag), m->seq_len, m->n_heads, m->n_kv_heads, m->head_size, stream) == NITRO_OK,
+                    ERR_INVALID_ARGUMENT, nitro_last_error());
+        };
+        if (prefill) rope(nitro_rope_kv_append_prefill, 0);
+        if (prefill < rows) rope(nitro_rope_kv_append, (size_t)prefill);
+    };
+    hip_check(launch_embed_rows(m->f32(m->o_emb), tokens, m->x.ptr, rows, dim, m->vocab, pool->bad_pages.ptr, m->ss.ptr,
+                                Q8SplitOut{}, s),
+              "embed launch");
+    for (int l = 0; l < m->n_layers; l++) {
+        hold(m->x.ptr, m->f32(m->o_rms_att) + (size_t)l * dim, dim);
+        Row8Matmul qkv{};
+        qkv.w[0] = m->q8t(m->t_wq, l, dim, dim), qkv.w[1] = m->q8t(m->t_wk, l, kv, dim), qkv.w[2] = m->q8t(m->t_wv, l, kv, dim);
+        qkv.out[0] = m->q.ptr, qkv.out[1] = k, qkv.out[2] = v;
+        qkv.d[0] = dim, qkv.d[1] = qkv.d[2] = kv;
+        qkv.mats = 3;
+        multiply(qkv, dim, "row8 wq/wk/wv launch");
+        append(l);
+        attend(l);
+        hold(m->attn.ptr, nullptr, dim);
+        Row8Matmul back{};  // x += w . rows
+        back.w[0] = m->q8t(m->t_wo, l, dim, dim), back.out[0] = m->x.ptr, back.residual = m->x.ptr, back.d[0] = dim, back.mats = 1;
+        multiply(back, dim, "row8 wo launch");
+        hold(m->x.ptr, m->f32(m->o_rms_ffn) + (size_t)l * dim, dim);
+        Row8Matmul ffn{};
+        ffn.w[0] = m->q8t(m->t_w1, l, hid, dim), ffn.w[1] = m->q8t(m->t_w3, l, hid, dim);
+        ffn.out[0] = hb, ffn.d[0] = hid, ffn.mats = 1;
+        ffn.gated = true, ffn.activation = NITRO_ACT_SILU;
+        multiply(ffn, dim, "row8 w1/w3 launch");
+        hold(hb, nullptr, hid);
+        back.w[0] = m->q8t(m->t_w2, l, dim, hid);
+        multiply(back, hid, "row8 w2 launch");
+    }
 }
 
 // The layer loop shared by the decode, prefill and mixed forwards.  x is the
@@ -166,8 +241,9 @@ void final_logits(nitro_model* m, float* x, int first, int total, int rows, floa
 // squares the next norm needs in `ss` (src/model_q8.cpp:584-684).  After it x
 // holds the final residual stream.
 template <typename Attend>
-void layers(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, int rows, int semantics, Q8Rope rope,
+void layers(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, int rows, int prefill, int semantics, Q8Rope rope,
             hipStream_t s, Attend attend) {
+    if (semantics == NITRO_Q8_ROW8) return layers_row8(m, pool, tokens, rows, prefill, s, attend);
     const int dim = m->dim, kv = m->kv_dim, hid = m->hidden;
     const bool last = semantics == NITRO_Q8_LAST_BLOCK;
     const int parts = (dim + 15) / 16;  // partials per row left by wo / w2
@@ -254,9 +330,9 @@ Q8Rope rope_args(const nitro_model* m, nitro_kvpool* pool, const int32_t* pos_a,
 }
 
 // Over an 8-bit pool: layer l's rows, `prefill` of the prefill batch's and then
-// `decode` of the decode batch's, into the cache.
-void append_held(const nitro_model* m, nitro_kvpool* pool, int l, int prefill, int decode, void* stream) {
-    if (!pool->q8) return;
+// `decode` of the decode batch's, into the cache (8-bit rows are there by then).
+void append_held(const nitro_model* m, nitro_kvpool* pool, int l, int prefill, int decode, int semantics, void* stream) {
+    if (!pool->q8 || semantics == NITRO_Q8_ROW8) return;
     const float* k = m->kv_rows.ptr;
     const float* v = k + (size_t)m->max_rows * m->kv_dim;
     const size_t after = (size_t)prefill * m->kv_dim;
@@ -311,12 +387,12 @@ void forward_mixed(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, in
     if (!prefill_as_decode && P > 0) check_positions(m, pf.max_pos);
     // every row's RoPE position and K/V slot: the decode batch's, or the
     // prefill batch's for rows [0, P) when those go through the prefill kernel
-    reserve_rows(m, pool, P + B, semantics == NITRO_Q8_LAST_BLOCK);
+    reserve_rows(m, pool, P + B, semantics);
     const Q8Rope rope = prefill_as_decode || P == 0
                             ? rope_args(m, pool, d.pos.ptr, d.slots.ptr, P + B, nullptr, nullptr)
                             : rope_args(m, pool, pf.row_pos.ptr, pf.slots.ptr, P, d.pos.ptr, d.slots.ptr);
-    layers(m, pool, tokens, P + B, semantics, rope, s, [&](int l) {
-        append_held(m, pool, l, prefill_as_decode ? 0 : P, prefill_as_decode ? P + B : B, stream);
+    layers(m, pool, tokens, P + B, prefill_as_decode ? 0 : P, semantics, rope, s, [&](int l) {
+        append_held(m, pool, l, prefill_as_decode ? 0 : P, prefill_as_decode ? P + B : B, semantics, stream);
         if (prefill_as_decode) {
             // every row attends its own prefix (keys 0..position) in one
             // decode-attention launch; a chunk row at position p sees the same
@@ -344,7 +420,7 @@ void forward_mixed(nitro_model* m, nitro_kvpool* pool, const int32_t* tokens, in
     const int out_rows = P + B - first;
     if (out_rows == 0) return;
     float* x = m->x.ptr + first * dim;
-    final_logits(m, x, first, P + B, out_rows, logits, s);
+    final_logits(m, x, first, P + B, out_rows, semantics != NITRO_Q8_ROW8, logits, s);
     hip_check(launch_argmax_rows(logits, next, out_rows, m->vocab, s), "argmax launch");
     pool->last_stream = s;
 }
@@ -445,25 +521,24 @@ int nitro_forward_decode_batch(nitro_model* m, nitro_kvpool* pool, const int32_t
     return guarded([&] {
         check_model_pool(m, pool);
         require(logits != nullptr, ERR_INVALID_ARGUMENT, "null logits");
-        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK, ERR_INVALID_ARGUMENT,
-                "unknown Q8 semantics");
+        check_semantics(semantics);
         require(pool->decode.batch > 0, ERR_NO_BATCH, "no decode batch uploaded");
         require(batch == pool->decode.batch, ERR_INVALID_ARGUMENT,
                 "batch differs from the uploaded decode batch");
         hipStream_t s = as_stream(stream);
         const DecodeBatch& d = pool->decode;
         check_positions(m, max_of(d.positions));
-        reserve_rows(m, pool, batch, semantics == NITRO_Q8_LAST_BLOCK);
+        reserve_rows(m, pool, batch, semantics);
         upload_tokens(m, tokens, batch, s);
         const Q8Rope rope = rope_args(m, pool, d.pos.ptr, d.slots.ptr, batch, nullptr, nullptr);
-        layers(m, pool, m->tokens.ptr, batch, semantics, rope, s, [&](int l) {
-            append_held(m, pool, l, 0, batch, stream);
+        layers(m, pool, m->tokens.ptr, batch, 0, semantics, rope, s, [&](int l) {
+            append_held(m, pool, l, 0, batch, semantics, stream);
             require(nitro_paged_attn_decode(pool, l, m->q.ptr, m->attn.ptr, m->n_heads, m->n_kv_heads,
                                             m->head_size, stream) == NITRO_OK,
                     ERR_INVALID_ARGUMENT, nitro_last_error());
         });
         // logits = wcls . rms_norm(x) (:687-692)
-        final_logits(m, m->x.ptr, 0, batch, batch, logits, s);
+        final_logits(m, m->x.ptr, 0, batch, batch, semantics != NITRO_Q8_ROW8, logits, s);
         pool->last_stream = s;
     });
 }
@@ -473,20 +548,19 @@ int nitro_forward_prefill(nitro_model* m, nitro_kvpool* pool, const int32_t* tok
     return guarded([&] {
         check_model_pool(m, pool);
         require(logits != nullptr, ERR_INVALID_ARGUMENT, "null logits");
-        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK, ERR_INVALID_ARGUMENT,
-                "unknown Q8 semantics");
+        check_semantics(semantics);
         const PrefillBatch& p = pool->prefill;
         require(p.batch > 0, ERR_NO_BATCH, "no prefill batch uploaded");
         require(total_rows == p.total_rows, ERR_INVALID_ARGUMENT,
                 "total_rows differs from the uploaded prefill batch");
         hipStream_t s = as_stream(stream);
-        reserve_rows(m, pool, total_rows, semantics == NITRO_Q8_LAST_BLOCK);
+        reserve_rows(m, pool, total_rows, semantics);
         m->last.reserve((size_t)p.batch * m->dim);
         upload_tokens(m, tokens, total_rows, s);
         check_positions(m, p.max_pos);
         const Q8Rope rope = rope_args(m, pool, p.row_pos.ptr, p.slots.ptr, total_rows, nullptr, nullptr);
-        layers(m, pool, m->tokens.ptr, total_rows, semantics, rope, s, [&](int l) {
-            append_held(m, pool, l, total_rows, 0, stream);
+        layers(m, pool, m->tokens.ptr, total_rows, total_rows, semantics, rope, s, [&](int l) {
+            append_held(m, pool, l, total_rows, 0, semantics, stream);
             require(nitro_paged_attn_prefill(pool, l, m->q.ptr, m->attn.ptr, m->n_heads, m->n_kv_heads,
                                              m->head_size, stream) == NITRO_OK,
                     ERR_INVALID_ARGUMENT, nitro_last_error());

@@ -162,8 +162,8 @@ int nitro_server_create(nitro_scheduler* sched, nitro_model* model, nitro_kvpool
         require(out != nullptr, ERR_INVALID_ARGUMENT, "null output pointer");
         *out = nullptr;
         require(sched && model && pool, ERR_INVALID_ARGUMENT, "null handle");
-        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK, ERR_INVALID_ARGUMENT,
-                "unknown Q8 semantics");
+        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK || semantics == NITRO_Q8_ROW8,
+                ERR_INVALID_ARGUMENT, "unknown Q8 semantics");
         require(max_prompt_tokens > 0, ERR_INVALID_ARGUMENT, "max_prompt_tokens must be positive");
         auto* s = new nitro_server();
         s->sched = sched;

@@ -131,8 +131,8 @@ int nitro_sched_step(nitro_scheduler* sched, nitro_model* model, nitro_kvpool* p
                      void* stream) {
     return guarded([&] {
         require(sched != nullptr && model != nullptr && pool != nullptr, ERR_INVALID_ARGUMENT, "null handle");
-        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK, ERR_INVALID_ARGUMENT,
-                "unknown Q8 semantics");
+        require(semantics == NITRO_Q8_FULL_ROWS || semantics == NITRO_Q8_LAST_BLOCK || semantics == NITRO_Q8_ROW8,
+                ERR_INVALID_ARGUMENT, "unknown Q8 semantics");
         ContinuousScheduler& h = sched->host;
         int32_t dims[5];
         model_dims(model, dims);

@@ -10,7 +10,7 @@ import numpy as np
 
 from . import _native as N
 from .attention import _dev, _stream_ptr
-from .q8 import FULL_ROWS, LAST_BLOCK  # noqa: F401  (re-exported semantics)
+from .q8 import FULL_ROWS, LAST_BLOCK, ROW8  # noqa: F401  (re-exported semantics)
 
 HEADER_FIELDS = ("dim", "hidden_dim", "n_layers", "n_heads", "n_kv_heads", "vocab_size", "seq_len")
 

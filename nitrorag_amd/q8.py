@@ -14,6 +14,7 @@ from .attention import _dev, _stream_ptr
 
 FULL_ROWS = 0    # matmul (src/model_q8.cpp:92-125)
 LAST_BLOCK = 1   # matmul_bulk (src/model_q8.cpp:382-420): only the last 32 columns count
+ROW8 = 2         # of a model's forwards: full rows, the products' inputs held in 8 bits
 BLOCK = 32
 BLOCK_BYTES = 36
 # launches of tile_rows: q8_matmul, and a model's wo / w2, w1 + w3, wq + wk + wv
