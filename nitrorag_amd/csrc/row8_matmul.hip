@@ -45,6 +45,27 @@ __device__ __forceinline__ int member_of(const Row8Matmul& a, int& ct, int cols)
     return m;
 }
 
+// A launch's output tiles, and which of the two orders of them the XCDs share out: each
+// takes an eighth, of the rows' panels (every column tile of one after the other) or of the
+// columns', whichever brings less into its L2.  (512 rows of 4096 x 4096 as panels of rows:
+// every L2 reads the whole matrix, 161 MB of misses where the matrix has 19.)  A single panel
+// of rows is taken as it comes: there is nothing to share, and neighbouring tiles on different
+// XCDs read faster (one row of 11008 x 4096: 10.1 against 11.3 us).
+struct Tiles {
+    int rows, cols;
+    bool by_columns;
+};
+struct Place {
+    int row, col;
+};
+__device__ __forceinline__ Place place_of(const Tiles& t) {
+    if (t.rows == 1) return {0, (int)blockIdx.x};
+    const int wg = blockIdx.x, total = gridDim.x, per = total >> 3, rem = total & 7, xcd = wg & 7;
+    const int i = xcd * per + min(xcd, rem) + (wg >> 3);
+    if (t.by_columns) return {i % t.rows, i / t.rows};
+    return {i / t.cols, i % t.cols};
+}
+
 // ---------------------------------------------------------- split over waves
 // A workgroup owns RT x CT tiles of U batch rows x U weight rows (U = 16 or 32, the matrix
 // instruction's); its W waves split the blocks, each with sums of its own, which are
@@ -107,7 +128,7 @@ struct Tile<32> {
 };
 
 template <int U, int RT, int CT, int W, int OCC, bool GATED>
-__global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a) {
+__global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, Tiles tiling) {
     typedef Tile<U> T;
     constexpr int ROWS = U * RT, COLS = U * CT / (GATED ? 2 : 1);  // of the output
     constexpr int ROUND = 4, PITCH = ROUND * Q8_BLOCK + 16;  // blocks a round; bytes of a row in LDS
@@ -115,10 +136,11 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a) {
     constexpr int PART = RT * CT * T::SUMS * 64, XBYTES = W * ROWS * PITCH, SBYTES = W * PART * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[XBYTES > SBYTES ? XBYTES : SBYTES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int ct = blockIdx.x;
+    const Place place = place_of(tiling);
+    int ct = place.col;
     const int member = member_of(a, ct, COLS);
     const int d = a.d[member], n = a.n, nb = n / Q8_BLOCK, tiles = (d + 15) / 16;
-    const int b0 = blockIdx.y * ROWS;
+    const int b0 = place.row * ROWS;
 
     // Weight tiles of 16 rows, the last one for those past the end; with a gate, tile 2t is
     // the gate's and 2t + 1 the other matrix's.
@@ -242,7 +264,7 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a) {
 // each two.  x lies as four planes (a block's halves) of 16 bytes a row, so that lanes read
 // consecutive rows; the weights as in the tile layout, runs of 8 k.
 template <int MT, int NT, int DEPTH, int OCC, bool GATED>
-__global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, int col_tiles) {
+__global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles tiling) {
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
     constexpr int PLANE = BM * 16 + 32;  // (the planes' banks lie 32 bytes apart: a row's four runs are written together)
     constexpr int XB = 4 * PLANE, WB = 2 * BN * 32, BUF = XB + WB + 2 * BN * 4;
@@ -255,14 +277,9 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, int c
     const int lane = tid & 63, wave = tid >> 6;
     const int wm = wave & 1, wn = wave >> 1, lc = lane & 31, lh = lane >> 5;
 
-    // Column tiles fastest, XCD i taking the i-th eighth of the work.
-    int wg = blockIdx.x;
-    {
-        const int total = gridDim.x, per = total >> 3, rem = total & 7, xcd = wg & 7;
-        wg = xcd * per + min(xcd, rem) + (wg >> 3);
-    }
-    const int b0 = wg / col_tiles * BM;
-    int ct = wg % col_tiles;
+    const Place place = place_of(tiling);
+    const int b0 = place.row * BM;
+    int ct = place.col;
     const int member = member_of(a, ct, COLS);
     const int d = a.d[member], n = a.n, nb = n / Q8_BLOCK, tiles = (d + 15) / 16;
 
@@ -451,78 +468,77 @@ struct Form {
     int rows, cols, blocks, split, resident;
     float fixed, alone, busy;
     bool gates;  // its column tiles are even in number
-    bool tall;   // batch rows in the grid's first dimension
     int threads;
-    void (*launch)(const Row8Matmul&, dim3, int, hipStream_t);
+    void (*launch)(const Row8Matmul&, const Tiles&, hipStream_t);
 };
 
 template <int U, int RT, int CT, int W, int OCC>
 constexpr Form split_form(int resident, float fixed, float alone, float busy) {
-    return {U * RT, U * CT, 4, W, resident, fixed, alone, busy, CT % 2 == 0, false, 64 * W,
-            [](const Row8Matmul& a, dim3 grid, int, hipStream_t stream) {
+    return {U * RT, U * CT, 4, W, resident, fixed, alone, busy, CT % 2 == 0, 64 * W,
+            [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
+                const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(64 * W);
                 if constexpr (CT % 2 == 0) {
                     if (a.gated) {
-                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, true>), grid, dim3(64 * W), 0, stream, a);
+                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, true>), grid, block, 0, stream, a, t);
                         return;
                     }
                 }
-                hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, dim3(64 * W), 0, stream, a);
+                hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, block, 0, stream, a, t);
             }};
 }
 
 template <int MT, int NT, int DEPTH, int OCC>
 constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
-    return {64 * MT, 64 * NT, 2, 1, resident, fixed, alone, busy, NT == 2, true, 256,
-            [](const Row8Matmul& a, dim3 grid, int col_tiles, hipStream_t stream) {
+    return {64 * MT, 64 * NT, 2, 1, resident, fixed, alone, busy, NT == 2, 256,
+            [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
+                const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(256);
                 if constexpr (NT == 2) {
                     if (a.gated) {
-                        hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, true>), grid, dim3(256), 0, stream, a, col_tiles);
+                        hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, true>), grid, block, 0, stream, a, t);
                         return;
                     }
                 }
-                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, false>), grid, dim3(256), 0, stream, a, col_tiles);
+                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, false>), grid, block, 0, stream, a, t);
             }};
 }
 
-// Each timed over some 300 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384,
-// gated or not) as graph replays, and fitted to within 5 to 9% of its own times.  The
-// choice by these estimates takes 1.3% longer in the mean than the best of the forms each
-// time (at most 29%).
+// Each timed over 340 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
+// or not) as graph replays, and fitted to within 4 to 8% of its own times.  The choice by
+// these estimates takes 1.1% longer in the mean than the best of the forms each time; at
+// most 41%, 7.9 against 5.6 us, for a gated pair of 80 rows of 128.
 constexpr Form FORMS[] = {
-    split_form<16, 1, 1, 4, 5>(9, 2.14f, 0.329f, 0.309f),
-    split_form<16, 1, 1, 8, 4>(3, 2.10f, 0.129f, 0.588f),
-    split_form<16, 1, 2, 4, 4>(5, 2.26f, 0.677f, 0.521f),
-    split_form<16, 1, 2, 8, 4>(3, 2.12f, 0.175f, 1.084f),
-    split_form<16, 2, 2, 8, 4>(2, 2.24f, 1.402f, 1.420f),
-    split_form<32, 1, 1, 4, 4>(4, 2.77f, 0.574f, 0.554f),
-    split_form<32, 2, 2, 4, 2>(1, 4.84f, 0.048f, 1.582f),
-    gemm_form<1, 1, 2, 4>(4, 2.91f, 0.418f, 0.196f),
-    gemm_form<1, 2, 2, 3>(2, 3.64f, 0.516f, 0.365f),
-    gemm_form<2, 2, 1, 3>(2, 5.60f, 0.805f, 0.569f),
-    gemm_form<4, 2, 1, 2>(2, 11.60f, 1.374f, 0.981f),
+    split_form<16, 1, 1, 4, 5>(10, 2.25f, 0.314f, 0.294f),
+    split_form<16, 1, 1, 8, 4>(3, 2.15f, 0.064f, 0.584f),
+    split_form<16, 1, 2, 4, 4>(6, 2.40f, 0.632f, 0.514f),
+    split_form<16, 1, 2, 8, 4>(2, 2.18f, 0.221f, 1.047f),
+    split_form<16, 2, 2, 8, 4>(1, 2.41f, 0.026f, 1.244f),
+    split_form<32, 1, 1, 4, 4>(4, 2.84f, 0.587f, 0.564f),
+    split_form<32, 2, 2, 4, 2>(1, 5.45f, 1.546f, 0.069f),
+    gemm_form<1, 1, 2, 4>(4, 3.08f, 0.341f, 0.195f),
+    gemm_form<1, 2, 2, 3>(3, 3.80f, 0.514f, 0.342f),
+    gemm_form<2, 2, 1, 3>(2, 5.66f, 0.794f, 0.576f),
+    gemm_form<4, 2, 1, 2>(3, 8.90f, 1.377f, 1.050f),
 };
 
-struct Grid {
-    int64_t x, y;
-    int col_tiles;
-};
-// (a grid's threads in x count in 32 bits, its workgroups in y in 16)
-bool grid_of(const Form& f, const Row8Matmul& a, Grid& g) {
-    g.col_tiles = col_tiles_of(a, a.gated ? f.cols / 2 : f.cols);
-    const int64_t row_tiles = ((int64_t)a.rows + f.rows - 1) / f.rows;
-    g.x = f.tall ? g.col_tiles * row_tiles : g.col_tiles, g.y = f.tall ? 1 : row_tiles;
-    return (f.gates || !a.gated) && g.y < 65536 && g.x * f.threads < (1ll << 32);
+// (A grid's threads count in 32 bits.)
+bool tiles_of(const Form& f, const Row8Matmul& a, Tiles& t) {
+    t.cols = col_tiles_of(a, a.gated ? f.cols / 2 : f.cols);
+    t.rows = (a.rows + f.rows - 1) / f.rows;
+    // codes against weights, as rows of n (a weight has 1.125 bytes)
+    const float x = (float)t.rows * f.rows, w = 1.125f * t.cols * f.cols;
+    t.by_columns = x + w / 8 < x / 8 + w;
+    return (f.gates || !a.gated) && (int64_t)t.rows * t.cols * f.threads < (1ll << 32);
 }
 
-float estimate(const Form& f, const Row8Matmul& a, const Grid& g, int cus) {
-    const int64_t groups = (g.x * g.y + cus - 1) / cus;  // of the busiest CU
+float estimate(const Form& f, const Row8Matmul& a, const Tiles& t, int cus) {
+    const int groups = (int)(((int64_t)t.rows * t.cols + cus - 1) / cus);  // of the busiest CU
     const int blocks = a.n / Q8_BLOCK, steps = (blocks + f.blocks - 1) / f.blocks;
     const float chain = (float)((steps + f.split - 1) / f.split);
     const float set = 0.3f * f.fixed;
-    const int64_t full = groups / f.resident, rest = groups % f.resident;
-    float t = f.fixed + full * (set + chain * std::max(f.alone, f.resident * f.busy));
-    if (rest) t += set + chain * std::max(f.alone, rest * f.busy);
-    return t;
+    const int full = groups / f.resident, rest = groups % f.resident;
+    float us = f.fixed + full * (set + chain * std::max(f.alone, f.resident * f.busy));
+    if (rest) us += set + chain * std::max(f.alone, rest * f.busy);
+    return us;
 }
 
 // Rows of one launch at most.
@@ -540,16 +556,16 @@ hipError_t launch_row8_matmul(const Row8Matmul& whole, hipStream_t stream) {
         if (a.residual) a.residual += (size_t)r0 * a.d[0];
         for (int m = 0; m < a.mats; m++) a.out[m] += (size_t)r0 * a.d[m];
         const Form* best = nullptr;
-        Grid grid{};
+        Tiles tiles{};
         float least = 0.0f;
         for (const Form& f : FORMS) {
-            Grid g;
-            if (!grid_of(f, a, g)) continue;
-            const float t = estimate(f, a, g, cus);
-            if (!best || t < least) best = &f, least = t, grid = g;
+            Tiles t;
+            if (!tiles_of(f, a, t)) continue;
+            const float us = estimate(f, a, t, cus);
+            if (!best || us < least) best = &f, least = us, tiles = t;
         }
         if (!best) return hipErrorInvalidConfiguration;
-        best->launch(a, dim3((unsigned)grid.x, (unsigned)grid.y), grid.col_tiles, stream);
+        best->launch(a, tiles, stream);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
