@@ -1,6 +1,10 @@
 // Rows into 8 bits for gfx950 (row8.hpp), with the rms_norm and the residual's
 // addition that come before in a model's layer (src/model_q8.cpp:128-140).
 //
+// Bound by bytes, 5 or 9 (with a residual and its sum 13) an entry: 8192 rows of 4096 with
+// residual and sum 84 us (5.2 TB/s, what a copy has), held only 31 us, read back 34 us; one
+// row of 4096 4.2, 2.4 and 2.4 us: latency (launch, loads, two joins over the row).
+//
 // Mathematics.  h = fp32(x + residual), y = fp32(h * weight / sqrt(mean(h^2) + eps)).
 // The mean, its root and the products are taken in 64 bits and y is rounded once:
 // a code is a step of 1/127 of the row's largest entry, so an error of one fp32 rounding
@@ -229,9 +233,11 @@ void launch_rows(const Row8Norm& a, hipStream_t stream) {
 
 }  // namespace
 
-// A wave to a row up to 1024 entries, then a workgroup, four groups of four to a lane;
-// where the CUs have a row each at most, as many lanes as there are groups (one row of
-// 4096: 3.7 us, with 256 lanes 4.6).  Past the registers of 1024 lanes a row is read again.
+// A wave to a row up to 1024 entries, then a workgroup with four groups of four to a lane
+// (as many lanes as groups, 1024 of one each, gained 0.2 us of 4.2 at one row of 4096 and lost
+// 15 to 40% past 512 rows).  A norm's row past 1024 lanes' registers is read again for each
+// use (3.7 to 4.2 TB/s of what it cannot do without, where shorter rows have 4.5 to 5.6); the
+// registers of rows that are only held go further, for they need no 64-bit values.
 hipError_t launch_row8_norm(const Row8Norm& whole, hipStream_t stream) {
     constexpr int SLICE = 1 << 21;  // rows of a launch at most (a grid's threads count in 32 bits)
     for (int r0 = 0; r0 < whole.rows; r0 += std::min(SLICE, whole.rows - r0)) {
@@ -242,12 +248,9 @@ hipError_t launch_row8_norm(const Row8Norm& whole, hipStream_t stream) {
         a.x += at, a.codes += at, a.scales += r0;
         if (a.residual) a.residual += at;
         if (a.sum) a.sum += at;
-        const bool few = a.rows <= device_cus();
         if (n <= 256) launch_rows<64, 1>(a, stream);
         else if (n <= 512) launch_rows<64, 2>(a, stream);
         else if (n <= 1024) launch_rows<64, 4>(a, stream);
-        else if (few && n <= 4096) launch_rows<1024, 1>(a, stream);
-        else if (few && n <= 8192) launch_rows<1024, 2>(a, stream);
         else if (n <= 2048) launch_rows<256, 2>(a, stream);
         else if (n <= 4096) launch_rows<256, 4>(a, stream);
         else if (n <= 8192) launch_rows<512, 4>(a, stream);

@@ -452,10 +452,12 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
     }
 }
 
-int col_tiles_of(const Row8Matmul& a, int cols) {
-    if (a.gated) return (a.d[0] + cols - 1) / cols;
+constexpr int log2_of(int x) { return x == 1 ? 0 : 1 + log2_of(x / 2); }
+int tiles_over(int x, int log2) { return (int)(((int64_t)x + (1 << log2) - 1) >> log2); }
+
+int col_tiles_of(const Row8Matmul& a, int log2) {
     int t = 0;
-    for (int m = 0; m < a.mats; m++) t += (a.d[m] + cols - 1) / cols;
+    for (int m = 0; m < (a.gated ? 1 : a.mats); m++) t += tiles_over(a.d[m], log2);
     return t;
 }
 
@@ -465,7 +467,8 @@ int col_tiles_of(const Row8Matmul& a, int cols) {
 // do, at most `resident` at once; `fixed` us for a launch, a third of it again for every
 // set of resident workgroups.
 struct Form {
-    int rows, cols, blocks, split, resident;
+    int rows, cols, blocks, split;  // as powers of two (a call looks at every form)
+    int resident;
     float fixed, alone, busy;
     bool gates;  // its column tiles are even in number
     int threads;
@@ -474,7 +477,7 @@ struct Form {
 
 template <int U, int RT, int CT, int W, int OCC>
 constexpr Form split_form(int resident, float fixed, float alone, float busy) {
-    return {U * RT, U * CT, 4, W, resident, fixed, alone, busy, CT % 2 == 0, 64 * W,
+    return {log2_of(U * RT), log2_of(U * CT), 2, log2_of(W), resident, fixed, alone, busy, CT % 2 == 0, 64 * W,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
                 const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(64 * W);
                 if constexpr (CT % 2 == 0) {
@@ -489,7 +492,7 @@ constexpr Form split_form(int resident, float fixed, float alone, float busy) {
 
 template <int MT, int NT, int DEPTH, int OCC>
 constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
-    return {64 * MT, 64 * NT, 2, 1, resident, fixed, alone, busy, NT == 2, 256,
+    return {log2_of(64 * MT), log2_of(64 * NT), 1, 0, resident, fixed, alone, busy, NT == 2, 256,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
                 const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(256);
                 if constexpr (NT == 2) {
@@ -522,18 +525,17 @@ constexpr Form FORMS[] = {
 
 // (A grid's threads count in 32 bits.)
 bool tiles_of(const Form& f, const Row8Matmul& a, Tiles& t) {
-    t.cols = col_tiles_of(a, a.gated ? f.cols / 2 : f.cols);
-    t.rows = (a.rows + f.rows - 1) / f.rows;
+    t.cols = col_tiles_of(a, f.cols - (a.gated ? 1 : 0));
+    t.rows = tiles_over(a.rows, f.rows);
     // codes against weights, as rows of n (a weight has 1.125 bytes)
-    const float x = (float)t.rows * f.rows, w = 1.125f * t.cols * f.cols;
+    const float x = (float)t.rows * (float)(1 << f.rows), w = 1.125f * (float)t.cols * (float)(1 << f.cols);
     t.by_columns = x + w / 8 < x / 8 + w;
     return (f.gates || !a.gated) && (int64_t)t.rows * t.cols * f.threads < (1ll << 32);
 }
 
 float estimate(const Form& f, const Row8Matmul& a, const Tiles& t, int cus) {
-    const int groups = (int)(((int64_t)t.rows * t.cols + cus - 1) / cus);  // of the busiest CU
-    const int blocks = a.n / Q8_BLOCK, steps = (blocks + f.blocks - 1) / f.blocks;
-    const float chain = (float)((steps + f.split - 1) / f.split);
+    const int groups = (t.rows * t.cols + cus - 1) / cus;  // of the busiest CU
+    const float chain = (float)tiles_over(tiles_over(a.n / Q8_BLOCK, f.blocks), f.split);
     const float set = 0.3f * f.fixed;
     const int full = groups / f.resident, rest = groups % f.resident;
     float us = f.fixed + full * (set + chain * std::max(f.alone, f.resident * f.busy));
