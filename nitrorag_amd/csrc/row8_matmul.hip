@@ -505,22 +505,23 @@ constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
             }};
 }
 
-// Each timed over 340 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
-// or not) as graph replays, and fitted to within 4 to 8% of its own times.  The choice by
+// Each timed over 400 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
+// or not) as graph replays, and fitted to within 4 to 9% of its own times.  The choice by
 // these estimates takes 1.1% longer in the mean than the best of the forms each time; at
-// most 41%, 7.9 against 5.6 us, for a gated pair of 80 rows of 128.
+// most 34%, 8.0 against 5.9 us, for a gated pair of 1606 rows of 96.
 constexpr Form FORMS[] = {
-    split_form<16, 1, 1, 4, 5>(10, 2.25f, 0.314f, 0.294f),
-    split_form<16, 1, 1, 8, 4>(3, 2.15f, 0.064f, 0.584f),
-    split_form<16, 1, 2, 4, 4>(6, 2.40f, 0.632f, 0.514f),
-    split_form<16, 1, 2, 8, 4>(2, 2.18f, 0.221f, 1.047f),
-    split_form<16, 2, 2, 8, 4>(1, 2.41f, 0.026f, 1.244f),
-    split_form<32, 1, 1, 4, 4>(4, 2.84f, 0.587f, 0.564f),
-    split_form<32, 2, 2, 4, 2>(1, 5.45f, 1.546f, 0.069f),
-    gemm_form<1, 1, 2, 4>(4, 3.08f, 0.341f, 0.195f),
-    gemm_form<1, 2, 2, 3>(3, 3.80f, 0.514f, 0.342f),
-    gemm_form<2, 2, 1, 3>(2, 5.66f, 0.794f, 0.576f),
-    gemm_form<4, 2, 1, 2>(3, 8.90f, 1.377f, 1.050f),
+    split_form<16, 1, 1, 4, 5>(8, 2.24f, 0.312f, 0.281f),
+    split_form<16, 1, 1, 8, 4>(4, 2.13f, 0.554f, 0.584f),
+    split_form<16, 1, 2, 4, 4>(6, 2.36f, 0.661f, 0.517f),
+    split_form<16, 1, 2, 8, 4>(2, 2.22f, 0.058f, 1.040f),
+    split_form<16, 2, 2, 4, 4>(4, 2.65f, 0.900f, 0.647f),
+    split_form<16, 2, 2, 8, 4>(3, 2.34f, 0.092f, 1.368f),
+    split_form<32, 1, 1, 4, 4>(4, 2.81f, 0.576f, 0.566f),
+    split_form<32, 2, 2, 4, 2>(1, 4.98f, 1.584f, 0.038f),
+    gemm_form<1, 1, 2, 4>(3, 3.09f, 0.342f, 0.192f),
+    gemm_form<1, 2, 2, 3>(3, 3.75f, 0.507f, 0.341f),
+    gemm_form<2, 2, 1, 3>(3, 6.27f, 0.803f, 0.555f),
+    gemm_form<4, 2, 1, 2>(2, 8.45f, 1.441f, 1.043f),
 };
 
 // (A grid's threads count in 32 bits.)
