@@ -96,8 +96,12 @@ int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_
 int nitro_q8_weights_destroy(nitro_q8_weights* weights) {
     if (!weights) return NITRO_OK;
     return guarded([&] {
+        int now = 0;  // the launches to wait for are on the weights' device
+        const bool other = hipGetDevice(&now) == hipSuccess && now != weights->device;
+        if (other) (void)hipSetDevice(weights->device);
         (void)hipDeviceSynchronize();
         delete weights;
+        if (other) (void)hipSetDevice(now);
     });
 }
 
