@@ -263,11 +263,12 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
 // row l % 32).  Two blocks of x and of the weights lie in LDS, two buffers, a barrier for
 // each two.  x lies as four planes (a block's halves) of 16 bytes a row, so that lanes read
 // consecutive rows; the weights as in the tile layout, runs of 8 k.
-template <int MT, int NT, int DEPTH, int OCC, bool GATED>
+template <int MT, int NT, int STEP, int DEPTH, int OCC, bool GATED>
 __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles tiling) {
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
     constexpr int PLANE = BM * 16 + 32;  // (the planes' banks lie 32 bytes apart: a row's four runs are written together)
-    constexpr int XB = 4 * PLANE, WB = 2 * BN * 32, BUF = XB + WB + 2 * BN * 4;
+    constexpr int XB = 2 * STEP * PLANE, WB = STEP * BN * 32, BUF = XB + WB + STEP * BN * 4;
+    constexpr int XU = MT * STEP / 2, WU = NT * STEP / 2, SU = (STEP * BN + 255) / 256;  // units a thread
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF < 16384 ? 16384 : 2 * BUF];
     const int tid = threadIdx.x;
     auto xl = [&](int buf) __attribute__((always_inline)) { return lds + buf * BUF; };
@@ -288,48 +289,59 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
         const int at = GATED ? ct * (COLS / 16) + j / 4 * 2 + j % 2 : ct * (COLS / 16) + j;
         return a.w[GATED ? j / 2 % 2 : member] + (size_t)min(at, tiles - 1) * nb * Q8_TILE_BYTES;
     };
-    // Staging: x as MT units of 16 bytes a thread, weights NT, one scale (of 2 BN).
-    const int8_t* xp[MT];
-    int xk, xdst[MT];
-    xk = tid % 4 * 16;
+    // Staging: x and weights in units of 16 bytes, scales one by one.
+    constexpr bool EVEN = STEP * BN % 256 == 0;  // every thread has its scales
+    const int8_t* xp[XU];
+    int xdst[XU];
+    const int xk = tid % (2 * STEP) * 16;
 #pragma unroll
-    for (int u = 0; u < MT; u++) {
-        const int row = tid / 4 + 64 * u;
+    for (int u = 0; u < XU; u++) {
+        const int row = (tid + 256 * u) / (2 * STEP);
         xp[u] = a.codes + (size_t)min(b0 + row, a.rows - 1) * n;
-        xdst[u] = tid % 4 * PLANE + row * 16;
+        xdst[u] = tid % (2 * STEP) * PLANE + row * 16;
     }
-    const uint8_t* wp[NT];
-    int wblk[NT];
+    const uint8_t* wp[WU];
+    int wblk[WU];
 #pragma unroll
-    for (int u = 0; u < NT; u++) {
+    for (int u = 0; u < WU; u++) {
         const int e = tid + 256 * u;
         wblk[u] = e / (2 * BN);
         wp[u] = tile_at(e / 32 % (BN / 16)) + 64 + e % 32 * 16;
     }
-    const int sblk = tid / BN, srow = tid % BN;
-    const uint8_t* sp = tile_at(srow / 16) + 4 * (srow % 16);
+    const uint8_t* sp[SU];
+    int sblk[SU];
+#pragma unroll
+    for (int u = 0; u < SU; u++) {
+        const int e = tid + 256 * u;
+        sblk[u] = e / BN;
+        sp[u] = tile_at(e % BN / 16) + 4 * (e % 16);
+    }
 
     struct Stage {
-        i4 x[MT], w[NT];
-        float s;
+        i4 x[XU], w[WU];
+        float s[SU];
     };
     auto load = [&](Stage& S, int blk) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < MT; u++)
+        for (int u = 0; u < XU; u++)
             S.x[u] = *reinterpret_cast<const i4*>(xp[u] + min(blk * Q8_BLOCK + xk, n - 16));
 #pragma unroll
-        for (int u = 0; u < NT; u++)
+        for (int u = 0; u < WU; u++)
             S.w[u] = *reinterpret_cast<const i4*>(wp[u] + (size_t)min(blk + wblk[u], nb - 1) * Q8_TILE_BYTES);
-        if (2 * BN == 256 || tid < 2 * BN)
-            S.s = *reinterpret_cast<const float*>(sp + (size_t)min(blk + sblk, nb - 1) * Q8_TILE_BYTES);
+#pragma unroll
+        for (int u = 0; u < SU; u++)
+            if (EVEN || tid < STEP * BN)
+                S.s[u] = *reinterpret_cast<const float*>(sp[u] + (size_t)min(blk + sblk[u], nb - 1) * Q8_TILE_BYTES);
     };
     auto put = [&](const Stage& S, int buf, int blk) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < MT; u++) *reinterpret_cast<i4*>(xl(buf) + xdst[u]) = S.x[u];
+        for (int u = 0; u < XU; u++) *reinterpret_cast<i4*>(xl(buf) + xdst[u]) = S.x[u];
 #pragma unroll
-        for (int u = 0; u < NT; u++) *reinterpret_cast<i4*>(wl(buf) + (tid + 256 * u) * 16) = S.w[u];
+        for (int u = 0; u < WU; u++) *reinterpret_cast<i4*>(wl(buf) + (tid + 256 * u) * 16) = S.w[u];
         // (a block past the end repeats the last one, times 0)
-        if (2 * BN == 256 || tid < 2 * BN) sl(buf)[tid] = blk + sblk < nb ? S.s : 0.0f;
+#pragma unroll
+        for (int u = 0; u < SU; u++)
+            if (EVEN || tid < STEP * BN) sl(buf)[tid + 256 * u] = blk + sblk[u] < nb ? S.s[u] : 0.0f;
     };
 
     f16v acc[MT][NT];
@@ -349,22 +361,34 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
 #pragma unroll
         for (int i = 0; i < 16; i++) to[i] = fmaf(late_s, (float)late[i], to[i]);
     };
+    // A block's operands.  AHEAD: read while the block before is multiplied (larger tiles
+    // have no registers for it, and more to do meanwhile).
+    constexpr bool AHEAD = MT * NT <= 2;
+    struct Operands {
+        i4 x[MT], w[NT];
+        float s[NT];
+    };
+    auto read = [&](Operands& o, int buf, int h) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int j = wn * 2 * NT + 2 * t + lc / 16;
+            const uint8_t* p = wl(buf) + (h * (BN / 16) + j) * 512 + (2 * lh * 16 + lc % 16) * 8;
+            const int2 lo = *reinterpret_cast<const int2*>(p), hi = *reinterpret_cast<const int2*>(p + 128);
+            o.w[t] = i4{lo.x, lo.y, hi.x, hi.y};
+            o.s[t] = sl(buf)[h * BN + wn * 32 * NT + 32 * t + lc];
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+            o.x[m] = *reinterpret_cast<const i4*>(xl(buf) + (2 * h + lh) * PLANE + (wm * 32 * MT + 32 * m + lc) * 16);
+    };
     auto compute = [&](int buf) __attribute__((always_inline)) {
+        Operands o[AHEAD ? 2 : 1];
+        if constexpr (AHEAD) read(o[0], buf, 0);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            i4 x[MT], w[NT];
-            float s[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int j = wn * 2 * NT + 2 * t + lc / 16;
-                const uint8_t* p = wl(buf) + (h * (BN / 16) + j) * 512 + (2 * lh * 16 + lc % 16) * 8;
-                const int2 lo = *reinterpret_cast<const int2*>(p), hi = *reinterpret_cast<const int2*>(p + 128);
-                w[t] = i4{lo.x, lo.y, hi.x, hi.y};
-                s[t] = sl(buf)[h * BN + wn * 32 * NT + 32 * t + lc];
-            }
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-                x[m] = *reinterpret_cast<const i4*>(xl(buf) + (2 * h + lh) * PLANE + (wm * 32 * MT + 32 * m + lc) * 16);
+        for (int h = 0; h < STEP; h++) {
+            Operands& now = o[AHEAD ? h % 2 : 0];
+            if constexpr (!AHEAD) read(now, buf, h);
+            else if (h + 1 < STEP) read(o[(h + 1) % 2], buf, h + 1);
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -372,26 +396,26 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
                     i16 zero;
 #pragma unroll
                     for (int i = 0; i < 16; i++) zero[i] = 0;
-                    const i16 p = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[m], w[t], zero, 0, 0, 0);
+                    const i16 p = __builtin_amdgcn_mfma_i32_32x32x32_i8(now.x[m], now.w[t], zero, 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                     scale_in(m ? acc[m - 1][t] : t ? acc[MT - 1][t - 1] : acc[MT - 1][NT - 1]);
-                    late = p, late_s = s[t];
+                    late = p, late_s = now.s[t];
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
     };
-    const int steps = (nb + 1) / 2;
+    const int steps = (nb + STEP - 1) / STEP;
     auto step = [&](int i, Stage& S) __attribute__((always_inline)) {
         __syncthreads();  // step i is staged; the other buffer's readers are done
-        put(S, (i + 1) & 1, 2 * i + 2);
-        load(S, 2 * (i + 1 + DEPTH));
+        put(S, (i + 1) & 1, STEP * (i + 1));
+        load(S, STEP * (i + 1 + DEPTH));
         compute(i & 1);
     };
     Stage sa, sb;
     load(sa, 0);
-    if constexpr (DEPTH == 2) load(sb, 2);
+    if constexpr (DEPTH == 2) load(sb, STEP);
     put(sa, 0, 0);
-    load(sa, 2 * DEPTH);
+    load(sa, STEP * DEPTH);
     if constexpr (DEPTH == 1) {
 #pragma unroll 1
         for (int i = 0; i < steps; i++) step(i, sa);
@@ -490,38 +514,38 @@ constexpr Form split_form(int resident, float fixed, float alone, float busy) {
             }};
 }
 
-template <int MT, int NT, int DEPTH, int OCC>
+template <int MT, int NT, int STEP, int DEPTH, int OCC>
 constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
-    return {log2_of(64 * MT), log2_of(64 * NT), 1, 0, resident, fixed, alone, busy, NT == 2, 256,
+    return {log2_of(64 * MT), log2_of(64 * NT), log2_of(STEP), 0, resident, fixed, alone, busy, NT == 2, 256,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
                 const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(256);
                 if constexpr (NT == 2) {
                     if (a.gated) {
-                        hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, true>), grid, block, 0, stream, a, t);
+                        hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, STEP, DEPTH, OCC, true>), grid, block, 0, stream, a, t);
                         return;
                     }
                 }
-                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, DEPTH, OCC, false>), grid, block, 0, stream, a, t);
+                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, STEP, DEPTH, OCC, false>), grid, block, 0, stream, a, t);
             }};
 }
 
-// Each timed over 400 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
-// or not) as graph replays, and fitted to within 4 to 9% of its own times.  The choice by
-// these estimates takes 1.1% longer in the mean than the best of the forms each time; at
-// most 34%, 8.0 against 5.9 us, for a gated pair of 1606 rows of 96.
+// Each timed over 420 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
+// or not) as graph replays, and fitted to within 4 to 8% of its own times.  The choice by
+// these estimates takes 1.2% longer in the mean than the best of the forms each time; at
+// most 23%, 7.1 against 5.8 us, for a gated pair of 9588 rows of 32.
 constexpr Form FORMS[] = {
-    split_form<16, 1, 1, 4, 5>(8, 2.24f, 0.312f, 0.281f),
-    split_form<16, 1, 1, 8, 4>(4, 2.13f, 0.554f, 0.584f),
-    split_form<16, 1, 2, 4, 4>(6, 2.36f, 0.661f, 0.517f),
-    split_form<16, 1, 2, 8, 4>(2, 2.22f, 0.058f, 1.040f),
-    split_form<16, 2, 2, 4, 4>(4, 2.65f, 0.900f, 0.647f),
-    split_form<16, 2, 2, 8, 4>(3, 2.34f, 0.092f, 1.368f),
-    split_form<32, 1, 1, 4, 4>(4, 2.81f, 0.576f, 0.566f),
-    split_form<32, 2, 2, 4, 2>(1, 4.98f, 1.584f, 0.038f),
-    gemm_form<1, 1, 2, 4>(3, 3.09f, 0.342f, 0.192f),
-    gemm_form<1, 2, 2, 3>(3, 3.75f, 0.507f, 0.341f),
-    gemm_form<2, 2, 1, 3>(3, 6.27f, 0.803f, 0.555f),
-    gemm_form<4, 2, 1, 2>(2, 8.45f, 1.441f, 1.043f),
+    split_form<16, 1, 1, 4, 5>(8, 2.23f, 0.313f, 0.282f),
+    split_form<16, 1, 1, 8, 4>(4, 2.15f, 0.138f, 0.582f),
+    split_form<16, 1, 2, 4, 4>(6, 2.39f, 0.664f, 0.494f),
+    split_form<16, 1, 2, 8, 4>(3, 2.19f, 0.053f, 1.009f),
+    split_form<16, 2, 2, 4, 4>(4, 2.69f, 0.873f, 0.649f),
+    split_form<16, 2, 2, 8, 4>(2, 2.35f, 0.038f, 1.308f),
+    split_form<32, 1, 1, 4, 4>(4, 2.72f, 0.589f, 0.549f),
+    split_form<32, 2, 2, 4, 2>(1, 4.57f, 1.636f, 0.043f),
+    gemm_form<1, 1, 4, 2, 3>(2, 3.00f, 0.520f, 0.362f),
+    gemm_form<1, 2, 2, 2, 3>(2, 3.81f, 0.454f, 0.335f),
+    gemm_form<2, 2, 2, 1, 3>(2, 5.58f, 0.787f, 0.596f),
+    gemm_form<4, 2, 2, 1, 2>(2, 9.49f, 1.484f, 1.071f),
 };
 
 // (A grid's threads count in 32 bits.)
