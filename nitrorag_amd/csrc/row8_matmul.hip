@@ -21,14 +21,25 @@ typedef int i16 __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-// (NaN goes through all of them.)
+// exp and the quotient by the hardware's 2^x and 1 / x: a few roundings of the result, and
+// one of the exponent's argument times it, as expf and a division have.  (NaN goes through
+// all of the activations; a quotient by an infinity is 0.)
+__device__ __forceinline__ float logistic_of(float x, float t) {  // x / (1 + 2^t)
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+}
+__device__ __forceinline__ float relu(float x) { return x < 0.0f ? 0.0f : x; }
+__device__ __forceinline__ float silu(float x) { return logistic_of(x, x * -1.4426950408889634f); }
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(x * -0.70710678118654752f); }
+// 0.5 x (1 + tanh(u)) = x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+__device__ __forceinline__ float gelu_tanh(float x) {
+    return logistic_of(x, x * fmaf(x * x, -0.10294324f, -2.3022082f));
+}
 __device__ __forceinline__ float activate(float x, int activation) {
     switch (activation) {
-        case NITRO_ACT_RELU: return x < 0.0f ? 0.0f : x;
-        case NITRO_ACT_SILU: return x / (1.0f + expf(-x));
-        case NITRO_ACT_GELU: return 0.5f * x * erfcf(x * -0.70710678118654752f);
-        // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-        case NITRO_ACT_GELU_TANH: return x / (1.0f + expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+        case NITRO_ACT_RELU: return relu(x);
+        case NITRO_ACT_SILU: return silu(x);
+        case NITRO_ACT_GELU: return gelu(x);
+        case NITRO_ACT_GELU_TANH: return gelu_tanh(x);
         default: return x;
     }
 }
@@ -449,14 +460,31 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
             const float bias = a.bias ? a.bias[near] : 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) y[i] = acc[m][t][i] * xs[i] + bias;
-            if (a.activation) {
-                // (through LDS: one copy of the functions, not 16 MT NT)
+            switch (a.activation) {
+                case NITRO_ACT_RELU:
 #pragma unroll
-                for (int i = 0; i < 16; i++) mine[64 * i] = y[i];
+                    for (int i = 0; i < 16; i++) y[i] = relu(y[i]);
+                    break;
+                case NITRO_ACT_SILU:
+#pragma unroll
+                    for (int i = 0; i < 16; i++) y[i] = silu(y[i]);
+                    break;
+                case NITRO_ACT_GELU_TANH:
+#pragma unroll
+                    for (int i = 0; i < 16; i++) y[i] = gelu_tanh(y[i]);
+                    break;
+                case NITRO_ACT_GELU:  // (through LDS: four copies of the function, not 16 MT NT)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) mine[64 * i] = y[i];
 #pragma unroll 1
-                for (int i = 0; i < 16; i++) mine[64 * i] = activate(mine[64 * i], a.activation);
+                    for (int i = 0; i < 16; i += 4) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) y[i] = mine[64 * i];
+                        for (int j = 0; j < 4; j++) mine[64 * (i + j)] = gelu(mine[64 * (i + j)]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) y[i] = mine[64 * i];
+                    break;
+                default: break;
             }
             if constexpr (GATED) {
                 const float second = a.bias ? a.bias[d + near] : 0.0f;
