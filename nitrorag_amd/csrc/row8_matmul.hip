@@ -23,13 +23,31 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 // exp and the quotient by the hardware's 2^x and 1 / x: a few roundings of the result, and
 // one of the exponent's argument times it, as expf and a division have.  (NaN goes through
-// all of the activations; a quotient by an infinity is 0.)
+// all of the activations; a quotient by an infinity is 0.)  They are a tile's whole time where
+// n is small: 8192 rows of 768 x 2048 with gelu 49 us, 63 through erfcf; 4637 rows of 32 x
+// 5522 31 us, with gelu_tanh 34, gelu 38, and 51 and 52 through expf, erfcf and divisions.
 __device__ __forceinline__ float logistic_of(float x, float t) {  // x / (1 + 2^t)
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
 __device__ __forceinline__ float relu(float x) { return x < 0.0f ? 0.0f : x; }
 __device__ __forceinline__ float silu(float x) { return logistic_of(x, x * -1.4426950408889634f); }
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(x * -0.70710678118654752f); }
+// x Phi(x), with Phi(-|x|) = exp(-x^2 / 2) t Q(t), t = 1 / (1 + 0.35 |x|): Q is the polynomial
+// of degree 8 with the least relative error for |x| <= 14.5 (3.2e-8, half a rounding), a
+// weighted least-squares fit in 64 bits; in fp32 at most 7 roundings of 1 + x^2.
+__device__ __forceinline__ float gelu(float x) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(x), 1.0f));
+    float q = -0.029157886f;
+    q = fmaf(q, t, 0.14403091f);
+    q = fmaf(q, t, -0.25583899f);
+    q = fmaf(q, t, 0.1593197f);
+    q = fmaf(q, t, -0.023212353f);
+    q = fmaf(q, t, 0.1055525f);
+    q = fmaf(q, t, 0.11982129f);
+    q = fmaf(q, t, 0.13986352f);
+    q = fmaf(q, t, 0.1396213f);
+    const float below = q * t * __builtin_amdgcn_exp2f(x * x * -0.72134752f);
+    return x * (x < 0.0f ? below : 1.0f - below);
+}
 // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
 __device__ __forceinline__ float gelu_tanh(float x) {
     return logistic_of(x, x * fmaf(x * x, -0.10294324f, -2.3022082f));
@@ -86,9 +104,10 @@ __device__ __forceinline__ Place place_of(const Tiles& t) {
 //    wave's own, and back in operand order.  (Loaded in operand order, 16 rows to a load,
 //    every eight bytes were a lookup of their own in the vector cache: 128 rows of 4096 x
 //    4096 23 us, 14 us so; 16 rows of 4096 x 11008 17 us, 11 us so.)
-// Bound by the weights' bytes for few rows (8 rows of a gated 4096 x 11008 pair 20.5 us,
-// 4.9 TB/s, where loads alone take 18 us), by latency for small matrices (3.3 us at 768 x
-// 2048), and by the vector unit, at half its rate, towards 512 rows.
+// Bound by the weights' bytes for few rows (8 rows of a gated 4096 x 11008 pair 23 us, 4.4
+// TB/s, where the loads alone take 18), by latency for small matrices (16 rows of 768 x 2048
+// 3.1 us; one of 4096 x 4096 6.0, 3.1 TB/s), and from 32 rows on by its loads' latency and
+// the vector unit together (64 rows of the pair 36 us, 128 of 4096 x 4096 13 us).
 template <int U>
 struct Tile;
 template <>
@@ -271,16 +290,24 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
 // --------------------------------------------------------------- many rows
 // A workgroup of 4 waves owns 64 MT batch rows x 64 NT weight rows (wave: half of each, as
 // MT x NT tiles of v_mfma_i32_32x32x32_i8: lane l holds 16 k, half l / 32 of a block, of
-// row l % 32).  Two blocks of x and of the weights lie in LDS, two buffers, a barrier for
-// each two.  x lies as four planes (a block's halves) of 16 bytes a row, so that lanes read
-// consecutive rows; the weights as in the tile layout, runs of 8 k.
+// row l % 32).  STEP blocks of x and of the weights lie in LDS, in two buffers with a barrier
+// for each, and are loaded DEPTH steps before they are put there.  x lies as 2 STEP planes
+// (the blocks' halves) of 16 bytes a row, so that lanes read consecutive rows; the weights as
+// in the tile layout, runs of 8 k.
+// Bound by the vector unit: a product's 16 sums a lane take 16 conversions and 16 fma, 64 + 64
+// cycles of a SIMD, next to the matrix instruction's 32.  4096 rows of 11008 x 4096: 390 to 410
+// us, 900 to 950 TFLOP/s, with the vector unit busy for 89% of the cycles; 1024 rows of a gated
+// 4096 x 11008 pair 215 to 230 us, 800 to 860.  (The codes as halves, whose sums need no
+// conversion, took 387 us where this took 374 in the same run: two matrix instructions a block,
+// and a lower clock.)  512 rows of 4096 x 4096, 32 us, 540 TFLOP/s: few workgroups a CU, and
+// each waits for its loads.
 template <int MT, int NT, int STEP, int DEPTH, int OCC, bool GATED>
 __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles tiling) {
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
     constexpr int PLANE = BM * 16 + 32;  // (the planes' banks lie 32 bytes apart: a row's four runs are written together)
     constexpr int XB = 2 * STEP * PLANE, WB = STEP * BN * 32, BUF = XB + WB + STEP * BN * 4;
     constexpr int XU = MT * STEP / 2, WU = NT * STEP / 2, SU = (STEP * BN + 255) / 256;  // units a thread
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF < 16384 ? 16384 : 2 * BUF];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
     const int tid = threadIdx.x;
     auto xl = [&](int buf) __attribute__((always_inline)) { return lds + buf * BUF; };
     auto wl = [&](int buf) __attribute__((always_inline)) { return lds + buf * BUF + XB; };
@@ -441,8 +468,6 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
     scale_in(acc[MT - 1][NT - 1]);
 
     // Lane l holds row 8 * (i / 4) + 4 * (l / 32) + i % 4, column l % 32 of a tile.
-    __syncthreads();
-    float* const mine = reinterpret_cast<float*>(lds) + wave * 1024 + lane;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int row0 = b0 + (wm * MT + m) * 32 + 4 * lh;
@@ -473,16 +498,12 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
 #pragma unroll
                     for (int i = 0; i < 16; i++) y[i] = gelu_tanh(y[i]);
                     break;
-                case NITRO_ACT_GELU:  // (through LDS: four copies of the function, not 16 MT NT)
+                case NITRO_ACT_GELU:
 #pragma unroll
-                    for (int i = 0; i < 16; i++) mine[64 * i] = y[i];
-#pragma unroll 1
-                    for (int i = 0; i < 16; i += 4) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) mine[64 * (i + j)] = gelu(mine[64 * (i + j)]);
+                    for (int i = 0; i < 16; i++) {
+                        y[i] = gelu(y[i]);
+                        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time: registers)
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) y[i] = mine[64 * i];
                     break;
                 default: break;
             }
@@ -519,7 +540,7 @@ int col_tiles_of(const Row8Matmul& a, int log2) {
 // do, at most `resident` at once; `fixed` us for a launch, a third of it again for every
 // set of resident workgroups.
 struct Form {
-    int rows, cols, blocks, split;  // as powers of two (a call looks at every form)
+    int rows, cols, blocks, split;  // their logarithms to base 2 (a call looks at every form)
     int resident;
     float fixed, alone, busy;
     bool gates;  // its column tiles are even in number

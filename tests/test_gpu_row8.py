@@ -218,6 +218,26 @@ def test_activations(rows, d, activation, gated):
           forms.product([(q, s) for _, q, s in mats], codes, scales, bias, None, activation), activation)
 
 
+@pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [1, 40, 1100])
+def test_activations_of_any_number(rows, activation):
+    """Rows of zeros leave the bias alone in front of the activation."""
+    row = np.array([0, 1e-38, 1e-30, 1e-4, 1, 5, 9, 13, 20, 60, 88, 89, 100, 104, 200, 1e4, 1e10, 1e19, 1e20, 1e30, 3e38, np.inf], np.float32)
+    bias = np.tile(np.concatenate([row, -row, [np.nan]]).astype(np.float32), 90 if rows > 1000 else 2)
+    w, q, s = forms.matrix(np.random.default_rng(rows), len(bias), 64)
+    codes, scales = np.zeros((rows, 64), np.int8), np.zeros(rows, np.float32)
+    got = on_gpu([(w, q, s)], codes, scales, bias=bias, activation=activation)
+    with np.errstate(all="ignore"):
+        want, bound = forms.product([(q, s)], codes[:1], scales[:1], bias, None, activation)
+        finite = np.isfinite(want[0])
+        over = np.abs(got[:, finite] - want[0, finite]) > bound[0, finite]
+    assert not over.any(), (got[:, finite][over][:4], np.broadcast_to(bias[finite], over.shape)[over][:4])
+    if activation != "relu":  # from 20 on exp(-p) is nothing next to 1: the roundings alone
+        large = finite & (bias >= 20)
+        assert (np.abs(got[:, large] - bias[large].astype(np.float64)) <= 16 * forms.EPS32 * bias[large].astype(np.float64)).all()
+    np.testing.assert_array_equal(got[:, ~finite], np.broadcast_to(want[0, ~finite], (rows, (~finite).sum())))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 100, 1100])
 def test_residual_in_place_and_rows_behind(rows):
     import torch
