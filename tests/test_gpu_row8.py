@@ -327,6 +327,41 @@ def test_matrix_past_4_gib_of_codes():
     assert (x[-1] - last.float()).abs().max().item() <= 0.5001 * top / 127 and (x[0] == 0).all()
 
 
+def test_more_rows_than_a_launch_takes():
+    """Rows past 2^20 (products), 2^21 (norm, quantising) and 2^25 (reading) in one call."""
+    import torch
+
+    import nitrorag_amd as na
+
+    rng = np.random.default_rng(9)
+    rows, n = (1 << 25) + 9, 1
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    codes, scales = held_on_gpu(lambda c, s: na.row8_quantize(to_gpu(x), c, s), rows, n)
+    np.testing.assert_array_equal(codes, 127 * np.sign(x))
+    np.testing.assert_array_equal(scales, np.abs(x[:, 0]) / np.float32(127))
+    back = torch.empty((rows, n), device="cuda")
+    na.row8_read(to_gpu(codes), to_gpu(scales), back)
+    np.testing.assert_array_equal(back.cpu().numpy(), codes * scales[:, None])
+
+    rows, n = (1 << 21) + 5, 3
+    x, add = (rng.standard_normal((rows, n)).astype(np.float32) for _ in range(2))
+    weight, h = rng.uniform(0.5, 1.5, n).astype(np.float32), torch.empty((rows, n), device="cuda")
+    codes, scales = held_on_gpu(lambda c, s: na.rms_norm_row8(to_gpu(x), to_gpu(weight), c, s, residual=to_gpu(add), sum=h), rows, n)
+    want, y = forms.normed(x, weight, add)
+    np.testing.assert_array_equal(h.cpu().numpy(), want)
+    top = np.abs(y).max(1)
+    np.testing.assert_array_equal(scales, top / np.float32(127))
+    np.testing.assert_array_equal(codes, np.rint(y.astype(np.float64) * (np.float32(127) / top)[:, None]))
+
+    rows, n, d = (1 << 20) + 77, 32, 17
+    codes, scales = rng.integers(-127, 128, (rows, n)).astype(np.int8), rng.uniform(0.5, 1.5, rows).astype(np.float32)
+    residual, mats = rng.standard_normal((rows, d)).astype(np.float32), [forms.matrix(rng, d, n) for _ in range(2)]
+    for pair in (mats[:1], mats):
+        out = to_gpu(residual)
+        na.Q8Weights(*(to_gpu(m[0]) for m in pair)).matmul(to_gpu(codes), to_gpu(scales), out, residual=out, activation="relu")
+        check(out.cpu().numpy(), forms.product([m[1:] for m in pair], codes, scales, None, residual, "relu"), f"{len(pair)}")
+
+
 # ----------------------------------------------------- together, streams, graphs
 
 class Layer:
