@@ -543,54 +543,53 @@ struct Form {
     int rows, cols, blocks, split;  // their logarithms to base 2 (a call looks at every form)
     int resident;
     float fixed, alone, busy;
-    bool gates;  // its column tiles are even in number
+    bool single, pairs;  // takes matrices one by one; takes gated pairs
     int threads;
     void (*launch)(const Row8Matmul&, const Tiles&, hipStream_t);
 };
 
-template <int U, int RT, int CT, int W, int OCC>
+// (A pair needs column tiles that are even in number.)
+template <int U, int RT, int CT, int W, int OCC, bool SINGLE = true>
 constexpr Form split_form(int resident, float fixed, float alone, float busy) {
-    return {log2_of(U * RT), log2_of(U * CT), 2, log2_of(W), resident, fixed, alone, busy, CT % 2 == 0, 64 * W,
+    return {log2_of(U * RT), log2_of(U * CT), 2, log2_of(W), resident, fixed, alone, busy, SINGLE, CT % 2 == 0, 64 * W,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
                 const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(64 * W);
-                if constexpr (CT % 2 == 0) {
-                    if (a.gated) {
+                if constexpr (CT % 2 == 0)
+                    if (a.gated)
                         hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, true>), grid, block, 0, stream, a, t);
-                        return;
-                    }
-                }
-                hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, block, 0, stream, a, t);
+                if constexpr (SINGLE)
+                    if (!a.gated)
+                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, block, 0, stream, a, t);
             }};
 }
 
 template <int MT, int NT, int STEP, int DEPTH, int OCC>
 constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
-    return {log2_of(64 * MT), log2_of(64 * NT), log2_of(STEP), 0, resident, fixed, alone, busy, NT == 2, 256,
+    return {log2_of(64 * MT), log2_of(64 * NT), log2_of(STEP), 0, resident, fixed, alone, busy, true, NT == 2, 256,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
                 const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(256);
-                if constexpr (NT == 2) {
-                    if (a.gated) {
+                if constexpr (NT == 2)
+                    if (a.gated)
                         hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, STEP, DEPTH, OCC, true>), grid, block, 0, stream, a, t);
-                        return;
-                    }
-                }
-                hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, STEP, DEPTH, OCC, false>), grid, block, 0, stream, a, t);
+                if (!a.gated)
+                    hipLaunchKernelGGL((row8_gemm_kernel<MT, NT, STEP, DEPTH, OCC, false>), grid, block, 0, stream, a, t);
             }};
 }
 
 // Each timed over 420 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
 // or not) as graph replays, and fitted to within 4 to 8% of its own times.  The choice by
 // these estimates takes 1.2% longer in the mean than the best of the forms each time; at
-// most 23%, 7.1 against 5.8 us, for a gated pair of 9588 rows of 32.
+// most 23%, 7.1 against 5.8 us, for a gated pair of 9588 rows of 32.  (Two of the forms are the
+// least only for pairs.)
 constexpr Form FORMS[] = {
     split_form<16, 1, 1, 4, 5>(8, 2.23f, 0.313f, 0.282f),
     split_form<16, 1, 1, 8, 4>(4, 2.15f, 0.138f, 0.582f),
     split_form<16, 1, 2, 4, 4>(6, 2.39f, 0.664f, 0.494f),
     split_form<16, 1, 2, 8, 4>(3, 2.19f, 0.053f, 1.009f),
-    split_form<16, 2, 2, 4, 4>(4, 2.69f, 0.873f, 0.649f),
+    split_form<16, 2, 2, 4, 4, false>(4, 2.69f, 0.873f, 0.649f),
     split_form<16, 2, 2, 8, 4>(2, 2.35f, 0.038f, 1.308f),
     split_form<32, 1, 1, 4, 4>(4, 2.72f, 0.589f, 0.549f),
-    split_form<32, 2, 2, 4, 2>(1, 4.57f, 1.636f, 0.043f),
+    split_form<32, 2, 2, 4, 2, false>(1, 4.57f, 1.636f, 0.043f),
     gemm_form<1, 1, 4, 2, 3>(2, 3.00f, 0.520f, 0.362f),
     gemm_form<1, 2, 2, 2, 3>(2, 3.81f, 0.454f, 0.335f),
     gemm_form<2, 2, 2, 1, 3>(2, 5.58f, 0.787f, 0.596f),
@@ -604,7 +603,7 @@ bool tiles_of(const Form& f, const Row8Matmul& a, Tiles& t) {
     // codes against weights, as rows of n (a weight has 1.125 bytes)
     const float x = (float)t.rows * (float)(1 << f.rows), w = 1.125f * (float)t.cols * (float)(1 << f.cols);
     t.by_columns = x + w / 8 < x / 8 + w;
-    return (f.gates || !a.gated) && (int64_t)t.rows * t.cols * f.threads < (1ll << 32);
+    return (a.gated ? f.pairs : f.single) && (int64_t)t.rows * t.cols * f.threads < (1ll << 32);
 }
 
 float estimate(const Form& f, const Row8Matmul& a, const Tiles& t, int cus) {
