@@ -106,7 +106,7 @@ __device__ __forceinline__ Place place_of(const Tiles& t) {
 //    4096 23 us, 14 us so; 16 rows of 4096 x 11008 17 us, 11 us so.)
 // Bound by the weights' bytes for few rows (8 rows of a gated 4096 x 11008 pair 23 us, 4.4
 // TB/s, where the loads alone take 18), by latency for small matrices (16 rows of 768 x 2048
-// 3.1 us; one of 4096 x 4096 6.0, 3.1 TB/s), and from 32 rows on by its loads' latency and
+// 3.1 us; one of 4096 x 4096 5.7, 3.3 TB/s), and from 32 rows on by its loads' latency and
 // the vector unit together (64 rows of the pair 36 us, 128 of 4096 x 4096 13 us).
 template <int U>
 struct Tile;
@@ -157,13 +157,16 @@ struct Tile<32> {
     static __device__ __forceinline__ int lane_at(int row, int col) { return row / 4 % 2 * 32 + col; }
 };
 
-template <int U, int RT, int CT, int W, int OCC, bool GATED>
+// X: rows of x that are loaded, all of the tile's or 8 (for up to 8 rows; the tile's others are
+// the same again and go nowhere: one row of 4096 x 11008 10.1 us, 10.5 with all 16 loaded; 8 rows
+// of 11008 x 4096 10.5, 11.1).
+template <int U, int RT, int CT, int W, int OCC, int X, bool GATED>
 __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, Tiles tiling) {
     typedef Tile<U> T;
     constexpr int ROWS = U * RT, COLS = U * CT / (GATED ? 2 : 1);  // of the output
     constexpr int ROUND = 4, PITCH = ROUND * Q8_BLOCK + 16;  // blocks a round; bytes of a row in LDS
-    constexpr int LOADS = ROWS / 8;                          // of 8 rows of x
-    constexpr int PART = RT * CT * T::SUMS * 64, XBYTES = W * ROWS * PITCH, SBYTES = W * PART * 4;
+    constexpr int LOADS = X / 8;                             // of 8 rows of x
+    constexpr int PART = RT * CT * T::SUMS * 64, XBYTES = W * X * PITCH, SBYTES = W * PART * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[XBYTES > SBYTES ? XBYTES : SBYTES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Place place = place_of(tiling);
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
     const int xk = lane % 8 * 16;
 #pragma unroll
     for (int r = 0; r < LOADS; r++) x[r] = a.codes + (size_t)min(b0 + 8 * r + lane / 8, a.rows - 1) * n;
-    int8_t* const mine = reinterpret_cast<int8_t*>(lds) + wave * ROWS * PITCH;
+    int8_t* const mine = reinterpret_cast<int8_t*>(lds) + wave * X * PITCH;
 
     typename T::Sums acc[RT][CT];
 #pragma unroll
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
         for (int u = 0; u < ROUND; u++) {
             typename T::Operand xq[RT];
 #pragma unroll
-            for (int r = 0; r < RT; r++) xq[r] = T::x(mine + (U * r + (lane & T::MASK)) * PITCH + u * Q8_BLOCK, lane);
+            for (int r = 0; r < RT; r++) xq[r] = T::x(mine + (U * r + (lane & T::MASK)) % X * PITCH + u * Q8_BLOCK, lane);
 #pragma unroll
             for (int t = 0; t < CT; t++) {
                 const float s = round * ROUND + u < nb ? R.s[u][t] : 0.0f;
@@ -548,18 +551,26 @@ struct Form {
     void (*launch)(const Row8Matmul&, const Tiles&, hipStream_t);
 };
 
+template <int U, int RT, int CT, int W, int OCC, bool GATED>
+void launch_split(const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
+    const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(64 * W);
+    if constexpr (U * RT == 16)
+        if (a.rows <= 8) {
+            hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, 8, GATED>), grid, block, 0, stream, a, t);
+            return;
+        }
+    hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, U * RT, GATED>), grid, block, 0, stream, a, t);
+}
+
 // (A pair needs column tiles that are even in number.)
 template <int U, int RT, int CT, int W, int OCC, bool SINGLE = true>
 constexpr Form split_form(int resident, float fixed, float alone, float busy) {
     return {log2_of(U * RT), log2_of(U * CT), 2, log2_of(W), resident, fixed, alone, busy, SINGLE, CT % 2 == 0, 64 * W,
             [](const Row8Matmul& a, const Tiles& t, hipStream_t stream) {
-                const dim3 grid((unsigned)t.rows * (unsigned)t.cols), block(64 * W);
                 if constexpr (CT % 2 == 0)
-                    if (a.gated)
-                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, true>), grid, block, 0, stream, a, t);
+                    if (a.gated) launch_split<U, RT, CT, W, OCC, true>(a, t, stream);
                 if constexpr (SINGLE)
-                    if (!a.gated)
-                        hipLaunchKernelGGL((row8_split_kernel<U, RT, CT, W, OCC, false>), grid, block, 0, stream, a, t);
+                    if (!a.gated) launch_split<U, RT, CT, W, OCC, false>(a, t, stream);
             }};
 }
 
