@@ -2,8 +2,8 @@
 // addition that come before in a model's layer (src/model_q8.cpp:128-140).
 //
 // Bound by bytes, 5 or 9 (with a residual and its sum 13) an entry: 8192 rows of 4096 with
-// residual and sum 84 us (5.2 TB/s, what a copy has), held only 31 us, read back 34 us; one
-// row of 4096 4.2, 2.4 and 2.4 us: latency (launch, loads, two joins over the row).
+// residual and sum 82 us (5.3 TB/s, what a copy has), held only 31 us, read back 34 us; one
+// row of 4096 3.6, 2.3 and 2.4 us: latency (launch, loads, two joins over the row).
 //
 // Mathematics.  h = fp32(x + residual), y = fp32(h * weight / sqrt(mean(h^2) + eps)).
 // The mean, its root and the products are taken in 64 bits and y is rounded once:
@@ -32,12 +32,44 @@ __device__ __forceinline__ void store4(int8_t* row, int at, uint32_t codes) { *r
 
 __device__ __forceinline__ double joined(double a, double b) { return a + b; }
 __device__ __forceinline__ uint32_t joined(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// x joined with another lane's, by a data-parallel move; with the next 16 lanes', 32 lanes'.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double moved(double x) {
+    return __hiloint2double((int)moved<CTRL>((uint32_t)__double2hiint(x)), (int)moved<CTRL>((uint32_t)__double2loint(x)));
+}
+__device__ __forceinline__ uint32_t over_16(uint32_t x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return joined((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ uint32_t over_32(uint32_t x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return joined((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ double over_16(double x) {
+    const uint32_t h = (uint32_t)__double2hiint(x), l = (uint32_t)__double2loint(x);
+    const auto hi = __builtin_amdgcn_permlane16_swap(h, h, false, false), lo = __builtin_amdgcn_permlane16_swap(l, l, false, false);
+    return joined(__hiloint2double((int)hi[0], (int)lo[0]), __hiloint2double((int)hi[1], (int)lo[1]));
+}
+__device__ __forceinline__ double over_32(double x) {
+    const uint32_t h = (uint32_t)__double2hiint(x), l = (uint32_t)__double2loint(x);
+    const auto hi = __builtin_amdgcn_permlane32_swap(h, h, false, false), lo = __builtin_amdgcn_permlane32_swap(l, l, false, false);
+    return joined(__hiloint2double((int)hi[0], (int)lo[0]), __hiloint2double((int)hi[1], (int)lo[1]));
+}
 // Sums (double) or the largest (bits) over the T lanes of a row, in the same order every
-// time; all of them get the result.
+// time; all of them get the result.  (Moves between lanes take a few cycles, through LDS a
+// hundred each: with them, and the weights loaded with x, one row of 4096 takes 3.75 us, 4.25
+// before; held only 2.3, 2.45.)
 template <int T, class V>
 __device__ __forceinline__ V over_row(V x, V* parts) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = joined(x, (V)__shfl_xor(x, m));
+    x = joined(x, moved<0xB1>(x));   // quad_perm [1,0,3,2]
+    x = joined(x, moved<0x4E>(x));   // quad_perm [2,3,0,1]
+    x = joined(x, moved<0x141>(x));  // row_half_mirror: the other four of eight
+    x = joined(x, moved<0x140>(x));  // row_mirror: the other eight of sixteen
+    x = over_32(over_16(x));
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = x;
         __syncthreads();
@@ -91,6 +123,7 @@ __device__ __forceinline__ uint32_t codes_of(f32x4 y, float inv) {
 template <int T, int V, bool NORM>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a) {
     constexpr int ROWS = T < 256 ? 256 / T : 1;
+    constexpr bool EARLY = T < 1024;  // the weights come with x (more lanes have no registers for it)
     __shared__ double sums[T / 64];
     __shared__ uint32_t tops[T / 64];
     const int lane = threadIdx.x % T, n = a.n, end = n & ~3;
@@ -109,6 +142,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a
     }
     if (last) tail = x[end + lane];
     if constexpr (NORM) {
+        f32x4 w[EARLY ? V : 1];
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                w[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (4 * (lane + i * T) < end) w[i] = load4(a.weight, 4 * (lane + i * T));
+            }
+        }
         if (a.residual) {
 #pragma unroll
             for (int i = 0; i < V; i++)
@@ -121,16 +162,17 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a
                 if (4 * (lane + i * T) < end) store4(a.sum + at, 4 * (lane + i * T), h[i]);
             if (last) a.sum[at + end + lane] = tail;
         }
+        const double each = 1.0 / n;  // (while x comes; a quotient behind the sum cost 0.1 us)
         double s = (double)tail * (double)tail;
 #pragma unroll
         for (int i = 0; i < V; i++) {
             s = squares(h[i], s);
             if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (64-bit values of four groups at a time)
         }
-        const double r = 1.0 / sqrt(over_row<T>(s, sums) / n + a.eps);
+        const double r = rsqrt(over_row<T>(s, sums) * each + a.eps);
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            if (4 * (lane + i * T) < end) h[i] = normed(h[i], load4(a.weight, 4 * (lane + i * T)), r);
+            if (4 * (lane + i * T) < end) h[i] = normed(h[i], EARLY ? w[EARLY ? i : 0] : load4(a.weight, 4 * (lane + i * T)), r);
             if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
         if (last) tail = normed(tail, a.weight[end + lane], r);
@@ -164,6 +206,7 @@ __global__ __launch_bounds__(1024) void row8_long_kernel(Row8Norm a) {
     if constexpr (NORM) {
         if (last && residual) tail += residual[end + lane];
         if (last && a.sum) a.sum[at + end + lane] = tail;
+        const double each = 1.0 / n;
         double s = (double)tail * (double)tail;
 #pragma unroll 4
         for (int v = 4 * lane; v < end; v += 4 * T) {
@@ -173,7 +216,7 @@ __global__ __launch_bounds__(1024) void row8_long_kernel(Row8Norm a) {
             s = squares(h, s);
         }
         if (a.sum) x = a.sum + at, residual = nullptr;  // (it may lie over either; a lane reads what it wrote)
-        r = 1.0 / sqrt(over_row<T>(s, sums) / n + a.eps);
+        r = rsqrt(over_row<T>(s, sums) * each + a.eps);
         if (last) tail = normed(tail, a.weight[end + lane], r);
     }
     uint32_t top = largest(tail, 0);
