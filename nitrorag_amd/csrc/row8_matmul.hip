@@ -307,8 +307,8 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
 // (the blocks' halves) of 16 bytes a row, so that lanes read consecutive rows; the weights as
 // in the tile layout, runs of 8 k.
 // Bound by the vector unit: a product's 16 sums a lane take 16 conversions and 16 fma, 64 + 64
-// cycles of a SIMD, next to the matrix instruction's 32.  4096 rows of 11008 x 4096: 390 to 420
-// us, 880 to 950 TFLOP/s, with the vector unit busy for 86 to 89% of the cycles; 1024 rows of a gated
+// cycles of a SIMD, next to the matrix instruction's 32.  4096 rows of 11008 x 4096: 390 to 425
+// us, 870 to 950 TFLOP/s, with the vector unit busy for 86 to 89% of the cycles; 1024 rows of a gated
 // 4096 x 11008 pair 215 to 230 us, 800 to 860.  (The codes as halves, whose sums need no
 // conversion, took 387 us where this took 374 in the same run: two matrix instructions a block,
 // and a lower clock.)  512 rows of 4096 x 4096, 32 us, 540 TFLOP/s: few workgroups a CU, and
