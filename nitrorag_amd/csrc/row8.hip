@@ -189,8 +189,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row8_norm_kernel(Row8Norm a
     if (last) codes[end + lane] = (int8_t)code_of(tail, inv);
 }
 
-// Rows of any width, a workgroup each, read again for every use.
-template <bool NORM>
+// Rows past the registers of a workgroup, a workgroup each, read again for every use: the sum
+// of squares, y and its maximum, the codes.  With V > 0 (rows up to 4096 V entries, normed) y
+// stays in V groups of registers: one row of 65536 with residual and sum 14.7 us, 18.2 without;
+// 2000 rows of 20000 112 us, 124.
+template <bool NORM, int V>
 __global__ __launch_bounds__(1024) void row8_long_kernel(Row8Norm a) {
     constexpr int T = 1024;
     __shared__ double sums[T / 64];
@@ -219,18 +222,34 @@ __global__ __launch_bounds__(1024) void row8_long_kernel(Row8Norm a) {
         r = rsqrt(over_row<T>(s, sums) * each + a.eps);
         if (last) tail = normed(tail, a.weight[end + lane], r);
     }
+    auto value = [&](int v) __attribute__((always_inline)) {
+        f32x4 h = load4(x, v);
+        if (residual) h += load4(residual, v);
+        if constexpr (NORM) h = normed(h, load4(a.weight, v), r);
+        return h;
+    };
     uint32_t top = largest(tail, 0);
-    for (int pass = 0; pass < 2; pass++) {
+    if constexpr (V > 0) {
+        f32x4 y[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (4 * (lane + i * T) < end) y[i] = value(4 * (lane + i * T));
+            top = largest(y[i], top);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (64-bit values of four groups at a time)
+        }
+        top = over_row<T>(top, tops);
+        const float inv = inverse_of(top);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (4 * (lane + i * T) < end) store4(codes, 4 * (lane + i * T), codes_of(y[i], inv));
+    } else {
+#pragma unroll 4
+        for (int v = 4 * lane; v < end; v += 4 * T) top = largest(value(v), top);
+        top = over_row<T>(top, tops);
         const float inv = inverse_of(top);
 #pragma unroll 4
-        for (int v = 4 * lane; v < end; v += 4 * T) {
-            f32x4 h = load4(x, v);
-            if (residual) h += load4(residual, v);
-            if constexpr (NORM) h = normed(h, load4(a.weight, v), r);
-            if (pass == 0) top = largest(h, top);
-            else store4(codes, v, codes_of(h, inv));
-        }
-        if (pass == 0) top = over_row<T>(top, tops);
+        for (int v = 4 * lane; v < end; v += 4 * T) store4(codes, v, codes_of(value(v), inv));
     }
     if (last) codes[end + lane] = (int8_t)code_of(tail, inverse_of(top));
     if (lane == 0) a.scales[blockIdx.x] = scale_of(top);
@@ -274,13 +293,26 @@ void launch_rows(const Row8Norm& a, hipStream_t stream) {
         hipLaunchKernelGGL((row8_norm_kernel<T, V, false>), grid, block, 0, stream, a);
 }
 
+template <bool NORM>
+void launch_long(const Row8Norm& a, hipStream_t stream) {
+    const dim3 grid(a.rows), block(1024);
+    if (a.n > 65536)
+        hipLaunchKernelGGL((row8_long_kernel<NORM, 0>), grid, block, 0, stream, a);
+    else if (a.n > 32768) {
+        if constexpr (NORM) hipLaunchKernelGGL((row8_long_kernel<true, 16>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((row8_norm_kernel<1024, 16, false>), grid, block, 0, stream, a);
+    } else {
+        if constexpr (NORM) hipLaunchKernelGGL((row8_long_kernel<true, 8>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((row8_norm_kernel<1024, 8, false>), grid, block, 0, stream, a);
+    }
+}
+
 }  // namespace
 
 // A wave to a row up to 1024 entries, then a workgroup with four groups of four to a lane
-// (as many lanes as groups, 1024 of one each, gained 0.2 us of 4.2 at one row of 4096 and lost
-// 15 to 40% past 512 rows).  A norm's row past 1024 lanes' registers is read again for each
-// use (3.7 to 4.2 TB/s of what it cannot do without, where shorter rows have 4.5 to 5.6); the
-// registers of rows that are only held go further, for they need no 64-bit values.
+// (as many lanes as groups, 1024 of one each, gained 0.2 us at one row of 4096 and lost 15 to
+// 40% past 512 rows).  Past 16384 entries a norm's row is read twice, its 64-bit values leaving
+// no registers for it; past 65536 every row three times, or two where nothing is normed.
 hipError_t launch_row8_norm(const Row8Norm& whole, hipStream_t stream) {
     constexpr int SLICE = 1 << 21;  // rows of a launch at most (a grid's threads count in 32 bits)
     for (int r0 = 0; r0 < whole.rows; r0 += std::min(SLICE, whole.rows - r0)) {
@@ -298,9 +330,8 @@ hipError_t launch_row8_norm(const Row8Norm& whole, hipStream_t stream) {
         else if (n <= 4096) launch_rows<256, 4>(a, stream);
         else if (n <= 8192) launch_rows<512, 4>(a, stream);
         else if (n <= 16384) launch_rows<1024, 4>(a, stream);
-        else if (n <= 32768 && !a.weight) hipLaunchKernelGGL((row8_norm_kernel<1024, 8, false>), dim3(a.rows), dim3(1024), 0, stream, a);
-        else if (a.weight) hipLaunchKernelGGL((row8_long_kernel<true>), dim3(a.rows), dim3(1024), 0, stream, a);
-        else hipLaunchKernelGGL((row8_long_kernel<false>), dim3(a.rows), dim3(1024), 0, stream, a);
+        else if (a.weight) launch_long<true>(a, stream);
+        else launch_long<false>(a, stream);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -9,7 +9,7 @@ from gpu_helpers import to_gpu
 pytestmark = pytest.mark.gpu
 
 # one group of four or less, the borders of the kernels' widths, odd ones, past all registers
-WIDTHS = [1, 3, 4, 31, 64, 255, 256, 257, 768, 1024, 1025, 2049, 4096, 4099, 5003, 8192, 8195, 11008, 16385, 40001, 65536, 65539]
+WIDTHS = [1, 3, 4, 31, 64, 255, 256, 257, 768, 1024, 1025, 2049, 4096, 4099, 5003, 8192, 8195, 11008, 16385, 32768, 32769, 40001, 65536, 65539]
 
 
 @pytest.fixture(scope="module", autouse=True)
