@@ -499,3 +499,34 @@ def test_refusals():
     with pytest.raises(TypeError):
         na.row8_read(codes, scales, x.half())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "codes", "scales", "residual", "sum"])
+def test_norm_refuses_each_tensor(which):
+    """Of another shape, type, layout or place, or none where one is needed."""
+    import torch
+
+    import nitrorag_amd as na
+
+    x = torch.zeros((3, 64), device="cuda")
+    good = {"x": x, "weight": x[0], "codes": torch.zeros((3, 64), dtype=torch.int8, device="cuda"),
+            "scales": torch.zeros(3, device="cuda"), "residual": x, "sum": x}
+    na.rms_norm_row8(**good)
+    t = good[which]
+    shapes = [t[:-1].contiguous(), t[None], t.new_zeros(0)]
+    for wrong in shapes:
+        with pytest.raises(na.NitroError):
+            na.rms_norm_row8(**{**good, which: wrong})
+    strided = t.new_zeros((*t.shape, 2))[..., 0]
+    for wrong in [t.cpu(), t.double(), strided, t.cpu().numpy(), 3] + [None] * (which not in ("residual", "sum")):
+        with pytest.raises(TypeError):
+            na.rms_norm_row8(**{**good, which: wrong})
+    if which in ("x", "codes", "scales"):
+        given = {"x": x, "codes": good["codes"], "scales": good["scales"]}
+        for call in (na.row8_quantize, na.row8_read):
+            for wrong in shapes:
+                with pytest.raises(na.NitroError):
+                    call(**{**given, which: wrong})
+            for wrong in (t.cpu(), strided, None):
+                with pytest.raises(TypeError):
+                    call(**{**given, which: wrong})
