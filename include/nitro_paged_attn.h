@@ -379,7 +379,8 @@ int nitro_q8_tile_rows(int32_t launch, int32_t batch, int32_t n, int32_t d, int3
  * fp32, the product exact, ties to even); the value is code * scale.  Rows with a <
  * 2^-100 are held as zeros.  A row with an infinity or a NaN in it gets a NaN for its
  * scale and zeros for codes: all that is computed from it is NaN, and nothing else is.
- *   codes: device int8 [rows][n]; scales: device fp32 [rows].  Rows of any n > 0. */
+ *   codes: device int8 [rows][n]; scales: device fp32 [rows].  Rows of any n from 1 to
+ * 2^30, at any address (floats 4-byte aligned). */
 
 /* codes, scales = rms_norm (src/model_q8.cpp:128-140) of x [rows][n], held:
  *   h = x + residual (fp32; residual may be NULL)
@@ -392,8 +393,8 @@ int nitro_row8_quantize(const float* x, int8_t* codes, float* scales, int32_t ro
 int nitro_row8_read(const int8_t* codes, const float* scales, float* x, int32_t rows, int32_t n, void* stream);
 
 /* A Q8_0 matrix laid out for such rows: w is device BlockQ8 rows (d rows of n / 32
- * blocks, 4-byte aligned), n a multiple of 32; a copy of 1.125 bytes a weight is made
- * (the caller may free w).  With w_gate, of the same shape, the pair computes
+ * blocks, 4-byte aligned), n a multiple of 32 up to 2^30, d up to 2^29; a copy of
+ * 1.125 bytes a weight is made (the caller may free w; the call waits for the device).  With w_gate, of the same shape, the pair computes
  * act(w_gate . x) * (w . x).  Used on the device that was current at its creation. */
 typedef struct nitro_q8_weights nitro_q8_weights;
 int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_t d, nitro_q8_weights** out);
