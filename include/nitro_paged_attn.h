@@ -394,8 +394,8 @@ int nitro_row8_read(const int8_t* codes, const float* scales, float* x, int32_t 
 
 /* A Q8_0 matrix laid out for such rows: w is device BlockQ8 rows (d rows of n / 32
  * blocks, 4-byte aligned), n a multiple of 32 up to 2^30, d up to 2^29; a copy of
- * 1.125 bytes a weight is made (the caller may free w; the call waits for the device).  With w_gate, of the same shape, the pair computes
- * act(w_gate . x) * (w . x).  Used on the device that was current at its creation. */
+ * 1.125 bytes a weight is made (the caller may free w; the call waits for the device).
+ * With w_gate, of the same shape, the pair computes act(w_gate . x) * (w . x).  Used on the device that was current at its creation. */
 typedef struct nitro_q8_weights nitro_q8_weights;
 int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_t d, nitro_q8_weights** out);
 int nitro_q8_weights_destroy(nitro_q8_weights* weights);
