@@ -14,10 +14,16 @@ from .attention import _torch_module
 from .q8 import BLOCK, BLOCK_BYTES
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+_INT32 = (1 << 31) - 1  # (ctypes takes a larger number's low 32 bits without a word)
 
 
 def _refuse(func: str, message: str):
     raise N.NitroError(N.INVALID_ARGUMENT, func, message)
+
+
+def _refuse_sizes(func: str, rows: int, n: int):
+    raise N.NitroError(N.UNSUPPORTED, func,
+                       "rows of more than 2^30 entries" if n > _INT32 else "more than 2^31 - 1 rows")
 
 
 _bound = None
@@ -83,6 +89,8 @@ def rms_norm_row8(x, weight, codes, scales, residual=None, sum=None, eps: float 
     if not good:
         _check_call("rms_norm_row8", codes, scales, dev, lambda rows, n: (
             ("x", _missing(x), (rows, n)), ("residual", residual, (rows, n)), ("weight", _missing(weight), (n,)), ("sum", sum, (rows, n))))
+    if rows | n > _INT32:
+        _refuse_sizes("rms_norm_row8", rows, n)
     N.call("nitro_rms_norm_row8", x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), eps,
            None if sum is None else sum.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, n,
            raw_stream(dev) if stream is None else stream.cuda_stream)
@@ -101,6 +109,8 @@ def _rows_and_values(func: str, x, codes, scales, stream):
         good = False
     if not good:
         _check_call(func, codes, scales, dev, lambda rows, n: (("x", _missing(x), (rows, n)),))
+    if rows | n > _INT32:
+        _refuse_sizes(func, rows, n)
     return (x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, n,
             raw_stream(dev) if stream is None else stream.cuda_stream)
 
@@ -133,6 +143,8 @@ class Q8Weights:
         self.d = w.shape[0]
         self.n = w.numel() // self.d // BLOCK_BYTES * BLOCK
         self.gated = up is not None
+        if self.n > 1 << 30 or self.d > 1 << 29:
+            raise N.NitroError(N.UNSUPPORTED, "Q8Weights", "more than 2^30 columns or 2^29 rows")
         h = ctypes.c_void_p()
         N.call("nitro_q8_weights_create", (up if self.gated else w).data_ptr(), w.data_ptr() if self.gated else None,
                self.n, self.d, ctypes.byref(h))
@@ -160,6 +172,8 @@ class Q8Weights:
                 ("bias", bias, (wide,)), ("residual", residual, (rows, d)), ("out", _missing(out), (rows, d))))
         if n != self.n:
             _refuse("Q8Weights.matmul", f"the rows have {n} entries, the weights {self.n}")
+        if rows > _INT32:
+            _refuse_sizes("Q8Weights.matmul", rows, n)
         act = ACTIVATIONS.get(activation)
         if act is None:
             _refuse("Q8Weights.matmul", f"activation must be one of {', '.join(ACTIVATIONS)}")
