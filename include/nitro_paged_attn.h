@@ -416,6 +416,11 @@ enum {
  * calls on one matrix may overlap. */
 int nitro_row8_matmul(const nitro_q8_weights* weights, const int8_t* codes, const float* scales, const float* bias,
                       const float* residual, float* out, int32_t rows, int32_t activation, void* stream);
+/* Which kernel takes such a product on the current device: a workgroup owns tile[0] rows x
+ * tile[1] weight rows (of a pair half of them each matrix's), and tile[2] waves split a
+ * row's blocks (1: none; the kernel for many rows).  gated: a pair; d_kv > 0: a model's
+ * wq, wk and wv (d rows and twice d_kv).  Past 2^20 rows, the first 2^20's.  Needs no GPU. */
+int nitro_row8_tile(int32_t rows, int32_t n, int32_t d, int32_t d_kv, int32_t gated, int32_t* tile);
 
 /* ------------------------ transformer step (model) -------------------------
  * The forward passes of src/model_q8.cpp around the attention path, on the

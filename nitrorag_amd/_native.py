@@ -109,6 +109,7 @@ SIGNATURES = {
     "nitro_q8_weights_create": [_vp, _vp, _i32, _i32, ctypes.POINTER(_vp)],
     "nitro_q8_weights_destroy": [_vp],
     "nitro_row8_matmul": [_vp, _vp, _fp, _fp, _fp, _fp, _i32, _i32, _vp],
+    "nitro_row8_tile": [_i32, _i32, _i32, _i32, _i32, _i32p],
     "nitro_model_create": [_vp, ctypes.c_uint64, ctypes.POINTER(_vp)],
     "nitro_model_destroy": [_vp],
     "nitro_model_config": [_vp, _i32p],

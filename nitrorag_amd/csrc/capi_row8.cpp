@@ -126,4 +126,19 @@ int nitro_row8_matmul(const nitro_q8_weights* weights, const int8_t* codes, cons
     });
 }
 
+int nitro_row8_tile(int32_t rows, int32_t n, int32_t d, int32_t d_kv, int32_t gated, int32_t* tile) {
+    return guarded([&] {
+        require(tile != nullptr, ERR_INVALID_ARGUMENT, "null output pointer");
+        require(rows > 0 && n > 0 && d > 0 && d_kv >= 0 && n % 32 == 0, ERR_INVALID_ARGUMENT,
+                "rows, n and d must be positive, d_kv not negative, n a multiple of 32");
+        require(n <= 1 << 30 && d <= 1 << 29 && d_kv <= 1 << 29, ERR_UNSUPPORTED, "more than 2^30 columns or 2^29 rows");
+        require(!gated || d_kv == 0, ERR_INVALID_ARGUMENT, "a pair has no d_kv");
+        Row8Matmul a{};
+        a.d[0] = d, a.d[1] = a.d[2] = d_kv;
+        a.mats = d_kv ? 3 : 1, a.gated = gated != 0;
+        a.rows = rows, a.n = n;
+        require(row8_matmul_tile(a, tile), ERR_UNSUPPORTED, "no kernel takes a product of these sizes");
+    });
+}
+
 }  // extern "C"

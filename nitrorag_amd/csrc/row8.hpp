@@ -42,5 +42,7 @@ struct Row8Matmul {
     int32_t rows, n, activation;
 };
 hipError_t launch_row8_matmul(const Row8Matmul& a, hipStream_t stream);
+// nitro_row8_tile: of a's sizes (rows, n, d, mats, gated); false where no kernel takes them.
+bool row8_matmul_tile(const Row8Matmul& a, int32_t* tile);
 
 }  // namespace nitro

@@ -648,10 +648,33 @@ float estimate(const Form& f, const Row8Matmul& a, const Tiles& t, int cus) {
 // Rows of one launch at most.
 constexpr int SLICE = 1 << 20;
 
+// The form with the least estimate (null: none takes the launch), and its tiles.
+const Form* chosen_form(const Row8Matmul& a, Tiles& tiles) {
+    const int cus = device_cus();
+    const Form* best = nullptr;
+    float least = 0.0f;
+    for (const Form& f : FORMS) {
+        Tiles t;
+        if (!tiles_of(f, a, t)) continue;
+        const float us = estimate(f, a, t, cus);
+        if (!best || us < least) best = &f, least = us, tiles = t;
+    }
+    return best;
+}
+
 }  // namespace
 
+bool row8_matmul_tile(const Row8Matmul& whole, int32_t* tile) {
+    Row8Matmul a = whole;
+    a.rows = std::min(SLICE, whole.rows);
+    Tiles tiles{};
+    const Form* f = chosen_form(a, tiles);
+    if (!f) return false;
+    tile[0] = 1 << f->rows, tile[1] = 1 << f->cols, tile[2] = 1 << f->split;
+    return true;
+}
+
 hipError_t launch_row8_matmul(const Row8Matmul& whole, hipStream_t stream) {
-    const int cus = device_cus();
     for (int r0 = 0; r0 < whole.rows; r0 += std::min(SLICE, whole.rows - r0)) {
         Row8Matmul a = whole;
         a.rows = std::min(SLICE, whole.rows - r0);
@@ -659,15 +682,8 @@ hipError_t launch_row8_matmul(const Row8Matmul& whole, hipStream_t stream) {
         a.scales += r0;
         if (a.residual) a.residual += (size_t)r0 * a.d[0];
         for (int m = 0; m < a.mats; m++) a.out[m] += (size_t)r0 * a.d[m];
-        const Form* best = nullptr;
         Tiles tiles{};
-        float least = 0.0f;
-        for (const Form& f : FORMS) {
-            Tiles t;
-            if (!tiles_of(f, a, t)) continue;
-            const float us = estimate(f, a, t, cus);
-            if (!best || us < least) best = &f, least = us, tiles = t;
-        }
+        const Form* best = chosen_form(a, tiles);
         if (!best) return hipErrorInvalidConfiguration;
         best->launch(a, tiles, stream);
         const hipError_t e = hipGetLastError();

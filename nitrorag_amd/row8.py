@@ -126,6 +126,16 @@ def row8_read(codes, scales, x, stream=None) -> None:
     N.call("nitro_row8_read", pc, ps, px, rows, n, s)
 
 
+def product_tile(rows: int, n: int, d: int, d_kv: int = 0, gated: bool = False) -> tuple:
+    """(rows, weight rows, waves that split the blocks) of the kernel that takes a product of
+    8-bit rows, a gated pair's or a model's wq, wk and wv (nitro_row8_tile)."""
+    if max(rows, n, d, d_kv) > _INT32:
+        raise N.NitroError(N.UNSUPPORTED, "product_tile", "sizes past 2^31 - 1")
+    tile = (ctypes.c_int32 * 3)()
+    N.call("nitro_row8_tile", rows, n, d, d_kv, gated, tile)
+    return tuple(tile)
+
+
 class Q8Weights:
     """A Q8_0 matrix w (uint8 GPU tensor, d rows of n / 32 BlockQ8) laid out for products
     with 8-bit rows, or with two matrices the gated pair: Q8Weights(gate, up) computes
