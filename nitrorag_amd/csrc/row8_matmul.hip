@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
     constexpr int PLANE = BM * 16 + 32;  // (the planes' banks lie 32 bytes apart: a row's four runs are written together)
     constexpr int XB = 2 * STEP * PLANE, WB = STEP * BN * 32, BUF = XB + WB + STEP * BN * 4;
-    constexpr int XU = MT * STEP / 2, WU = NT * STEP / 2, SU = (STEP * BN + 255) / 256;  // units a thread
+    constexpr int XU = MT * STEP / 2, WU = NT * STEP / 2, SU = STEP * BN / 256;  // units a thread
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
     __shared__ __attribute__((aligned(16))) float row_scales[BM];
     const int tid = threadIdx.x;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
         return a.w[GATED ? j / 2 % 2 : member] + (size_t)min(at, tiles - 1) * nb * Q8_TILE_BYTES;
     };
     // Staging: x and weights in units of 16 bytes, scales one by one.
-    constexpr bool EVEN = STEP * BN % 256 == 0;  // every thread has its scales
+    static_assert(STEP * BN % 256 == 0, "every thread has its scales");
     const int8_t* xp[XU];
     int xdst[XU];
     const int xk = tid % (2 * STEP) * 16;
@@ -381,8 +381,7 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
             S.w[u] = *reinterpret_cast<const i4*>(wp[u] + (size_t)min(blk + wblk[u], nb - 1) * Q8_TILE_BYTES);
 #pragma unroll
         for (int u = 0; u < SU; u++)
-            if (EVEN || tid < STEP * BN)
-                S.s[u] = *reinterpret_cast<const float*>(sp[u] + (size_t)min(blk + sblk[u], nb - 1) * Q8_TILE_BYTES);
+            S.s[u] = *reinterpret_cast<const float*>(sp[u] + (size_t)min(blk + sblk[u], nb - 1) * Q8_TILE_BYTES);
     };
     auto put = [&](const Stage& S, int buf, int blk) __attribute__((always_inline)) {
 #pragma unroll
@@ -391,8 +390,7 @@ __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles
         for (int u = 0; u < WU; u++) *reinterpret_cast<i4*>(wl(buf) + (tid + 256 * u) * 16) = S.w[u];
         // (a block past the end repeats the last one, times 0)
 #pragma unroll
-        for (int u = 0; u < SU; u++)
-            if (EVEN || tid < STEP * BN) sl(buf)[tid + 256 * u] = blk + sblk[u] < nb ? S.s[u] : 0.0f;
+        for (int u = 0; u < SU; u++) sl(buf)[tid + 256 * u] = blk + sblk[u] < nb ? S.s[u] : 0.0f;
     };
 
     f16v acc[MT][NT];
