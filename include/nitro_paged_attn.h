@@ -395,7 +395,8 @@ int nitro_row8_read(const int8_t* codes, const float* scales, float* x, int32_t 
 /* A Q8_0 matrix laid out for such rows: w is device BlockQ8 rows (d rows of n / 32
  * blocks, 4-byte aligned), n a multiple of 32 up to 2^30, d up to 2^29; a copy of
  * 1.125 bytes a weight is made (the caller may free w; the call waits for the device).
- * With w_gate, of the same shape, the pair computes act(w_gate . x) * (w . x).  Used on the device that was current at its creation. */
+ * With w_gate, of the same shape, the pair computes act(w_gate . x) * (w . x).  Used on
+ * the device that was current at its creation. */
 typedef struct nitro_q8_weights nitro_q8_weights;
 int nitro_q8_weights_create(const void* w, const void* w_gate, int32_t n, int32_t d, nitro_q8_weights** out);
 int nitro_q8_weights_destroy(nitro_q8_weights* weights);
@@ -412,8 +413,8 @@ enum {
  * of a gated pair out = act(p_gate + bias[i]) * (p + bias[d + i]) + residual.
  * codes [rows][n] 16-byte aligned, bias [d] ([2][d] of a pair) or NULL, residual and out
  * [rows][d] fp32 (residual NULL, or out itself).  The sums over t are exact integers,
- * those over j fp32, in an order that depends on rows, n and d only.  Allocates nothing;
- * calls on one matrix may overlap. */
+ * those over j fp32, in an order that depends on rows, n, d, whether it is a pair, and the
+ * device's number of compute units.  Allocates nothing; calls on one matrix may overlap. */
 int nitro_row8_matmul(const nitro_q8_weights* weights, const int8_t* codes, const float* scales, const float* bias,
                       const float* residual, float* out, int32_t rows, int32_t activation, void* stream);
 /* Which kernel takes such a product on the current device: a workgroup owns tile[0] rows x

@@ -1,9 +1,10 @@
 // Products of 8-bit rows with Q8_0 matrices for gfx950 (row8.hpp):
 //   p[b][i] = xs[b] * sum_j ws[i][j] * (sum_t wq[i][32j + t] * xq[b][32j + t])
 //   out[b][i] = act(p + bias[i]) [* (p' + bias'[i])] + residual[b][i]
-// The inner sums are exact integers (at most 32 * 127 * 128) on the integer matrix cores,
-// and exact in fp32 (24 bits); a block of 32 k has its weight scale, so each takes one
-// conversion and one fma into fp32 sums.  The row's scale comes in once, at the end.
+// The inner sums are exact integers (at most 32 * 128 * 128: codes and weights may be -128)
+// on the integer matrix cores, and exact in fp32 (24 bits); a block of 32 k has its weight
+// scale, so each takes one conversion and one fma into fp32 sums.  The row's scale comes in
+// once, at the end.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,19 +22,22 @@ typedef int i16 __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-// exp and the quotient by the hardware's 2^x and 1 / x: a few roundings of the result, and
-// one of the exponent's argument times it, as expf and a division have.  (NaN goes through
-// all of the activations; a quotient by an infinity is 0.)  They are a tile's whole time where
-// n is small: 8192 rows of 768 x 2048 with gelu 49 us, 63 through erfcf; 4637 rows of 32 x
-// 5522 31 us, with gelu_tanh 34, gelu 38, and 51 and 52 through expf, erfcf and divisions.
+// exp and the quotient by the hardware's 2^x and 1 / x: a few roundings of the result, and as
+// many of the exponent's argument as that is large: its rounding moves 2^t by t of them, which
+// expf does not let grow.  Past t = 126 the quotient may be 0 where the result is below 1e-35.
+// (NaN goes through all of the activations; a quotient by an infinity is 0.)  They are a tile's
+// whole time where n is small: 8192 rows of 768 x 2048 with gelu 49 us, 63 through erfcf; 4637
+// rows of 32 x 5522 31 us, with gelu_tanh 34, gelu 38, and 51 and 52 through expf, erfcf and
+// divisions.
 __device__ __forceinline__ float logistic_of(float x, float t) {  // x / (1 + 2^t)
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
 __device__ __forceinline__ float relu(float x) { return x < 0.0f ? 0.0f : x; }
 __device__ __forceinline__ float silu(float x) { return logistic_of(x, x * -1.4426950408889634f); }
-// x Phi(x), with Phi(-|x|) = exp(-x^2 / 2) t Q(t), t = 1 / (1 + 0.35 |x|): Q is the polynomial
-// of degree 8 with the least relative error for |x| <= 14.5 (3.2e-8, half a rounding), a
-// weighted least-squares fit in 64 bits; in fp32 at most 7 roundings of 1 + x^2.
+// x Phi(x), with Phi(-|x|) = exp(-x^2 / 2) t Q(t), t = 1 / (1 + 0.35 |x|): Q is a polynomial of
+// degree 8, fitted in 64 bits by least squares, its weights raised where the relative error was
+// largest until that stayed below 3.2e-8 for |x| <= 14.5 (where Phi(-|x|) leaves fp32); 5.4e-8,
+// a rounding, with the coefficients in fp32.  The whole is off by at most 7 (1 + x^2) roundings.
 __device__ __forceinline__ float gelu(float x) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(x), 1.0f));
     float q = -0.029157886f;
@@ -310,9 +314,10 @@ __global__ __launch_bounds__(64 * W, OCC) void row8_split_kernel(Row8Matmul a, T
 // cycles of a SIMD, next to the matrix instruction's 32.  4096 rows of 11008 x 4096: 390 to 425
 // us, 870 to 950 TFLOP/s, with the vector unit busy for 86 to 89% of the cycles; 1024 rows of a gated
 // 4096 x 11008 pair 215 to 230 us, 800 to 860.  (The codes as halves, whose sums need no
-// conversion, took 387 us where this took 374 in the same run: two matrix instructions a block,
-// and a lower clock.)  512 rows of 4096 x 4096, 32 us, 540 TFLOP/s: few workgroups a CU, and
-// each waits for its loads.
+// conversion but two matrix instructions a block, took 387 us where this took 374 in the same run,
+// with the two back to back and the fma behind them: 148 cycles of a SIMD for a tile and block, of
+// which either unit has work for 64.  Other orders of them were not measured.)  512 rows of
+// 4096 x 4096, 32 us, 540 TFLOP/s: few workgroups a CU, and each waits for its loads.
 template <int MT, int NT, int STEP, int DEPTH, int OCC, bool GATED>
 __global__ __launch_bounds__(256, OCC) void row8_gemm_kernel(Row8Matmul a, Tiles tiling) {
     constexpr int BM = 64 * MT, BN = 64 * NT, COLS = GATED ? BN / 2 : BN;
@@ -606,7 +611,7 @@ constexpr Form gemm_form(int resident, float fixed, float alone, float busy) {
 // Each timed over 420 shapes (1 to 8192 rows, n from 32 to 16384, d from 16 to 16384, gated
 // or not) as graph replays, and fitted to within 4 to 8% of its own times.  The choice by
 // these estimates takes 1.2% longer in the mean than the best of the forms each time; at
-// most 23%, 7.1 against 5.8 us, for a gated pair of 9588 rows of 32.  (Two of the forms are the
+// most 23%, 7.1 against 5.8 us, for 35 rows and a gated pair of 9588 x 32.  (Two of the forms are the
 // least only for pairs.)
 constexpr Form FORMS[] = {
     split_form<16, 1, 1, 4, 5>(8, 2.23f, 0.313f, 0.282f),
