@@ -448,7 +448,12 @@ int nitro_row8_tile(int32_t rows, int32_t n, int32_t d, int32_t d_kv, int32_t ga
  * (NITRO_Q8_FULL_ROWS).  NITRO_Q8_ROW8, which the reference lacks, is full rows with each
  * product's input held in 8 bits ("rows held in 8 bits" above): rms_norm's output, the
  * attention's and SwiGLU's; its first forward of any size allocates the tile-layout copy.
- * The classifier is fp32 in all. */
+ * The classifier is fp32 in all.
+ *
+ * Captured forwards: a forward's buffers belong to the model and are sized by the most rows
+ * of any so far.  Before a capture a forward of as many rows, with the same semantics and
+ * kind of pool, is run eagerly.  A later forward of more rows than any before moves the
+ * buffers; forwards captured until then are not replayed after it. */
 typedef struct nitro_model nitro_model;
 int nitro_model_create(const void* blob, uint64_t bytes, nitro_model** out);
 int nitro_model_destroy(nitro_model* model);
